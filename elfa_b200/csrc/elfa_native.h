@@ -240,6 +240,18 @@ int elfa_gpt_stream(const unsigned long long* p, const long long* dims, float ep
 int elfa_efla_stream_work(const long long* dims, int step_tokens);
 int elfa_efla_stream(const unsigned long long* p, const long long* dims, const float* forget, float eps, int step_tokens, void* stream);
 
+// ---- paged_decode.cu, pages.cu, sample.cu --------------------------------------------------------
+int elfa_paged_attention_scratch(int N, int page, int H, int Hkv, int hd, int max_new);
+int elfa_paged_attention(const void* q, long long qs, const void* pages, const int* table, const int* q_start, const int* kv_len, void* out,
+                         float* scratch, int B, int N, int P, int page, int T, int H, int Hkv, int hd, int max_new, int window, int sinks,
+                         float scale, void* stream);
+int elfa_paged_write(const void* k, long long ks, const void* v, long long vs, void* pages, const int* table, const int* q_start,
+                     const int* kv_len, int B, int N, int P, int page, int T, int Hkv, int hd, void* stream);
+int elfa_copy_pages(void* pages, long long layer_bytes, long long page_bytes, int L, int P, const int* from, const int* to, int n, void* stream);
+int elfa_sample(const void* logits, int type, long long ld, const float* noise, long long ldn, const float* temperature, const int* top_k,
+                const float* top_p, const float* min_p, float temperature_all, int top_k_all, float top_p_all, float min_p_all, long long* out,
+                int B, int V, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

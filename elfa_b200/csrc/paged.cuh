@@ -1,0 +1,256 @@
+// What the kernels over a paged key / value cache share: the geometry of a call and how its work is cut.
+//
+// pages [P, 2, Hkv, page, hd] bf16; table [B, N] int32 names the pages of each sequence in order (negative: absent); sequence b brings the new
+// tokens q_start[b] .. q_start[b + 1] of the call and has kv_len[b] tokens with them, so its i-th new token stands at kv_len - n + i. A query at
+// `pos` sees the keys that lie in pages that are there and for which key <= pos and (key > pos - window or key < sinks).
+//
+// Work is counted in units: one tile of query rows (rows are (token, head of the group) pairs, token first, so a key is read once for all heads
+// that share it) against one block of keys. The units of all (sequence, tile, key head) items stand in one line, blocks innermost, and CTA c
+// of G takes c W / G up to (c + 1) W / G of them: every CTA gets the same number whatever the sequences' lengths are, and the host needs to know none of
+// them. An item that a CTA does not hold whole leaves a partial result: slot 2 c + 1 for the part that begins it, slot 2 c for a later part.
+#pragma once
+#include "common.cuh"
+
+namespace elfa {
+
+constexpr int PAGED_MAX_SEQS = 1024;       // per launch; the Python side cuts larger batches
+
+struct PagedGeom {
+  const int *table, *q_start, *kv_len;
+  int B, N, P, page_shift, T, max_new;     // T: rows of q; max_new: the most new tokens that the host has planned for
+  int H, Hkv, rep, hd;
+  int window, sinks;                       // window 0: none
+  int tile_rows;                           // query rows of a tile
+  unsigned int* status;
+};
+
+struct PagedSeq {
+  int q0, n, kv;                           // first new token, new tokens, tokens with them
+};
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedGeom& g, int b) {
+  const int a = g.q_start[b], e = g.q_start[b + 1], kv = g.kv_len[b];
+  const long long most = (long long)g.N << g.page_shift;
+  PagedSeq s;
+  s.q0 = min(max(a, 0), g.T);
+  s.n = min(max(e, s.q0), g.T) - s.q0;
+  s.kv = (int)min((long long)max(kv, 0), min(most, 0x7fffff00LL));
+  if (s.q0 != a || s.q0 + s.n != e || s.kv != kv || s.n > s.kv || s.n > g.max_new) atomicOr(g.status, (unsigned)ELFA_ST_BAD_PAGE);
+  return s;
+}
+__device__ __forceinline__ int paged_tiles(const PagedGeom& g, const PagedSeq& s) {
+  return (s.n * g.rep + g.tile_rows - 1) / g.tile_rows;
+}
+
+// key blocks that the rows of a tile see: i < ns is block i (sinks), later ones are w0 + i - ns. A tile that sees nothing still has one block.
+struct PagedSpan {
+  int ns, w0, n;
+  __device__ __forceinline__ int block(int i) const { return i < ns ? i : w0 + i - ns; }
+};
+template <int BLK>
+__device__ __forceinline__ PagedSpan paged_span(const PagedGeom& g, const PagedSeq& s, int t) {
+  const int r0 = t * g.tile_rows, lo_tok = r0 / g.rep, hi_tok = (min(r0 + g.tile_rows, s.n * g.rep) - 1) / g.rep;
+  const int pos0 = s.kv - s.n, hi = max(pos0 + hi_tok + 1, 0);
+  const int lo = g.window ? max(0, pos0 + lo_tok - g.window + 1) : 0;
+  PagedSpan p;
+  p.w0 = lo / BLK;
+  p.ns = g.window ? min((min(g.sinks, hi) + BLK - 1) / BLK, p.w0) : 0;
+  p.n = max(p.ns + (hi + BLK - 1) / BLK - p.w0, 1);
+  return p;
+}
+
+// units of a sequence (all tiles, all key heads); `lane` of `lanes` threads adds up every lanes-th tile
+template <int BLK>
+__device__ __forceinline__ long long paged_units(const PagedGeom& g, const PagedSeq& s, int lane, int lanes) {
+  const int tiles = paged_tiles(g, s);
+  long long u = 0;
+  for (int t = lane; t < tiles; t += lanes) u += paged_span<BLK>(g, s, t).n;
+  return u * g.Hkv;
+}
+
+// prefix[b] = units before sequence b, prefix[B] = W, by all threads of the block (ends with a barrier). wide: a warp per sequence (many tiles each).
+template <int BLK, int THREADS>
+__device__ __forceinline__ void paged_prefix(const PagedGeom& g, long long* prefix, long long* warp_tot, bool wide) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int WARPS = THREADS / 32;
+  if (wide) {
+    for (int b = warp; b < g.B; b += WARPS) {
+      const PagedSeq s = paged_seq(g, b);
+      long long u = paged_units<BLK>(g, s, lane, 32);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+      if (lane == 0) prefix[b + 1] = u;
+    }
+    __syncthreads();
+  }
+  long long run = 0;
+  for (int b0 = 0; b0 < g.B; b0 += THREADS) {
+    const int b = b0 + threadIdx.x;
+    long long u = 0;
+    if (b < g.B) u = wide ? prefix[b + 1] : paged_units<BLK>(g, paged_seq(g, b), 0, 1);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, u, o);
+      if (lane >= o) u += v;
+    }
+    if (lane == 31) warp_tot[warp] = u;
+    __syncthreads();
+    long long before = run;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) before += warp_tot[w];
+      run += warp_tot[w];
+    }
+    if (b < g.B) prefix[b + 1] = before + u;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) prefix[0] = 0;
+  __syncthreads();
+}
+
+struct PagedItem {
+  int b, t, h;
+  PagedSeq s;
+  PagedSpan span;
+  long long u0;                            // unit of its block 0
+  int tiles;
+};
+
+// the item that unit u belongs to; all lanes of a warp call it together
+template <int BLK>
+__device__ __forceinline__ PagedItem paged_find(const PagedGeom& g, const long long* prefix, long long u) {
+  int lo = 0, hi = g.B;                    // prefix[lo] <= u < prefix[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= u) lo = mid;
+    else hi = mid;
+  }
+  PagedItem it;
+  it.b = lo;
+  it.s = paged_seq(g, lo);
+  it.tiles = paged_tiles(g, it.s);
+  const int lane = threadIdx.x & 31;
+  long long base = prefix[lo];
+  it.t = 0;
+  if (it.tiles > 1) {
+    for (int t0 = 0;; t0 += 32) {
+      const int t = t0 + lane;
+      const long long mine = t < it.tiles ? (long long)paged_span<BLK>(g, it.s, t).n * g.Hkv : 0;
+      long long incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, base + incl > u && t < it.tiles);
+      if (hit || t0 + 32 >= it.tiles) {
+        const int l = hit ? __ffs(hit) - 1 : it.tiles - 1 - t0;
+        it.t = t0 + l;
+        base += __shfl_sync(0xffffffffu, incl - mine, l);
+        break;
+      }
+      base += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+  it.span = paged_span<BLK>(g, it.s, it.t);
+  it.h = (int)((u - base) / it.span.n);
+  it.u0 = base + (long long)it.h * it.span.n;
+  return it;
+}
+// the next item in line (there is one as long as its first unit is below W)
+template <int BLK>
+__device__ __forceinline__ void paged_next(const PagedGeom& g, PagedItem& it) {
+  it.u0 += it.span.n;
+  if (++it.h < g.Hkv) return;
+  it.h = 0;
+  if (++it.t >= it.tiles) {
+    it.t = 0;
+    do {
+      if (++it.b >= g.B) {                 // behind the last one
+        it.b = g.B - 1;
+        break;
+      }
+      it.s = paged_seq(g, it.b);
+      it.tiles = paged_tiles(g, it.s);
+    } while (it.tiles == 0);
+  }
+  it.span = paged_span<BLK>(g, it.s, it.t);
+}
+
+__device__ __forceinline__ long long paged_cut(long long W, int G, int c) { return c * W / G; }
+// the CTA that holds unit u
+__device__ __forceinline__ int paged_owner(long long W, int G, long long u) { return (int)(((u + 1) * G - 1) / W); }
+
+__device__ __forceinline__ bool paged_sees(const PagedGeom& g, int key, int pos) {
+  return key <= pos && (!g.window || key > pos - g.window || key < g.sinks);
+}
+// page of a key, negative when absent or outside the pool (which is recorded)
+__device__ __forceinline__ int paged_page(const PagedGeom& g, int b, int key) {
+  const int col = key >> g.page_shift;
+  if (col >= g.N) return -1;
+  const int id = g.table[(long long)b * g.N + col];
+  if (id >= g.P) {
+    atomicOr(g.status, (unsigned)ELFA_ST_BAD_PAGE);
+    return -1;
+  }
+  return id;
+}
+
+// One query row by one warp, key after key, nothing but what it sees: for rows whose result in the matrix form is not finite, which a
+// hidden value that is not finite makes of it too (0 times infinity). Lane l gets the columns l, l + 32, ...
+template <int HDP>
+__device__ __noinline__ void paged_row(const PagedGeom& g, const __nv_bfloat16* q, const __nv_bfloat16* pages, int b, int h, int pos, float scale,
+                                       float (&out)[HDP / 32]) {
+  const int lane = threadIdx.x & 31;
+  const long long head = (long long)g.hd << g.page_shift;                    // elements of one head of a page
+  const int mask = (1 << g.page_shift) - 1;
+  auto row_of = [&](int id, int key, int kv) { return pages + (((long long)id * 2 + kv) * g.Hkv + h) * head + (long long)(key & mask) * g.hd; };
+  auto score = [&](int key, bool& seen) {
+    seen = paged_sees(g, key, pos);
+    const int id = seen ? paged_page(g, b, key) : -1;
+    seen = id >= 0;
+    float a = 0.f;
+    if (seen) {
+      const __nv_bfloat16* k = row_of(id, key, 0);
+      for (int c = 0; c < g.hd; ++c) a += __bfloat162float(q[c]) * __bfloat162float(k[c]);
+    }
+    return a * scale;
+  };
+  float m = -INFINITY, l = 0.f;
+  const int lo = g.window ? max(0, pos - g.window + 1) : 0, skip = g.window ? min(min(g.sinks, lo), pos + 1) : 0;
+  const int count = pos < 0 ? 0 : skip + pos + 1 - lo;                       // visible keys: 0 .. skip, lo .. pos
+  auto key_at = [&](int i) { return i < skip ? i : lo + i - skip; };
+  for (int i = lane; i < count; i += 32) {
+    bool seen;
+    const float s = score(key_at(i), seen);
+    if (seen) m = fmaxf(m, s);                                               // a NaN score comes back with its exponential
+  }
+  m = warp_max(m);
+  const float ref = m == -INFINITY ? 0.f : m;
+  for (int x = 0; x < HDP / 32; ++x) out[x] = 0.f;
+  for (int i0 = 0; i0 < count; i0 += 32) {
+    bool seen = false;
+    const int key = i0 + lane < count ? key_at(i0 + lane) : -1;
+    float p = 0.f;
+    if (key >= 0) {
+      const float s = score(key, seen);
+      if (seen) p = expf(s - ref);
+    }
+    l += p;
+    const unsigned who = __ballot_sync(0xffffffffu, seen);
+    for (int j = 0; j < 32; ++j) {
+      const float w = __shfl_sync(0xffffffffu, p, j);
+      const int kj = __shfl_sync(0xffffffffu, key, j);
+      if (!(who >> j & 1)) continue;
+      const __nv_bfloat16* v = row_of(paged_page(g, b, kj), kj, 1);
+#pragma unroll
+      for (int x = 0; x < HDP / 32; ++x)
+        if (lane + 32 * x < g.hd) out[x] += w * __bfloat162float(v[lane + 32 * x]);
+    }
+  }
+  l = warp_sum(l);
+#pragma unroll
+  for (int x = 0; x < HDP / 32; ++x) out[x] = count == 0 || l == 0.f ? 0.f : out[x] / l;
+}
+
+}  // namespace elfa

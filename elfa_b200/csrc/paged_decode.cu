@@ -1,0 +1,483 @@
+// Attention over a paged cache for a few query rows per key head (decoding, a few proposed tokens): tiles of 16 rows on `mma.sync`.
+//
+// o = sum_j softmax_j(q k_j scale) v_j over the keys that a row sees, one pass over keys and values with a running maximum and sum. Bound by the
+// memory: every key and value is read once and meets 16 rows, 16 x 4 operations per element where the tensor cores would take hundreds. So
+// a warp fetches for itself: blocks of 32 keys by TMA into a ring of its own, three blocks deep (12 x 16 KB in flight per SM at 128-wide heads),
+// no barrier between the warps until an item ends, where their four partial results meet in shared memory. What a CTA leaves of an item
+// that others share goes to scratch in fp32; a second small launch joins those (in the order of the CTAs, so one call's result does not depend on timing).
+// The exponent's reference may lag behind the row's maximum by up to 2^8 before sums are scaled again.
+// Probabilities are rounded to bf16 for the second product (relative 2^-9 each, as the result will be); their sum is taken before that.
+#include "elfa_native.h"
+#include "mma_sync.cuh"
+#include "paged.cuh"
+
+namespace elfa {
+
+int make_paged_tmap(CUtensorMap* tm, const void* pages, long long P, int Hkv, int page, int hd, int box_rows);
+
+namespace {
+
+constexpr int DBLK = 32, DWARPS = 4, DST = 3, DROWS = 16;
+
+struct DecodeArgs {
+  PagedGeom g;
+  const __nv_bfloat16 *q, *pages;
+  __nv_bfloat16* out;
+  float *part, *stat;                  // [2 G][16][HDP], [2 G][16][2] (maximum, sum)
+  long long qs;                        // elements from a token's queries to the next one's
+  float scale;
+  int wide, whole;                     // a warp per sequence for the prefix; whole: CTA c takes item c, nothing is shared
+  int min_units;
+};
+
+template <int HDP>
+struct DecodeSmem {
+  static constexpr int NSUB = HDP / 64, HALF = NSUB * DBLK * 128, UNIT = 2 * HALF;
+  static constexpr int MERGE = DWARPS * DST * UNIT;                  // [2][16][HDP] fp32
+  static constexpr int STAT = MERGE + 2 * DROWS * HDP * 4;           // [4][16][2]
+  static constexpr int BAR = STAT + DWARPS * DROWS * 8;
+  static constexpr int TOT = BAR + DWARPS * DST * 8;                 // warp totals, abort flag
+  static constexpr int PREFIX = TOT + DWARPS * 8 + 16;
+  static constexpr int bytes(int B) { return PREFIX + 8 * (B + 1) + 1024; }
+};
+
+__device__ __forceinline__ int decode_ctas(long long W, int grid, int min_units) {
+  const long long most = (W + min_units - 1) / min_units;
+  return (int)(most < grid ? most : grid);
+}
+
+template <int HDP>
+__global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ DecodeArgs a) {
+  using L = DecodeSmem<HDP>;
+  constexpr int NSUB = L::NSUB;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* merge = reinterpret_cast<float*>(smem + L::MERGE);
+  float2* stat = reinterpret_cast<float2*>(smem + L::STAT);
+  long long* prefix = reinterpret_cast<long long*>(smem + L::PREFIX);
+  long long* warp_tot = reinterpret_cast<long long*>(smem + L::TOT);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::TOT + DWARPS * 8);
+  const PagedGeom& g = a.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, qd = lane & 3;
+  const uint32_t ring = smem_u32(smem) + warp * DST * L::UNIT, bars = smem_u32(smem + L::BAR) + warp * DST * 8;
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tm);
+    *abort_flag = 0;
+  }
+  if (lane < DST) mbar_init(bars + 8 * lane, 1);
+  fence_barrier_init();
+  long long u_begin, u_end;
+  PagedItem first;
+  if (a.whole) {
+    first.b = blockIdx.x / g.Hkv;
+    first.h = blockIdx.x % g.Hkv;
+    first.t = 0;
+    first.s = paged_seq(g, first.b);
+    first.tiles = paged_tiles(g, first.s);
+    first.span = paged_span<DBLK>(g, first.s, 0);
+    first.u0 = u_begin = 0;
+    u_end = first.tiles ? first.span.n : 0;
+    __syncthreads();
+  } else {
+    paged_prefix<DBLK, DWARPS * 32>(g, prefix, warp_tot, a.wide);
+    const long long W = prefix[g.B];
+    const int G = decode_ctas(W, gridDim.x, a.min_units);
+    u_begin = (int)blockIdx.x < G ? paged_cut(W, G, blockIdx.x) : 0;
+    u_end = (int)blockIdx.x < G ? paged_cut(W, G, blockIdx.x + 1) : 0;
+    if (u_begin < u_end) first = paged_find<DBLK>(g, prefix, u_begin);
+  }
+  pdl_next();
+  if (u_begin >= u_end) return;
+
+  // ---- the warp's own loads: unit u_begin + warp, then every fourth
+  PagedItem pi = first;
+  long long pu = u_begin + warp;
+  const int rows_per_box = min(1 << g.page_shift, DBLK), boxes = DBLK / rows_per_box;
+  uint32_t there = 0;                                    // two bits per ring slot: which half's page is there
+  auto issue = [&](int slot) {
+    if (pu >= u_end) return;
+    while (pu >= pi.u0 + pi.span.n) paged_next<DBLK>(g, pi);
+    const int key0 = pi.span.block((int)(pu - pi.u0)) * DBLK;
+    const uint32_t bar = bars + 8 * slot, dst = ring + slot * L::UNIT;
+    if (lane == 0) mbar_expect_tx(bar, L::UNIT);
+    const int box = lane / (2 * NSUB), sub = (lane >> 1) % NSUB, kv = lane & 1;
+    const int key = key0 + box * rows_per_box;
+    const int id = box < boxes && key < pi.s.kv ? paged_page(g, pi.b, key) : -1;
+    __syncwarp();
+    if (box < boxes)                                     // an absent page is read past the pool's end, which gives zeros
+      tma_load_3d(dst + kv * L::HALF + (sub * DBLK + box * rows_per_box) * 128, &tm, sub * 64, key & ((1 << g.page_shift) - 1),
+                  id < 0 ? 2 * g.P * g.Hkv : (2 * id + kv) * g.Hkv + pi.h, bar);
+    const unsigned ok = __ballot_sync(0xffffffffu, id >= 0);
+    const uint32_t two = (ok & 1u) | ((boxes > 1 ? ok >> (2 * NSUB) & 1u : ok & 1u) << 1);
+    there = (there & ~(3u << (2 * slot))) | two << (2 * slot);
+    pu += DWARPS;
+  };
+#pragma unroll
+  for (int s = 0; s < DST; ++s) issue(s);
+
+  const float sl2 = a.scale * 1.4426950408889634f;
+  PagedItem it = first;
+  int slot = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (long long u = u_begin; u < u_end;) {
+    const long long ue = min(u_end, it.u0 + it.span.n);
+    const int r0 = it.t * DROWS, rows = min(DROWS, it.s.n * g.rep - r0), pos0 = it.s.kv - it.s.n;
+    // rows behind the last one repeat it
+    const int ra = r0 + min(gr, rows - 1), rb = r0 + min(gr + 8, rows - 1), ta = ra / g.rep, tb = rb / g.rep;
+    const int pa = pos0 + ta, pb = pos0 + tb, pos_min = pos0 + r0 / g.rep, pos_max = pos0 + (r0 + rows - 1) / g.rep;
+    uint32_t qf[HDP / 16][4];
+    {
+      const __nv_bfloat16* qa = a.q + (it.s.q0 + ta) * a.qs + (it.h * g.rep + ra - ta * g.rep) * g.hd;
+      const __nv_bfloat16* qb = a.q + (it.s.q0 + tb) * a.qs + (it.h * g.rep + rb - tb * g.rep) * g.hd;
+#pragma unroll
+      for (int kk = 0; kk < HDP / 16; ++kk) {
+        const int c = kk * 16 + qd * 2;
+        qf[kk][0] = c < g.hd ? *reinterpret_cast<const uint32_t*>(qa + c) : 0u;
+        qf[kk][1] = c < g.hd ? *reinterpret_cast<const uint32_t*>(qb + c) : 0u;
+        qf[kk][2] = c + 8 < g.hd ? *reinterpret_cast<const uint32_t*>(qa + c + 8) : 0u;
+        qf[kk][3] = c + 8 < g.hd ? *reinterpret_cast<const uint32_t*>(qb + c + 8) : 0u;
+      }
+    }
+    float o[HDP / 8][4];
+#pragma unroll
+    for (int d = 0; d < HDP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    const int lead = (int)((warp - (u - u_begin)) & (DWARPS - 1));     // this warp's first unit of the item
+    for (long long x = u + lead; x < ue; x += DWARPS) {
+      const int key0 = it.span.block((int)(x - it.u0)) * DBLK;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(bars + 8 * slot, phase, abort_flag, g.status));
+      if (!ok) break;
+      const uint32_t kbase = ring + slot * L::UNIT, vbase = kbase + L::HALF;
+      const uint32_t two = there >> (2 * slot) & 3u;
+      if (key0 + DBLK > it.s.kv) {
+        // rows of the last page that hold no token yet: whatever lies there must not meet a probability of zero
+        const int from = max(it.s.kv - key0, 0);
+        for (int i = from * 8 + lane; i < DBLK * 8; i += 32)
+#pragma unroll
+          for (int s = 0; s < NSUB; ++s)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vbase + s * DBLK * 128 + i * 16), "r"(0) : "memory");
+        fence_proxy_async();                                           // the ring's next copy into this slot comes behind
+        __syncwarp();
+      }
+      float s[4][4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < HDP / 16; ++kk)
+#pragma unroll
+        for (int np = 0; np < 2; ++np) {
+          const int key = np * 16 + (lane >> 4) * 8 + (lane & 7), chunk = (kk & 3) * 2 + (lane >> 3 & 1);
+          uint32_t b[4];
+          ldsm4(b, kbase + (kk >> 2) * DBLK * 128 + key * 128 + ((chunk ^ (key & 7)) << 4));
+          mma_bf16(s[2 * np], qf[kk], b[0], b[1]);
+          mma_bf16(s[2 * np + 1], qf[kk], b[2], b[3]);
+        }
+      const bool need = two != 3u || key0 + DBLK - 1 > pos_min || (g.window && key0 <= pos_max - g.window && key0 + DBLK > g.sinks);
+      if (need) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = key0 + n * 8 + qd * 2 + (j & 1);
+            if (!(two >> (n >> 1) & 1u) || !paged_sees(g, key, j < 2 ? pa : pb)) s[n][j] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float mx = fmaxf(fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])),
+                         fmaxf(fmaxf(s[2][2 * r], s[2][2 * r + 1]), fmaxf(s[3][2 * r], s[3][2 * r + 1])));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * sl2;
+        const bool grow = mx - m[r] > 8.f;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float mn = grow ? mx : m[r], alpha = grow ? fast_exp2(m[r] - mn) : 1.f;
+#pragma unroll
+          for (int d = 0; d < HDP / 8; ++d) {
+            o[d][2 * r] *= alpha;
+            o[d][2 * r + 1] *= alpha;
+          }
+          l[r] *= alpha;
+          m[r] = mn;
+        }
+        const float neg = m[r] == -INFINITY ? 0.f : -m[r];             // nothing seen yet: exp2(-inf) without inf - inf
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            s[n][2 * r + j] = fast_exp2(fmaf(s[n][2 * r + j], sl2, neg));
+            l[r] += s[n][2 * r + j];
+          }
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const uint32_t p[4] = {pack_bf16(s[2 * ks][0], s[2 * ks][1]), pack_bf16(s[2 * ks][2], s[2 * ks][3]),
+                               pack_bf16(s[2 * ks + 1][0], s[2 * ks + 1][1]), pack_bf16(s[2 * ks + 1][2], s[2 * ks + 1][3])};
+#pragma unroll
+        for (int dp = 0; dp < HDP / 16; ++dp) {
+          const int key = ks * 16 + (lane >> 3 & 1) * 8 + (lane & 7), chunk = (dp & 3) * 2 + (lane >> 4);
+          uint32_t b[4];
+          ldsm4_t(b, vbase + (dp >> 2) * DBLK * 128 + key * 128 + ((chunk ^ (key & 7)) << 4));
+          mma_bf16(o[2 * dp], p, b[0], b[1]);
+          mma_bf16(o[2 * dp + 1], p, b[2], b[3]);
+        }
+      }
+      __syncwarp();                                                    // every lane has read the slot
+      issue(slot);
+      if (++slot == DST) {
+        slot = 0;
+        phase ^= 1;
+      }
+    }
+
+    // ---- the four warps' results meet
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if (qd == 0) stat[warp * DROWS + gr + 8 * r] = make_float2(m[r], l[r]);
+    }
+    __syncthreads();
+    float M[2], sum[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      M[r] = -INFINITY;
+      sum[r] = 0.f;
+#pragma unroll
+      for (int w = 0; w < DWARPS; ++w) M[r] = fmaxf(M[r], stat[w * DROWS + gr + 8 * r].x);
+#pragma unroll
+      for (int w = 0; w < DWARPS; ++w) {
+        const float2 st = stat[w * DROWS + gr + 8 * r];
+        sum[r] += st.y * (st.x == -INFINITY ? 1.f : fast_exp2(st.x - M[r]));   // a NaN sum without a maximum is handed on
+      }
+      const float f = m[r] == -INFINITY ? 1.f : fast_exp2(m[r] - M[r]);
+#pragma unroll
+      for (int d = 0; d < HDP / 8; ++d) {
+        o[d][2 * r] *= f;
+        o[d][2 * r + 1] *= f;
+      }
+    }
+    auto put = [&](float* buf) {
+#pragma unroll
+      for (int d = 0; d < HDP / 8; ++d) {
+        *reinterpret_cast<float2*>(buf + gr * HDP + ((d ^ (gr & 3)) * 8) + qd * 2) = make_float2(o[d][0], o[d][1]);
+        *reinterpret_cast<float2*>(buf + (gr + 8) * HDP + ((d ^ (gr & 3)) * 8) + qd * 2) = make_float2(o[d][2], o[d][3]);
+      }
+    };
+    auto add = [&](const float* buf) {
+#pragma unroll
+      for (int d = 0; d < HDP / 8; ++d) {
+        const float2 x = *reinterpret_cast<const float2*>(buf + gr * HDP + ((d ^ (gr & 3)) * 8) + qd * 2);
+        const float2 y = *reinterpret_cast<const float2*>(buf + (gr + 8) * HDP + ((d ^ (gr & 3)) * 8) + qd * 2);
+        o[d][0] += x.x; o[d][1] += x.y; o[d][2] += y.x; o[d][3] += y.y;
+      }
+    };
+    if (warp >= 2) put(merge + (warp - 2) * DROWS * HDP);
+    __syncthreads();
+    if (warp < 2) add(merge + warp * DROWS * HDP);
+    if (warp == 1) put(merge + DROWS * HDP);                           // the half that only this warp reads
+    __syncthreads();
+    if (warp == 0) {
+      add(merge + DROWS * HDP);
+      if (u == it.u0 && ue == it.u0 + it.span.n) {
+        unsigned bad = 0;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float inv = sum[r] == 0.f ? 0.f : 1.f / sum[r];        // a row that sees nothing gives zero
+          const int tok = r ? tb : ta, head = it.h * g.rep + (r ? rb : ra) - tok * g.rep;
+          __nv_bfloat16* po = a.out + ((long long)(it.s.q0 + tok) * g.H + head) * g.hd;
+          bool finite = true;
+#pragma unroll
+          for (int d = 0; d < HDP / 8; ++d) {
+            const float x = o[d][2 * r] * inv, y = o[d][2 * r + 1] * inv;
+            finite = finite && isfinite(x) && isfinite(y);
+            if (gr + 8 * r < rows && d * 8 < g.hd) *reinterpret_cast<uint32_t*>(po + d * 8 + qd * 2) = pack_bf16(x, y);
+          }
+          const unsigned who = __ballot_sync(0xffffffffu, !finite);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) bad |= (who >> (4 * i) & 15u ? 1u : 0u) << (i + 8 * r);
+        }
+        bad &= (1u << rows) - 1u;
+        __syncwarp();
+        while (bad) {                                                  // all lanes hold the same word
+          const int r = __ffs(bad) - 1;
+          bad &= bad - 1;
+          const int tok = (r0 + r) / g.rep, head = it.h * g.rep + (r0 + r) % g.rep;
+          const long long at = it.s.q0 + tok;
+          float res[HDP / 32];
+          paged_row<HDP>(g, a.q + at * a.qs + head * g.hd, a.pages, it.b, it.h, pos0 + tok, a.scale, res);
+#pragma unroll
+          for (int x = 0; x < HDP / 32; ++x)
+            if (lane + 32 * x < g.hd) a.out[(at * g.H + head) * g.hd + lane + 32 * x] = __float2bfloat16(res[x]);
+        }
+      } else {
+        const long long ps = 2LL * blockIdx.x + (u == it.u0);
+        float* po = a.part + ps * DROWS * HDP;
+#pragma unroll
+        for (int d = 0; d < HDP / 8; ++d) {
+          if (gr < rows) *reinterpret_cast<float2*>(po + gr * HDP + d * 8 + qd * 2) = make_float2(o[d][0], o[d][1]);
+          if (gr + 8 < rows) *reinterpret_cast<float2*>(po + (gr + 8) * HDP + d * 8 + qd * 2) = make_float2(o[d][2], o[d][3]);
+        }
+        if (qd == 0) {
+          float2* st = reinterpret_cast<float2*>(a.stat) + ps * DROWS;
+          st[gr] = make_float2(M[0], sum[0]);
+          st[gr + 8] = make_float2(M[1], sum[1]);
+        }
+      }
+    }
+    u = ue;
+    if (u < u_end) paged_next<DBLK>(g, it);
+  }
+}
+
+// Block c joins the item that the cut between CTAs c and c + 1 goes through, if no earlier cut does.
+template <int HDP>
+__global__ void __launch_bounds__(128) paged_decode_join_kernel(const __grid_constant__ DecodeArgs a, int grid) {
+  extern __shared__ long long prefix[];
+  __shared__ long long warp_tot[4];
+  __shared__ unsigned bad;
+  const PagedGeom& g = a.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  paged_prefix<DBLK, 128>(g, prefix, warp_tot, a.wide);
+  const long long W = prefix[g.B];
+  const int G = decode_ctas(W, grid, a.min_units), c = blockIdx.x + 1;
+  pdl_wait();
+  if (c >= G) return;
+  const long long u = paged_cut(W, G, c);
+  const PagedItem it = paged_find<DBLK>(g, prefix, u);
+  if (u == it.u0) return;
+  const int c0 = paged_owner(W, G, it.u0), c1 = paged_owner(W, G, it.u0 + it.span.n - 1);
+  if (c0 != c - 1) return;
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  const int r0 = it.t * DROWS, rows = min(DROWS, it.s.n * g.rep - r0);
+  constexpr int PER = 128 / HDP;                                       // rows side by side
+  const int col = threadIdx.x % HDP;
+  const float2* stat = reinterpret_cast<const float2*>(a.stat);
+  for (int r = threadIdx.x / HDP; r < rows; r += PER) {
+    const long long first = (2LL * c0 + 1) * DROWS + r, step = 2LL * DROWS, rest = (2LL * (c0 + 1)) * DROWS + r;
+    float M = stat[first].x;
+    for (int i = 0; i < c1 - c0; ++i) M = fmaxf(M, stat[rest + i * step].x);
+    float2 st = stat[first];
+    float w = st.x == -INFINITY ? 1.f : fast_exp2(st.x - M), den = w * st.y, num = w * a.part[first * HDP + col];
+#pragma unroll 4
+    for (int i = 0; i < c1 - c0; ++i) {
+      st = stat[rest + i * step];
+      w = st.x == -INFINITY ? 1.f : fast_exp2(st.x - M);               // without a maximum: sums of zero, or a NaN to hand on
+      den += w * st.y;
+      num += w * a.part[(rest + i * step) * HDP + col];
+    }
+    const float v = den == 0.f ? 0.f : num / den;
+    const int tok = (r0 + r) / g.rep;
+    if (col < g.hd) {
+      a.out[((long long)(it.s.q0 + tok) * g.H + it.h * g.rep + (r0 + r) % g.rep) * g.hd + col] = __float2bfloat16(v);
+      if (!isfinite(v)) atomicOr(&bad, 1u << r);
+    }
+  }
+  __syncthreads();
+  for (int r = warp; r < rows; r += 4) {
+    if (!(bad >> r & 1u)) continue;
+    const int tok = (r0 + r) / g.rep, head = it.h * g.rep + (r0 + r) % g.rep;
+    const long long at = it.s.q0 + tok;
+    float res[HDP / 32];
+    paged_row<HDP>(g, a.q + at * a.qs + head * g.hd, a.pages, it.b, it.h, it.s.kv - it.s.n + tok, a.scale, res);
+#pragma unroll
+    for (int x = 0; x < HDP / 32; ++x)
+      if (lane + 32 * x < g.hd) a.out[(at * g.H + head) * g.hd + lane + 32 * x] = __float2bfloat16(res[x]);
+  }
+}
+
+constexpr int WHOLE_KEYS = 256, MIN_UNITS = 4;
+
+int decode_grid(int hd) { return 148 * (hd <= 64 ? 2 : 1); }
+bool decode_whole(int max_new, int rep, long long most_keys) { return (long long)max_new * rep <= DROWS && most_keys <= WHOLE_KEYS; }
+
+template <int HDP>
+int launch_decode(DecodeArgs& a, int page, cudaStream_t st) {
+  CUtensorMap tm;
+  const int rc = make_paged_tmap(&tm, a.pages, a.g.P, a.g.Hkv, page, a.g.hd, page < DBLK ? page : DBLK);
+  if (rc != ELFA_OK) return rc;
+  const int smem = DecodeSmem<HDP>::bytes(a.whole ? 0 : a.g.B);
+  ELFA_CUDA(allow_shared<paged_decode_kernel<HDP>>(DecodeSmem<HDP>::bytes(PAGED_MAX_SEQS)));
+  const int grid = a.whole ? a.g.B * a.g.Hkv : decode_grid(a.g.hd);
+  paged_decode_kernel<HDP><<<grid, DWARPS * 32, smem, st>>>(tm, a);
+  ELFA_CUDA(cudaGetLastError());
+  ::elfa::count_launches(1);
+  if (a.whole) return ELFA_OK;
+  PdlScope scope(true);
+  ELFA_CUDA(launch_chain(paged_decode_join_kernel<HDP>, dim3(grid - 1), dim3(128), 8 * (a.g.B + 1), st, 1, a, grid));
+  ELFA_CUDA(cudaGetLastError());
+  ::elfa::count_launches(1);
+  return ELFA_OK;
+}
+
+}  // namespace
+
+// Pages as [P * 2 * Hkv][page][hd]: a box is `box_rows` tokens of one page and head, 64 columns.
+int make_paged_tmap(CUtensorMap* tm, const void* pages, long long P, int Hkv, int page, int hd, int box_rows) {
+  const uint64_t dims[3] = {(uint64_t)hd, (uint64_t)page, (uint64_t)(2 * P * Hkv)};
+  const uint64_t strides[2] = {(uint64_t)hd * 2, (uint64_t)hd * page * 2};
+  const uint32_t box[3] = {64, (uint32_t)box_rows, 1};
+  return make_tmap_nd_bf16(tm, pages, 3, dims, strides, box);
+}
+
+// Checks that both forms of the attention share, and the geometry.
+int paged_geom(PagedGeom* g, const void* pages, const int* table, const int* q_start, const int* kv_len, int B, int N, int P, int page, int T, int H,
+               int Hkv, int hd, int max_new, int window, int sinks) {
+  ELFA_REQUIRE(pages && table && q_start && kv_len, "paged: null pointer");
+  ELFA_REQUIRE(B > 0 && B <= PAGED_MAX_SEQS && N > 0 && P > 0 && T > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && max_new > 0, "paged: bad sizes");
+  ELFA_REQUIRE(page >= 16 && page <= 256 && (page & (page - 1)) == 0, "paged: tokens per page must be 16, 32, 64, 128 or 256");
+  ELFA_REQUIRE(hd >= 8 && hd <= 128 && hd % 8 == 0, "paged: head dimension must be a multiple of 8 up to 128");
+  ELFA_REQUIRE((long long)P * 2 * Hkv < 0x7fffffffLL && (long long)N * page < 0x7fffff00LL, "paged: too many pages");
+  ELFA_REQUIRE((long long)T * (H / Hkv) < 0x7ffff000LL, "paged: too many query rows");
+  ELFA_REQUIRE(window >= 0 && sinks >= 0, "paged: negative window or sinks");
+  ELFA_REQUIRE((reinterpret_cast<uintptr_t>(pages) & 15) == 0, "paged: pages must be 16-byte aligned");
+  g->status = status_word();
+  ELFA_REQUIRE(g->status != nullptr, "paged: no status word");
+  g->table = table; g->q_start = q_start; g->kv_len = kv_len;
+  g->B = B; g->N = N; g->P = P; g->T = T; g->max_new = max_new;
+  g->page_shift = __builtin_ctz((unsigned)page);
+  g->H = H; g->Hkv = Hkv; g->rep = H / Hkv; g->hd = hd;
+  g->window = window > (1 << 30) ? 0 : window;
+  g->sinks = sinks > (1 << 30) ? 1 << 30 : sinks;
+  return ELFA_OK;
+}
+
+}  // namespace elfa
+
+using namespace elfa;
+
+// Floats of scratch that elfa_paged_attention wants for a call of these sizes.
+ELFA_API int elfa_paged_attention_scratch(int N, int page, int H, int Hkv, int hd, int max_new) {
+  if (N <= 0 || page <= 0 || Hkv <= 0 || H % Hkv || max_new <= 0) return 0;
+  if (decode_whole(max_new, H / Hkv, (long long)N * page)) return 0;
+  return 2 * decode_grid(hd) * DROWS * ((hd <= 64 ? 64 : 128) + 2);
+}
+
+// q: rows [T] of H heads, `qs` elements apart, heads packed, 16-byte aligned; out: [T, H * hd] contiguous. max_new: at least the most new tokens of a sequence.
+ELFA_API int elfa_paged_attention(const void* q, long long qs, const void* pages, const int* table, const int* q_start, const int* kv_len, void* out,
+                                  float* scratch, int B, int N, int P, int page, int T, int H, int Hkv, int hd, int max_new, int window, int sinks,
+                                  float scale, void* stream) {
+  DecodeArgs a{};
+  const int rc = paged_geom(&a.g, pages, table, q_start, kv_len, B, N, P, page, T, H, Hkv, hd, max_new, window, sinks);
+  if (rc != ELFA_OK) return rc;
+  ELFA_REQUIRE(q && out, "paged_attention: null pointer");
+  ELFA_REQUIRE(qs % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
+               "paged_attention: query rows must lie on 16-byte boundaries");
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.pages = static_cast<const __nv_bfloat16*>(pages);
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.qs = qs;
+  a.scale = scale;
+  a.g.tile_rows = DROWS;
+  a.whole = decode_whole(max_new, a.g.rep, (long long)N * page);
+  a.wide = ((long long)max_new * a.g.rep + DROWS - 1) / DROWS > 4;
+  a.min_units = MIN_UNITS;
+  ELFA_REQUIRE(a.whole || scratch, "paged_attention: no scratch");
+  a.part = scratch;
+  a.stat = scratch + 2LL * decode_grid(hd) * DROWS * (hd <= 64 ? 64 : 128);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return hd <= 64 ? launch_decode<64>(a, page, st) : launch_decode<128>(a, page, st);
+}

@@ -28,6 +28,7 @@ ST_FLAG_TIMEOUT = 2
 ST_BAD_TARGET = 4
 ST_NONFINITE = 8
 ST_BOUNDS = 16
+ST_BAD_PAGE = 32
 
 EPI_BIAS, EPI_GELU, EPI_DGELU_AUX, EPI_ADD_AUX, EPI_ACCUM, EPI_OUT_F32, EPI_STORE_PREACT = 1, 2, 4, 8, 16, 32, 64
 
@@ -189,6 +190,8 @@ def check_status() -> None:
         raise CommTimeout(f"a device-side wait timed out (status 0x{st:x})")
     if st & ST_BAD_TARGET:
         raise NativeError("token or target id outside the vocabulary")
+    if st & ST_BAD_PAGE:
+        raise NativeError("paged cache: lengths that do not fit each other or the table, a new token without a page, or a page outside the pool")
     if st & ST_BOUNDS:
         raise NativeError("a kernel of the checked build computed an index outside the extents it was given (the access was skipped)")
 

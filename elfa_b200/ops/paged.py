@@ -1,0 +1,200 @@
+"""Attention over a cache of pages, and moving keys and values into and between them.
+
+A layer's cache is ``pages [P, 2, Hkv, page, hd]`` (keys, then values; ``page`` tokens of 16, 32, 64, 128 or 256), ``table [B, N]`` int32 names the
+pages of each sequence in order (negative: not there). A call takes new tokens of all sequences one after the other: those of sequence ``b`` are rows
+``q_start[b]`` to ``q_start[b + 1]`` (``q_start [B + 1]`` int32 from 0 to the number of rows), and ``kv_len [B]`` int32 counts its tokens with them. The i-th of
+``n`` new tokens stands at ``kv_len - n + i``.
+
+CUDA tensors run the kernels of ``csrc/paged_decode.cu`` and ``csrc/pages.cu``: bf16, on the current stream, nothing is read back; lengths or
+page numbers that do not fit are recorded in the device status word (``native.check_status``). CPU tensors run the formula. There is no backward
+pass: sequences are generated, not trained, from a cache. :class:`elfa_b200.runtime.paged_cache.PagedCache` keeps pools, tables and lengths.
+
+reference: ``src/eval/evaluator.zig:419-470`` (generation runs the whole context of one sequence again for every token).
+"""
+from __future__ import annotations
+
+import array
+import math
+from typing import Optional, Sequence
+
+import torch
+
+from ..native import lib, stream_ptr
+
+PAGE_SIZES = (16, 32, 64, 128, 256)
+_MAX_SEQS = 1024        # sequences of one launch
+
+
+def paged_attention_ref(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
+                        window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None) -> torch.Tensor:
+    """The formula in fp32 (fp64 for fp64 pages), sequence by sequence."""
+    T, H, hd = q.shape
+    Hkv, page = pages.shape[2], pages.shape[3]
+    acc = torch.float64 if pages.dtype == torch.float64 else torch.float32
+    sc = scale if scale is not None else 1.0 / math.sqrt(hd)
+    out = torch.zeros(T, H, hd, dtype=acc, device=q.device)
+    starts = q_start.tolist()
+    for b, kv in enumerate(kv_len.tolist()):
+        n = starts[b + 1] - starts[b]
+        if n <= 0:
+            continue
+        key = torch.arange(kv, device=q.device)
+        ids = table[b, key // page].long()
+        there = (ids >= 0) & (ids < pages.shape[0])
+        rows = pages[ids.clamp(0, pages.shape[0] - 1), :, :, key % page].to(acc)             # [kv, 2, Hkv, hd]
+        pos = torch.arange(kv - n, kv, device=q.device)[:, None]
+        sees = (key <= pos) & there
+        if window is not None:
+            sees = sees & ((key > pos - window) | (key < sinks))
+        qb = q[starts[b]:starts[b + 1]].to(acc).view(n, Hkv, H // Hkv, hd)
+        s = torch.einsum("nhrd,khd->hrnk", qb, rows[:, 0]) * sc
+        s = s.masked_fill(~sees, float("-inf"))
+        p = torch.softmax(s, -1).masked_fill(~sees, 0.0)                                     # a row that sees nothing: zeros
+        # what a row does not see must not reach it, not even as 0 times infinity
+        v = rows[:, 1]
+        if bool(torch.isfinite(v).all()):
+            o = torch.einsum("hrnk,khd->nhrd", p, v)
+        else:
+            o = torch.stack([torch.einsum("hrk,khd->hrd", p[:, :, i][..., sees[i]], v[sees[i]]) for i in range(n)])
+        out[starts[b]:starts[b + 1]] = o.reshape(n, H, hd)
+    return out.reshape(T, H * hd).to(q.dtype)
+
+
+def _check(pages: torch.Tensor, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, what: str) -> None:
+    if pages.dim() != 5 or pages.shape[1] != 2:
+        raise ValueError(f"{what}: pages must be [P, 2, Hkv, page, hd], got {tuple(pages.shape)}")
+    B = kv_len.shape[0] if kv_len.dim() == 1 else -1
+    if B < 0 or table.dim() != 2 or table.shape[0] != B or q_start.shape != (B + 1,):
+        raise ValueError(f"{what}: table [B, N], q_start [B + 1] and kv_len [B] do not fit each other: "
+                         f"{tuple(table.shape)}, {tuple(q_start.shape)}, {tuple(kv_len.shape)}")
+    dev = pages.device
+    if table.device != dev or q_start.device != dev or kv_len.device != dev:
+        raise ValueError(f"{what}: table, q_start and kv_len must be on the pages' device, {dev}")
+    if table.dtype != torch.int32 or q_start.dtype != torch.int32 or kv_len.dtype != torch.int32:
+        raise TypeError(f"{what}: table, q_start and kv_len must be int32")
+
+
+def _check_cuda(pages: torch.Tensor, what: str) -> None:
+    if pages.dtype != torch.bfloat16:
+        raise TypeError(f"{what}: bf16 required on CUDA, got {pages.dtype}")
+    if pages.shape[3] not in PAGE_SIZES or pages.shape[4] % 8 or not 8 <= pages.shape[4] <= 128:
+        raise ValueError(f"{what}: pages of {PAGE_SIZES} tokens and head dimensions that are multiples of 8 up to 128, got {pages.shape[3]} and {pages.shape[4]}")
+    if not pages.is_contiguous() or pages.data_ptr() % 16:
+        raise ValueError(f"{what}: pages must be contiguous and 16-byte aligned")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t [T, heads, hd]`` with packed heads on 16-byte boundaries: itself (a slice of a fused projection is), or a copy."""
+    if t.stride(2) == 1 and t.stride(1) == t.shape[2] and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def paged_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
+                    max_new: Optional[int] = None, window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None) -> torch.Tensor:
+    """The new tokens' queries ``q [T, H, hd]`` (rows may be strided) against the pages, which hold the new tokens' keys and values already
+    (:func:`paged_write`). A query at position ``p`` sees the keys up to ``p``; with a ``window`` the last ``window`` of them and the first ``sinks``; never those of
+    pages that are not there. A row that sees nothing (or only scores of -inf) is zero, and what a row does not see cannot reach it whatever it holds. ``H`` is a
+    multiple of ``Hkv``. ``max_new``: an upper bound of the new tokens of one sequence, known to the host; without it the number of rows. Returns ``[T, H * hd]``."""
+    _check(pages, table, q_start, kv_len, "paged_attention")
+    if q.dim() != 3 or q.shape[2] != pages.shape[4] or q.shape[1] < 1 or q.shape[1] % pages.shape[2]:
+        raise ValueError(f"paged_attention: q must be [T, H, {pages.shape[4]}] with H a multiple of {pages.shape[2]}, got {tuple(q.shape)}")
+    if q.dtype != pages.dtype or q.device != pages.device:
+        raise TypeError("paged_attention: q and pages differ in type or device")
+    if window is not None and window < 1:
+        raise ValueError("paged_attention: a window holds at least the token itself")
+    if sinks < 0:
+        raise ValueError("paged_attention: negative sinks")
+    if torch.is_grad_enabled() and (q.requires_grad or pages.requires_grad):
+        raise RuntimeError("paged_attention has no backward pass: call it without gradients")
+    T, H, hd = q.shape
+    B, N = table.shape
+    if not q.is_cuda:
+        return paged_attention_ref(q, pages, table, q_start, kv_len, window, sinks, scale)
+    _check_cuda(pages, "paged_attention")
+    out = torch.empty((T, H * hd), dtype=q.dtype, device=q.device)
+    if T == 0:
+        return out
+    if B == 0 or N == 0:
+        return out.zero_()
+    q, table = _rows(q), table.contiguous()
+    P, _, Hkv, page, _ = pages.shape
+    max_new = T if max_new is None else min(int(max_new), T)
+    if max_new < 1:
+        raise ValueError("paged_attention: max_new must be positive where there are new tokens")
+    if not q_start.is_contiguous() or not kv_len.is_contiguous():
+        q_start, kv_len = q_start.contiguous(), kv_len.contiguous()
+    n = lib.raw("elfa_paged_attention_scratch")(N, page, H, Hkv, hd, max_new)
+    scratch = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+    sc = scale if scale is not None else hd ** -0.5
+    stream = stream_ptr(q)
+    for b in range(0, B, _MAX_SEQS):           # q_start counts from the first row of the whole call in every part
+        m = min(_MAX_SEQS, B - b)
+        lib.call("elfa_paged_attention", q, q.stride(0), pages, table.data_ptr() + 4 * b * N, q_start.data_ptr() + 4 * b, kv_len.data_ptr() + 4 * b, out,
+                 scratch, m, N, P, page, T, H, Hkv, hd, max_new, min(window or 0, 1 << 30), min(sinks, 1 << 30), sc, stream)
+    return out
+
+
+def paged_write(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor) -> None:
+    """Writes the new tokens' keys and values ``k, v [T, Hkv, hd]`` (rows may be strided) into their places, in place. Every new token needs a page."""
+    _check(pages, table, q_start, kv_len, "paged_write")
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (pages.shape[2], pages.shape[4]):
+        raise ValueError(f"paged_write: k and v must be [T, {pages.shape[2]}, {pages.shape[4]}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype != pages.dtype or v.dtype != pages.dtype or k.device != pages.device or v.device != pages.device:
+        raise TypeError("paged_write: k, v and pages differ in type or device")
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or pages.requires_grad):
+        raise RuntimeError("paged_write has no backward pass: call it without gradients")
+    T, Hkv, hd = k.shape
+    B, N = table.shape
+    if T == 0:
+        return
+    if B == 0 or N == 0:
+        raise ValueError("paged_write: new tokens without a sequence or a page")
+    if not k.is_cuda:
+        page = pages.shape[3]
+        starts = q_start.tolist()
+        for b, kv in enumerate(kv_len.tolist()):
+            n = starts[b + 1] - starts[b]
+            pos = torch.arange(kv - n, kv)
+            ids = table[b, pos // page].long()
+            if bool(((ids < 0) | (ids >= pages.shape[0])).any()):
+                raise ValueError("paged_write: a new token without a page")
+            pages[ids, 0, :, pos % page] = k[starts[b]:starts[b + 1]]
+            pages[ids, 1, :, pos % page] = v[starts[b]:starts[b + 1]]
+        return
+    _check_cuda(pages, "paged_write")
+    k, v, table = _rows(k), _rows(v), table.contiguous()
+    if not q_start.is_contiguous() or not kv_len.is_contiguous():
+        q_start, kv_len = q_start.contiguous(), kv_len.contiguous()
+    lib.call("elfa_paged_write", k, k.stride(0), v, v.stride(0), pages, table, q_start, kv_len, B, N, pages.shape[0], pages.shape[3], T, Hkv, hd, stream_ptr(k))
+
+
+def copy_pages(pages: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> None:
+    """Copies page ``src[i]`` over page ``dst[i]`` for all ``i`` at once, in place: ``pages [P, ...]`` of one layer (5 dimensions) or ``[L, P, ...]`` of all
+    (6). The page numbers come from the host, which knows them; they travel with the launch. No page may be written twice, or read and written."""
+    if pages.dim() not in (5, 6):
+        raise ValueError(f"copy_pages: pages must be [P, 2, Hkv, page, hd] or [L, P, 2, Hkv, page, hd], got {tuple(pages.shape)}")
+    if len(src) != len(dst):
+        raise ValueError("copy_pages: as many pages to read as to write")
+    if not pages.is_contiguous():
+        raise ValueError("copy_pages: pages must be contiguous")
+    if torch.is_grad_enabled() and pages.requires_grad:
+        raise RuntimeError("copy_pages has no backward pass: call it without gradients")
+    n = len(src)
+    if n == 0:
+        return
+    P = pages.shape[-5]
+    if not pages.is_cuda:
+        if min(min(src), min(dst)) < 0 or max(max(src), max(dst)) >= P:
+            raise ValueError("copy_pages: a page outside the pool")
+        if len(set(dst)) != n or not set(dst).isdisjoint(src):
+            raise ValueError("copy_pages: a page is written twice, or both read and written")
+        at = (slice(None),) * (pages.dim() - 5)
+        pages[at + (torch.tensor(list(dst)),)] = pages[at + (torch.tensor(list(src)),)]
+        return
+    L = pages.shape[0] if pages.dim() == 6 else 1
+    if L == 0:
+        return
+    size = pages.stride(-5) * pages.element_size()
+    a, b = array.array("i", src), array.array("i", dst)
+    lib.call("elfa_copy_pages", pages, P * size, size, L, P, a.buffer_info()[0], b.buffer_info()[0], n, stream_ptr(pages))
