@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(128) paged_decode_join_kernel(const __grid_con
   }
 }
 
-constexpr int WHOLE_KEYS = 256, MIN_UNITS = 4;
+constexpr int WHOLE_KEYS = 256, MIN_UNITS = 4, PREFILL_ROWS = 32;
 
 int decode_grid(int hd) { return 148 * (hd <= 64 ? 2 : 1); }
 bool decode_whole(int max_new, int rep, long long most_keys) { return (long long)max_new * rep <= DROWS && most_keys <= WHOLE_KEYS; }
@@ -445,6 +445,13 @@ int paged_geom(PagedGeom* g, const void* pages, const int* table, const int* q_s
   return ELFA_OK;
 }
 
+// paged_prefill.cu
+long long paged_prefill_scratch(int hd);
+int paged_prefill(PagedGeom g, const void* q, long long qs, const void* pages, void* out, float* scratch, int page, float scale, cudaStream_t st);
+
+// Which calls go to the tiles of 2 x 128 rows.
+static bool many_rows(int max_new, int rep) { return (long long)max_new * rep > PREFILL_ROWS && rep <= 128; }
+
 }  // namespace elfa
 
 using namespace elfa;
@@ -452,6 +459,7 @@ using namespace elfa;
 // Floats of scratch that elfa_paged_attention wants for a call of these sizes.
 ELFA_API int elfa_paged_attention_scratch(int N, int page, int H, int Hkv, int hd, int max_new) {
   if (N <= 0 || page <= 0 || Hkv <= 0 || H % Hkv || max_new <= 0) return 0;
+  if (many_rows(max_new, H / Hkv)) return (int)paged_prefill_scratch(hd);
   if (decode_whole(max_new, H / Hkv, (long long)N * page)) return 0;
   return 2 * decode_grid(hd) * DROWS * ((hd <= 64 ? 64 : 128) + 2);
 }
@@ -466,6 +474,11 @@ ELFA_API int elfa_paged_attention(const void* q, long long qs, const void* pages
   ELFA_REQUIRE(q && out, "paged_attention: null pointer");
   ELFA_REQUIRE(qs % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
                "paged_attention: query rows must lie on 16-byte boundaries");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (many_rows(max_new, a.g.rep)) {
+    ELFA_REQUIRE(scratch, "paged_attention: no scratch");
+    return paged_prefill(a.g, q, qs, pages, out, scratch, page, scale, st);
+  }
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.pages = static_cast<const __nv_bfloat16*>(pages);
   a.out = static_cast<__nv_bfloat16*>(out);
@@ -478,6 +491,5 @@ ELFA_API int elfa_paged_attention(const void* q, long long qs, const void* pages
   ELFA_REQUIRE(a.whole || scratch, "paged_attention: no scratch");
   a.part = scratch;
   a.stat = scratch + 2LL * decode_grid(hd) * DROWS * (hd <= 64 ? 64 : 128);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   return hd <= 64 ? launch_decode<64>(a, page, st) : launch_decode<128>(a, page, st);
 }

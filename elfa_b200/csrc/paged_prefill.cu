@@ -1,0 +1,578 @@
+// Attention over a paged cache for chunks of many query rows (prompts in pieces): pairs of 128-row tiles on tcgen05.
+//
+// The same sums as paged_decode.cu, bound by the tensor cores and the exponentials where rows are many. Rows of a tile are (token, head of the group), so the
+// heads that share a key head read its keys once: with rep heads per group a tile holds 128 / rep tokens, one TMA box {64 columns, rep heads, 128 / rep tokens}
+// per 64 columns. A CTA walks its share of the line of units (paged.cuh) with everything in flight across items: per pair of tiles and block of 128 keys
+//   warp 0      : TMA: queries once per item, keys one block ahead in two stages, values; a box per page
+//   warp 1      : every tcgen05.mma: S = Q K^T of the next block before O += P V of this one, also over the end of an item
+//   warp 2      : clears the value rows behind a sequence's last token before they are multiplied (what lies there may be anything)
+//   warps 4-11  : softmax and sums of tile 0 and tile 1, a thread per row, as in attention_fwd.cu: the whole S row in registers, P to shared memory in
+//                 bf16, O in tensor memory, scaled again when a row's maximum grows by more than 2^8
+// Parts of items go to scratch in fp32 and are joined by a second launch. Every wait is bounded.
+#include "elfa_native.h"
+#include "paged.cuh"
+
+namespace elfa {
+
+int make_paged_tmap(CUtensorMap* tm, const void* pages, long long P, int Hkv, int page, int hd, int box_rows);
+
+namespace {
+
+constexpr int PBLK = 128, PTHREADS = 384, PSUB = 128 * 128;
+
+struct PrefillArgs {
+  PagedGeom g;
+  const __nv_bfloat16 *q, *pages;
+  __nv_bfloat16* out;
+  float *part, *stat;                  // [2 G][2 tiles][HDP / 4][128] float4, [2 G][2 tiles][128] (maximum, sum)
+  long long qs;
+  float scale;
+  int tile_toks;                       // tokens of one of the two tiles
+};
+
+enum { PB_Q = 0, PB_QFREE, PB_KFULL, PB_KFREE = PB_KFULL + 2, PB_VFULL = PB_KFREE + 2, PB_VFREE, PB_VTAIL, PB_SFULL, PB_SREAD = PB_SFULL + 2,
+       PB_PREADY = PB_SREAD + 2, PB_OFULL = PB_PREADY + 2, PB_COUNT = PB_OFULL + 2 };
+
+template <int HDP>
+struct PrefillSmem {
+  static constexpr int NSUB = HDP / 64;
+  static constexpr int Q = 0, K = Q + 2 * NSUB * PSUB, V = K + 2 * NSUB * PSUB, P = V + NSUB * PSUB, BAR = P + 4 * PSUB;
+  static constexpr int TOTAL = BAR + PB_COUNT * 8 + 16 + 8 * (PTHREADS / 32);
+  static constexpr int DYN = TOTAL + 1024;
+  static_assert(8 * (PAGED_MAX_SEQS + 1) <= 4 * PSUB, "the prefix lies where P will");
+};
+
+// what a CTA does of an item: blocks i0 .. i1 of its list; tile 0 takes part up to n0, tile 1 up to n1
+struct Part {
+  int i0, i1, n0, n1;
+};
+__device__ __forceinline__ Part part_of(const PagedGeom& g, const PagedItem& it, long long u, long long u_end) {
+  Part p;
+  p.i0 = (int)(u - it.u0);
+  p.i1 = (int)(min(u_end, it.u0 + it.span.n) - it.u0);
+  const int half = g.tile_rows >> 1, r0 = it.t * g.tile_rows, rows = min(g.tile_rows, it.s.n * g.rep - r0);
+  if (rows <= half) {
+    p.n0 = p.i1;
+    p.n1 = p.i0;
+  } else {
+    const int hi = max(it.s.kv - it.s.n + (r0 + half - 1) / g.rep + 1, 0), b = (hi + PBLK - 1) / PBLK;      // blocks up to tile 0's last row
+    const int n = b >= it.span.w0 ? it.span.ns + b - it.span.w0 : min(it.span.ns, b);
+    p.n0 = min(max(n, p.i0), p.i1);
+    p.n1 = p.i1;
+  }
+  return p;
+}
+
+template <int HDP>
+__global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKV,
+                                                                    const __grid_constant__ PrefillArgs a) {
+  using L = PrefillSmem<HDP>;
+  constexpr int NSUB = L::NSUB;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + PB_COUNT);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  long long* warp_tot = reinterpret_cast<long long*>(tmem_holder + 4);
+  const uint32_t sbase = smem_u32(smem), bar0 = smem_u32(bars);
+  auto bar = [&](int i) { return bar0 + 8u * i; };
+  const PagedGeom& g = a.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int half_rows = g.tile_rows >> 1;
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmQ);
+    prefetch_tmap(&tmKV);
+    for (int i = 0; i < PB_COUNT; ++i)
+      mbar_init(bar(i), i == PB_SREAD || i == PB_SREAD + 1 || i == PB_PREADY || i == PB_PREADY + 1 ? 4 : 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_holder), 512);
+    tmem_relinquish();
+  }
+  // query rows that no box fills (rep does not divide 128) stay zero
+  for (int i = half_rows * 8 + threadIdx.x; i < 128 * 8; i += PTHREADS)
+#pragma unroll
+    for (int s = 0; s < 2 * NSUB; ++s)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sbase + L::Q + s * PSUB + i * 16), "r"(0) : "memory");
+  fence_proxy_async();
+  long long* prefix = reinterpret_cast<long long*>(smem + L::P);
+  paged_prefix<PBLK, PTHREADS>(g, prefix, warp_tot, true);
+  const long long W = prefix[g.B];
+  const int G = (int)min(W, (long long)gridDim.x);
+  const long long u_begin = (int)blockIdx.x < G ? paged_cut(W, G, blockIdx.x) : 0, u_end = (int)blockIdx.x < G ? paged_cut(W, G, blockIdx.x + 1) : 0;
+  PagedItem it;
+  if (u_begin < u_end) it = paged_find<PBLK>(g, prefix, u_begin);
+  pdl_next();
+  tc_fence_before();
+  __syncthreads();                                         // the prefix makes room for P
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  const uint32_t TM_S[2] = {tmem_base + 0, tmem_base + 128};
+  const uint32_t TM_O[2] = {tmem_base + 256, tmem_base + 256 + HDP};
+
+  if (warp < 4) {
+    reg_dec<80>();
+    if (warp == 0) {
+      // ---------------------------------------------------------------- loads
+      const int box_rows = min(1 << g.page_shift, PBLK), boxes = PBLK / box_rows, box = lane / NSUB, sub = lane % NSUB;
+      const bool mine = box < boxes;
+      const int none = 2 * g.P * g.Hkv;                    // past the pool's end: zeros
+      bool ok = true;
+      uint32_t kc = 0, vc = 0, qc = 0;
+      auto wait = [&](int b, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(b), parity, abort_flag, g.status)); };
+      auto page_of = [&](const PagedItem& x, int i) {
+        const int key = x.span.block(i) * PBLK + box * box_rows;
+        return mine && key < x.s.kv ? paged_page(g, x.b, key) : -1;
+      };
+      auto load_q = [&](const PagedItem& x) {
+        if (qc) wait(PB_QFREE, (qc - 1) & 1);
+        ++qc;
+        if (!ok) return;
+        const int tiles = min(g.tile_rows, x.s.n * g.rep - x.t * g.tile_rows) > half_rows ? 2 : 1;
+        if (lane == 0) mbar_expect_tx(bar(PB_Q), tiles * NSUB * half_rows * 128);
+        __syncwarp();
+        if (lane < tiles * NSUB)
+          tma_load_3d(sbase + L::Q + lane * PSUB, &tmQ, (lane % NSUB) * 64, x.h * g.rep, x.s.q0 + (2 * x.t + lane / NSUB) * a.tile_toks, bar(PB_Q));
+        __syncwarp();
+      };
+      auto load = [&](const PagedItem& x, int i, int id, int kv, uint32_t dst, int b) {
+        if (lane == 0) mbar_expect_tx(bar(b), NSUB * PSUB);
+        __syncwarp();
+        if (mine)
+          tma_load_3d(dst + sub * PSUB + box * box_rows * 128, &tmKV, sub * 64, (x.span.block(i) * PBLK + box * box_rows) & ((1 << g.page_shift) - 1),
+                      id < 0 ? none : (2 * id + kv) * g.Hkv + x.h, bar(b));
+        __syncwarp();
+      };
+      auto load_k = [&](const PagedItem& x, int i, int id) {
+        const int st = kc & 1;
+        if (kc >= 2) wait(PB_KFREE + st, ((kc >> 1) - 1) & 1);
+        ++kc;
+        if (ok) load(x, i, id, 0, sbase + L::K + st * NSUB * PSUB, PB_KFULL + st);
+      };
+      if (u_begin < u_end) {
+        int id = page_of(it, (int)(u_begin - it.u0));
+        load_q(it);
+        load_k(it, (int)(u_begin - it.u0), id);
+        for (long long u = u_begin; u < u_end && ok; ++u) {
+          const PagedItem cur = it;
+          const int i = (int)(u - cur.u0);
+          int next_id = -1;
+          if (u + 1 < u_end) {
+            const bool fresh = u + 1 >= it.u0 + it.span.n;
+            if (fresh) paged_next<PBLK>(g, it);
+            next_id = page_of(it, (int)(u + 1 - it.u0));
+            if (fresh) load_q(it);
+            load_k(it, (int)(u + 1 - it.u0), next_id);
+          }
+          if (vc) wait(PB_VFREE, (vc - 1) & 1);
+          ++vc;
+          if (ok) load(cur, i, id, 1, sbase + L::V, (cur.span.block(i) + 1) * PBLK > cur.s.kv ? PB_VTAIL : PB_VFULL);
+          id = next_id;
+        }
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- products
+      constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false), idesc_o = make_idesc_bf16(128, HDP, false, true);
+      bool ok = true;
+      uint32_t kc = 0, vc = 0, qc = 0, sI[2] = {0, 0}, pI[2] = {0, 0};
+      auto wait = [&](int b, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(b), parity, abort_flag, g.status)); };
+      auto commit = [&](int b) {
+        if (elect_one()) tc_commit(bar(b));
+        __syncwarp();
+      };
+      const uint64_t dq = make_smem_desc(sbase + L::Q, 16, 1024, 2), dk = make_smem_desc(sbase + L::K, 16, 1024, 2);
+      const uint64_t dp = make_smem_desc(sbase + L::P, 16, 1024, 2), dv = make_smem_desc(sbase + L::V, PSUB, 1024, 2);
+      const uint32_t q_lo = (uint32_t)dq, q_hi = (uint32_t)(dq >> 32), k_lo = (uint32_t)dk, k_hi = (uint32_t)(dk >> 32);
+      const uint32_t p_lo = (uint32_t)dp, p_hi = (uint32_t)(dp >> 32), v_lo = (uint32_t)dv, v_hi = (uint32_t)(dv >> 32);
+      auto scores = [&](const Part& p, int i) {            // S of block i for the tiles that take part
+        const int st = kc & 1;
+        wait(PB_KFULL + st, (kc >> 1) & 1);
+        if (i == p.i0) {
+          wait(PB_Q, qc & 1);
+          ++qc;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (i >= (t ? p.n1 : p.n0)) continue;
+          if (sI[t]) wait(PB_SREAD + t, (sI[t] - 1) & 1);
+          ++sI[t];
+          if (!ok) return;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < HDP / 16; ++kk) {
+              const uint32_t off = ((kk / 4) * PSUB + (kk % 4) * 32) >> 4;
+              tc_mma_f16_lh(TM_S[t], q_lo + ((t * NSUB * PSUB) >> 4) + off, q_hi, k_lo + ((st * NSUB * PSUB) >> 4) + off, k_hi, idesc_s, kk != 0);
+            }
+            tc_commit(bar(PB_SFULL + t));
+          }
+          __syncwarp();
+        }
+        commit(PB_KFREE + st);
+        ++kc;
+        if (i + 1 == p.i1) commit(PB_QFREE);
+      };
+      if (u_begin < u_end) {
+        Part p = part_of(g, it, u_begin, u_end);
+        scores(p, p.i0);
+        for (long long u = u_begin; u < u_end && ok; ++u) {
+          const Part c = p;
+          const int i = (int)(u - it.u0);
+          if (u + 1 < u_end) {
+            int ni = i + 1;
+            if (ni >= c.i1) {
+              paged_next<PBLK>(g, it);
+              p = part_of(g, it, u + 1, u_end);
+              ni = p.i0;
+            }
+            scores(p, ni);
+            if (!ok) break;
+          }
+          wait(PB_VFULL, vc & 1);
+          ++vc;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (i >= (t ? c.n1 : c.n0)) continue;
+            wait(PB_PREADY + t, pI[t] & 1);
+            ++pI[t];
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk) {
+                const uint32_t off = ((kk / 4) * PSUB + (kk % 4) * 32) >> 4;
+                tc_mma_f16_lh(TM_O[t], p_lo + ((t * 2 * PSUB) >> 4) + off, p_hi, v_lo + ((kk * 2048) >> 4), v_hi, idesc_o, i != c.i0 || kk != 0);
+              }
+              tc_commit(bar(PB_OFULL + t));
+            }
+            __syncwarp();
+          }
+          if (ok) commit(PB_VFREE);
+        }
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------------------------------- value rows that hold no token
+      uint32_t tails = 0;
+      for (long long u = u_begin; u < u_end;) {
+        const long long ue = min(u_end, it.u0 + it.span.n);
+        bool ok = true;
+        for (int i = (int)(u - it.u0); i < (int)(ue - it.u0) && ok; ++i) {
+          const int key0 = it.span.block(i) * PBLK;
+          if (key0 + PBLK <= it.s.kv) continue;
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_VTAIL), tails & 1, abort_flag, g.status));
+          ++tails;
+          if (!ok) break;
+          for (int x = max(it.s.kv - key0, 0) * 8 + lane; x < PBLK * 8; x += 32)
+#pragma unroll
+            for (int s = 0; s < NSUB; ++s)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sbase + L::V + s * PSUB + x * 16), "r"(0) : "memory");
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(PB_VFULL));
+        }
+        if (!ok) break;
+        u = ue;
+        if (u < u_end) paged_next<PBLK>(g, it);
+      }
+    }
+  } else {
+    reg_inc<208>();
+    // ---------------------------------------------------------------- softmax and sums
+    const int t = (warp - 4) >> 2, quarter = warp & 3, row_local = quarter * 32 + lane;
+    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+    const uint32_t p_row = sbase + L::P + t * 2 * PSUB + row_local * 128;
+    const float sl2 = a.scale * 1.4426950408889634f;
+    uint32_t sc = 0, oc = 0;                               // S rows taken, P tiles handed over
+    bool ok = true;
+    for (long long u = u_begin; u < u_end && ok;) {
+      const Part p = part_of(g, it, u, u_end);
+      const int n_t = t ? p.n1 : p.n0;
+      const int first_row = it.t * g.tile_rows + t * half_rows, rows = min(half_rows, it.s.n * g.rep - first_row);   // rows <= 0: no such tile
+      const int pos0 = it.s.kv - it.s.n;
+      const int r = first_row + min(row_local, max(rows, 1) - 1), tok = min(r / g.rep, it.s.n - 1), pos = pos0 + tok;
+      const int pos_min = pos0 + first_row / g.rep, pos_max = pos0 + (first_row + max(rows, 1) - 1) / g.rep;
+      const int lower = g.window ? pos - g.window + 1 : 0;
+      float m = -INFINITY, l = 0.f;
+      for (int i = p.i0; i < n_t; ++i) {
+        const int key0 = it.span.block(i) * PBLK;
+        const int col_key = key0 + lane * 16;              // whether the page of each 16 keys is there
+        const int id = lane < 8 && col_key < it.s.kv ? paged_page(g, it.b, col_key) : -1;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_SFULL + t), sc & 1, abort_flag, g.status));
+        ++sc;
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(TM_S[t] + lane_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+        tmem_ld_wait();
+        tc_fence_before();
+        const uint32_t there = __ballot_sync(0xffffffffu, id >= 0) & 0xffu;
+        if (lane == 0) mbar_arrive(bar(PB_SREAD + t));
+        bool landed = i == p.i0;                           // whether the product before is known to be complete (an item's end waits for it)
+        if (there != 0xffu || (g.window && key0 < pos_max - g.window + 1 && key0 + PBLK > g.sinks)) {
+          const int far = g.window ? lower : 0, keep = g.window ? g.sinks : 0;
+#pragma unroll
+          for (int x = 0; x < 128; ++x)
+            if (key0 + x > pos || (key0 + x < far && key0 + x >= keep) || !(there >> (x / 16) & 1u)) s[x] = 0xff800000u;
+        } else if (key0 + PBLK - 1 > pos_min) {
+#pragma unroll
+          for (int x = 0; x < 128; ++x)
+            if (key0 + x > pos) s[x] = 0xff800000u;        // -inf
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int x = 0; x < 128; x += 2) mx4[(x >> 1) & 3] = max3(mx4[(x >> 1) & 3], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
+        if (i == p.i0) {
+          m = mx;
+        } else {
+          const bool grow = mx - m > 8.f;
+          if (__any_sync(0xffffffffu, grow)) {
+            ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_OFULL + t), (oc - 1) & 1, abort_flag, g.status));
+            if (!ok) break;
+            landed = true;
+            tc_fence_after();
+            const float m_new = grow ? mx : m, alpha = m_new == m ? 1.f : fast_exp2(m - m_new);
+#pragma unroll 1
+            for (int c = 0; c < HDP / 16; ++c) {           // narrow pieces: the S row stays in registers meanwhile
+              uint32_t o[16];
+              tmem_ld16(TM_O[t] + lane_addr + c * 16, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+              tmem_st16(TM_O[t] + lane_addr + c * 16, o);
+            }
+            tmem_st_wait();
+            l *= alpha;
+            m = m_new;
+          }
+        }
+        const float neg_m = m == -INFINITY ? 0.f : -m;
+        const uint64_t sc2 = pack_f32x2(sl2, sl2), neg2 = pack_f32x2(neg_m, neg_m);
+        uint64_t ls[2] = {0ull, 0ull};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int x = 0; x < 32; x += 2) {
+            float x0, x1;
+            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[c * 32 + x]), __uint_as_float(s[c * 32 + x + 1])), sc2, neg2), x0, x1);
+            const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
+            ls[(x >> 1) & 1] = add_f32x2(ls[(x >> 1) & 1], pack_f32x2(e0, e1));
+            w[x >> 1] = pack_bf16(e0, e1);
+          }
+          if (c == 0 && !landed) {                         // P is still the operand of the product before
+            ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_OFULL + t), (oc - 1) & 1, abort_flag, g.status));
+          }
+          if (ok) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int q8 = c * 4 + x;
+              const uint32_t addr = p_row + (q8 >> 3) * PSUB + (((q8 & 7) ^ (row_local & 7)) << 4);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[x * 4]), "r"(w[x * 4 + 1]), "r"(w[x * 4 + 2]),
+                           "r"(w[x * 4 + 3]) : "memory");
+            }
+          }
+        }
+        if (!ok) break;
+        float a0, a1, a2, a3;
+        unpack_f32x2(ls[0], a0, a1);
+        unpack_f32x2(ls[1], a2, a3);
+        l += (a0 + a1) + (a2 + a3);
+        fence_proxy_async();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(PB_PREADY + t));
+        ++oc;
+      }
+      const bool any = n_t > p.i0, whole = p.i0 == 0 && p.i1 == it.span.n;
+      if (ok && any) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_OFULL + t), (oc - 1) & 1, abort_flag, g.status));
+        tc_fence_after();
+      }
+      if (ok && rows > 0) {
+        const bool valid = row_local < rows;
+        const long long at = it.s.q0 + tok;
+        const int head = it.h * g.rep + r - tok * g.rep;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        __nv_bfloat16* orow = a.out + (at * g.H + head) * g.hd;
+        const long long ps = (2LL * blockIdx.x + (p.i0 == 0)) * 2 + t;
+        float4* prow = reinterpret_cast<float4*>(a.part) + ps * (HDP / 4) * 128 + row_local;
+        bool finite = true;
+#pragma unroll 1
+        for (int c = 0; c < HDP / 32; ++c) {
+          uint32_t o[32];
+          if (any) {
+            __syncwarp();
+            tmem_ld32(TM_O[t] + lane_addr + c * 32, o);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = 0u;
+          }
+          if (!valid) continue;
+          if (whole) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) {
+              const float v = __uint_as_float(o[x]) * inv;
+              finite = finite && isfinite(v);
+              o[x] = __float_as_uint(v);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (c * 32 + x * 8 < g.hd)
+                *reinterpret_cast<uint4*>(orow + c * 32 + x * 8) =
+                    make_uint4(pack_bf16(__uint_as_float(o[x * 8]), __uint_as_float(o[x * 8 + 1])), pack_bf16(__uint_as_float(o[x * 8 + 2]), __uint_as_float(o[x * 8 + 3])),
+                               pack_bf16(__uint_as_float(o[x * 8 + 4]), __uint_as_float(o[x * 8 + 5])), pack_bf16(__uint_as_float(o[x * 8 + 6]), __uint_as_float(o[x * 8 + 7])));
+          } else {
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              prow[(c * 8 + x) * 128] = make_float4(__uint_as_float(o[x * 4]), __uint_as_float(o[x * 4 + 1]), __uint_as_float(o[x * 4 + 2]), __uint_as_float(o[x * 4 + 3]));
+          }
+        }
+        if (!whole && valid) reinterpret_cast<float2*>(a.stat)[ps * 128 + row_local] = make_float2(m, l);
+        __syncwarp();
+        unsigned bad = __ballot_sync(0xffffffffu, whole && valid && !finite);
+        while (bad) {
+          const int x = __ffs(bad) - 1, rx = first_row + quarter * 32 + x, tx = rx / g.rep;
+          bad &= bad - 1;
+          const int hx = it.h * g.rep + rx - tx * g.rep;
+          const long long ax = it.s.q0 + tx;
+          float res[HDP / 32];
+          paged_row<HDP>(g, a.q + ax * a.qs + hx * g.hd, a.pages, it.b, it.h, pos0 + tx, a.scale, res);
+#pragma unroll
+          for (int c = 0; c < HDP / 32; ++c)
+            if (lane + 32 * c < g.hd) a.out[(ax * g.H + hx) * g.hd + lane + 32 * c] = __float2bfloat16(res[c]);
+        }
+        tc_fence_before();
+        __syncwarp();
+      }
+      u = min(u_end, it.u0 + it.span.n);
+      if (u < u_end) paged_next<PBLK>(g, it);
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Block (c - 1, y) joins rows y, y + Y, ... of the item that the cut between CTAs c - 1 and c goes through, if no earlier cut does: a warp per row.
+template <int HDP>
+__global__ void __launch_bounds__(128) paged_prefill_join_kernel(const __grid_constant__ PrefillArgs a, int grid) {
+  extern __shared__ long long prefix[];
+  __shared__ long long warp_tot[4];
+  const PagedGeom& g = a.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  paged_prefix<PBLK, 128>(g, prefix, warp_tot, true);
+  const long long W = prefix[g.B];
+  const int G = (int)min(W, (long long)grid), c = blockIdx.x + 1;
+  pdl_wait();
+  if (c >= G) return;
+  const long long u = paged_cut(W, G, c);
+  const PagedItem it = paged_find<PBLK>(g, prefix, u);
+  if (u == it.u0) return;
+  const int c0 = paged_owner(W, G, it.u0), c1 = paged_owner(W, G, it.u0 + it.span.n - 1);
+  if (c0 != c - 1) return;
+  const int half_rows = g.tile_rows >> 1, r0 = it.t * g.tile_rows, rows = min(g.tile_rows, it.s.n * g.rep - r0);
+  const float2* stat = reinterpret_cast<const float2*>(a.stat);
+  const float4* part = reinterpret_cast<const float4*>(a.part);
+  constexpr int VECS = HDP / 4;
+  for (int r = blockIdx.y * 4 + warp; r < rows; r += gridDim.y * 4) {
+    const int t = r >= half_rows, local = r - t * half_rows;
+    auto slot = [&](int i) { return (i == 0 ? 2LL * c0 + 1 : 2LL * (c0 + i)) * 2 + t; };
+    const int n = c1 - c0 + 1;
+    float M = -INFINITY;
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, stat[slot(i) * 128 + local].x);
+    M = warp_max(M);
+    float den = 0.f;
+    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      float w = 0.f, wl = 0.f;
+      if (i0 + lane < n) {
+        const float2 st = stat[slot(i0 + lane) * 128 + local];
+        w = st.x == -INFINITY ? 1.f : fast_exp2(st.x - M);             // without a maximum: sums of zero, or a NaN to hand on
+        wl = w * st.y;
+      }
+      den += wl;
+      const int m = min(32, n - i0);
+#pragma unroll 4
+      for (int i = 0; i < m; ++i) {
+        const float f = __shfl_sync(0xffffffffu, w, i);
+        if (lane < VECS) {
+          const float4 v = part[(slot(i0 + i) * VECS + lane) * 128 + local];
+          num.x += f * v.x; num.y += f * v.y; num.z += f * v.z; num.w += f * v.w;
+        }
+      }
+    }
+    den = warp_sum(den);
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    const float v[4] = {num.x * inv, num.y * inv, num.z * inv, num.w * inv};
+    const bool bad = __any_sync(0xffffffffu, !(isfinite(v[0]) && isfinite(v[1]) && isfinite(v[2]) && isfinite(v[3])));
+    const int tok = (r0 + r) / g.rep, head = it.h * g.rep + (r0 + r) - tok * g.rep;
+    const long long at = it.s.q0 + tok;
+    __nv_bfloat16* po = a.out + (at * g.H + head) * g.hd;
+    if (!bad) {
+      if (lane * 4 < g.hd) *reinterpret_cast<uint2*>(po + lane * 4) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+      continue;
+    }
+    float res[HDP / 32];
+    paged_row<HDP>(g, a.q + at * a.qs + head * g.hd, a.pages, it.b, it.h, it.s.kv - it.s.n + tok, a.scale, res);
+#pragma unroll
+    for (int x = 0; x < HDP / 32; ++x)
+      if (lane + 32 * x < g.hd) po[lane + 32 * x] = __float2bfloat16(res[x]);
+  }
+}
+
+template <int HDP>
+int launch_prefill(PrefillArgs& a, int page, int join_y, cudaStream_t st) {
+  CUtensorMap tmQ, tmKV;
+  int rc = make_paged_tmap(&tmKV, a.pages, a.g.P, a.g.Hkv, page, a.g.hd, page < PBLK ? page : PBLK);
+  if (rc != ELFA_OK) return rc;
+  const uint64_t dims[3] = {(uint64_t)a.g.hd, (uint64_t)a.g.H, (uint64_t)a.g.T};
+  const uint64_t strides[2] = {(uint64_t)a.g.hd * 2, (uint64_t)a.qs * 2};
+  const uint32_t box[3] = {64, (uint32_t)a.g.rep, (uint32_t)a.tile_toks};
+  rc = make_tmap_nd_bf16(&tmQ, a.q, 3, dims, strides, box);
+  if (rc != ELFA_OK) return rc;
+  ELFA_CUDA(allow_shared<paged_prefill_kernel<HDP>>(PrefillSmem<HDP>::DYN));
+  const int grid = 148;
+  paged_prefill_kernel<HDP><<<grid, PTHREADS, PrefillSmem<HDP>::DYN, st>>>(tmQ, tmKV, a);
+  ELFA_CUDA(cudaGetLastError());
+  ::elfa::count_launches(1);
+  PdlScope scope(true);
+  ELFA_CUDA(launch_chain(paged_prefill_join_kernel<HDP>, dim3(grid - 1, join_y), dim3(128), 8 * (a.g.B + 1), st, 1, a, grid));
+  ELFA_CUDA(cudaGetLastError());
+  ::elfa::count_launches(1);
+  return ELFA_OK;
+}
+
+}  // namespace
+
+long long paged_prefill_scratch(int hd) { return 2LL * 148 * 2 * 128 * ((hd <= 64 ? 64 : 128) + 2); }
+
+int paged_prefill(PagedGeom g, const void* q, long long qs, const void* pages, void* out, float* scratch, int page, float scale, cudaStream_t st) {
+  PrefillArgs a{};
+  a.g = g;
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.pages = static_cast<const __nv_bfloat16*>(pages);
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.qs = qs;
+  a.scale = scale;
+  a.tile_toks = 128 / g.rep;
+  a.g.tile_rows = 2 * a.tile_toks * g.rep;
+  a.part = scratch;
+  a.stat = scratch + 2LL * 148 * 2 * 128 * (g.hd <= 64 ? 64 : 128);
+  // items are cut into about 148 / items parts each: more blocks per item where there are many parts to read
+  const long long items = g.Hkv * ((long long)g.T * g.rep / a.g.tile_rows + 1);
+  const int join_y = (int)(items >= 74 ? 8 : (items >= 16 ? 16 : 64));
+  return g.hd <= 64 ? launch_prefill<64>(a, page, join_y, st) : launch_prefill<128>(a, page, join_y, st);
+}
+
+}  // namespace elfa
