@@ -181,6 +181,25 @@ __device__ __forceinline__ long long paged_cut(long long W, int G, int c) { retu
 // the CTA that holds unit u
 __device__ __forceinline__ int paged_owner(long long W, int G, long long u) { return (int)(((u + 1) * G - 1) / W); }
 
+// What joins an item that several CTAs have parts of, written by the CTA that the item's first cut lies in front of: its parts are slot 2 first + 1 and
+// slots 2 c for first < c <= last. rows 0: nothing to join here.
+struct alignas(16) PagedJoin {
+  int rows, last, b, h, r0, q0, pos0, unused;
+};
+__device__ __forceinline__ void paged_join_note(const PagedGeom& g, PagedJoin* notes, const PagedItem& it, long long W, int G, int c, bool has_units, bool cut) {
+  PagedJoin j{};
+  if (has_units && cut && paged_owner(W, G, it.u0) == c - 1) {
+    j.rows = min(g.tile_rows, it.s.n * g.rep - it.t * g.tile_rows);
+    j.last = paged_owner(W, G, it.u0 + it.span.n - 1);
+    j.b = it.b;
+    j.h = it.h;
+    j.r0 = it.t * g.tile_rows;
+    j.q0 = it.s.q0;
+    j.pos0 = it.s.kv - it.s.n;
+  }
+  notes[c] = j;
+}
+
 __device__ __forceinline__ bool paged_sees(const PagedGeom& g, int key, int pos) {
   return key <= pos && (!g.window || key > pos - g.window || key < g.sinks);
 }

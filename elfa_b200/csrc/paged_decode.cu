@@ -24,6 +24,7 @@ struct DecodeArgs {
   const __nv_bfloat16 *q, *pages;
   __nv_bfloat16* out;
   float *part, *stat;                  // [2 G][16][HDP], [2 G][16][2] (maximum, sum)
+  PagedJoin* notes;                    // [G]
   long long qs;                        // elements from a token's queries to the next one's
   float scale;
   int wide, whole;                     // a warp per sequence for the prefix; whole: CTA c takes item c, nothing is shared
@@ -68,7 +69,7 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
   if (lane < DST) mbar_init(bars + 8 * lane, 1);
   fence_barrier_init();
   long long u_begin, u_end;
-  PagedItem first;
+  PagedItem first{};
   if (a.whole) {
     first.b = blockIdx.x / g.Hkv;
     first.h = blockIdx.x % g.Hkv;
@@ -86,6 +87,7 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
     u_begin = (int)blockIdx.x < G ? paged_cut(W, G, blockIdx.x) : 0;
     u_end = (int)blockIdx.x < G ? paged_cut(W, G, blockIdx.x + 1) : 0;
     if (u_begin < u_end) first = paged_find<DBLK>(g, prefix, u_begin);
+    if (threadIdx.x == 0) paged_join_note(g, a.notes, first, W, G, blockIdx.x, u_begin < u_end, u_begin > first.u0);
   }
   pdl_next();
   if (u_begin >= u_end) return;
@@ -332,57 +334,70 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
   }
 }
 
-// Block c joins the item that the cut between CTAs c and c + 1 goes through, if no earlier cut does.
+// Block c - 1 joins the item that CTA c has noted. Rows, and of few rows the parts too, go to groups of HDP / 4 threads with four columns each.
 template <int HDP>
-__global__ void __launch_bounds__(128) paged_decode_join_kernel(const __grid_constant__ DecodeArgs a, int grid) {
-  extern __shared__ long long prefix[];
-  __shared__ long long warp_tot[4];
+__global__ void __launch_bounds__(256) paged_decode_join_kernel(const __grid_constant__ DecodeArgs a) {
+  constexpr int VEC = HDP / 4, GROUPS = 256 / VEC;
+  __shared__ float4 sum[GROUPS][VEC];
+  __shared__ float total[GROUPS];
   __shared__ unsigned bad;
   const PagedGeom& g = a.g;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  paged_prefix<DBLK, 128>(g, prefix, warp_tot, a.wide);
-  const long long W = prefix[g.B];
-  const int G = decode_ctas(W, grid, a.min_units), c = blockIdx.x + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = threadIdx.x / VEC, v = threadIdx.x % VEC;
   pdl_wait();
-  if (c >= G) return;
-  const long long u = paged_cut(W, G, c);
-  const PagedItem it = paged_find<DBLK>(g, prefix, u);
-  if (u == it.u0) return;
-  const int c0 = paged_owner(W, G, it.u0), c1 = paged_owner(W, G, it.u0 + it.span.n - 1);
-  if (c0 != c - 1) return;
+  const int c = blockIdx.x + 1;
+  const PagedJoin j = a.notes[c];
+  if (j.rows == 0) return;
   if (threadIdx.x == 0) bad = 0;
-  __syncthreads();
-  const int r0 = it.t * DROWS, rows = min(DROWS, it.s.n * g.rep - r0);
-  constexpr int PER = 128 / HDP;                                       // rows side by side
-  const int col = threadIdx.x % HDP;
+  const int n = j.last - c + 2;                                        // parts: CTAs c - 1 to last
+  const int wide = min(j.rows <= 1 ? 1 : 1 << (32 - __clz(j.rows - 1)), GROUPS), subs = GROUPS / wide;   // rows side by side, groups per row
+  const int sub = group / wide;
   const float2* stat = reinterpret_cast<const float2*>(a.stat);
-  for (int r = threadIdx.x / HDP; r < rows; r += PER) {
-    const long long first = (2LL * c0 + 1) * DROWS + r, step = 2LL * DROWS, rest = (2LL * (c0 + 1)) * DROWS + r;
-    float M = stat[first].x;
-    for (int i = 0; i < c1 - c0; ++i) M = fmaxf(M, stat[rest + i * step].x);
-    float2 st = stat[first];
-    float w = st.x == -INFINITY ? 1.f : fast_exp2(st.x - M), den = w * st.y, num = w * a.part[first * HDP + col];
+  const float4* part = reinterpret_cast<const float4*>(a.part);
+  auto slot = [&](int i) { return i == 0 ? 2LL * c - 1 : 2LL * (c - 1 + i); };
+  for (int base = 0; base < j.rows; base += wide) {
+    const int r = base + group % wide;
+    const bool live = r < j.rows;
+    float M = -INFINITY;
+    for (int i = v; i < n && live; i += VEC) M = fmaxf(M, stat[slot(i) * DROWS + r].x);
+#pragma unroll
+    for (int o = VEC / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+    float den = 0.f;
+    if (live) {
 #pragma unroll 4
-    for (int i = 0; i < c1 - c0; ++i) {
-      st = stat[rest + i * step];
-      w = st.x == -INFINITY ? 1.f : fast_exp2(st.x - M);               // without a maximum: sums of zero, or a NaN to hand on
-      den += w * st.y;
-      num += w * a.part[(rest + i * step) * HDP + col];
+      for (int i = sub; i < n; i += subs) {
+        const float2 st = stat[slot(i) * DROWS + r];
+        const float4 x = part[(slot(i) * DROWS + r) * VEC + v];
+        const float w = st.x == -INFINITY ? 1.f : fast_exp2(st.x - M); // without a maximum: sums of zero, or a NaN to hand on
+        den += w * st.y;
+        num.x += w * x.x; num.y += w * x.y; num.z += w * x.z; num.w += w * x.w;
+      }
     }
-    const float v = den == 0.f ? 0.f : num / den;
-    const int tok = (r0 + r) / g.rep;
-    if (col < g.hd) {
-      a.out[((long long)(it.s.q0 + tok) * g.H + it.h * g.rep + (r0 + r) % g.rep) * g.hd + col] = __float2bfloat16(v);
-      if (!isfinite(v)) atomicOr(&bad, 1u << r);
+    sum[group][v] = num;
+    if (v == 0) total[group] = den;
+    __syncthreads();
+    if (sub == 0 && live) {
+      for (int s = 1; s < subs; ++s) {
+        const float4 x = sum[group + s * wide][v];
+        num.x += x.x; num.y += x.y; num.z += x.z; num.w += x.w;
+        den += total[group + s * wide];
+      }
+      const float inv = den == 0.f ? 0.f : 1.f / den;
+      num.x *= inv; num.y *= inv; num.z *= inv; num.w *= inv;
+      if (v * 4 < g.hd) {
+        const int tok = (j.r0 + r) / g.rep, head = j.h * g.rep + (j.r0 + r) - tok * g.rep;
+        *reinterpret_cast<uint2*>(a.out + ((long long)(j.q0 + tok) * g.H + head) * g.hd + v * 4) = make_uint2(pack_bf16(num.x, num.y), pack_bf16(num.z, num.w));
+        if (!(isfinite(num.x) && isfinite(num.y) && isfinite(num.z) && isfinite(num.w))) atomicOr(&bad, 1u << r);
+      }
     }
+    __syncthreads();
   }
-  __syncthreads();
-  for (int r = warp; r < rows; r += 4) {
+  for (int r = warp; r < j.rows; r += 8) {
     if (!(bad >> r & 1u)) continue;
-    const int tok = (r0 + r) / g.rep, head = it.h * g.rep + (r0 + r) % g.rep;
-    const long long at = it.s.q0 + tok;
+    const int tok = (j.r0 + r) / g.rep, head = j.h * g.rep + (j.r0 + r) % g.rep;
+    const long long at = j.q0 + tok;
     float res[HDP / 32];
-    paged_row<HDP>(g, a.q + at * a.qs + head * g.hd, a.pages, it.b, it.h, it.s.kv - it.s.n + tok, a.scale, res);
+    paged_row<HDP>(g, a.q + at * a.qs + head * g.hd, a.pages, j.b, j.h, j.pos0 + tok, a.scale, res);
 #pragma unroll
     for (int x = 0; x < HDP / 32; ++x)
       if (lane + 32 * x < g.hd) a.out[(at * g.H + head) * g.hd + lane + 32 * x] = __float2bfloat16(res[x]);
@@ -407,7 +422,7 @@ int launch_decode(DecodeArgs& a, int page, cudaStream_t st) {
   ::elfa::count_launches(1);
   if (a.whole) return ELFA_OK;
   PdlScope scope(true);
-  ELFA_CUDA(launch_chain(paged_decode_join_kernel<HDP>, dim3(grid - 1), dim3(128), 8 * (a.g.B + 1), st, 1, a, grid));
+  ELFA_CUDA(launch_chain(paged_decode_join_kernel<HDP>, dim3(grid - 1), dim3(256), 0, st, 1, a));
   ELFA_CUDA(cudaGetLastError());
   ::elfa::count_launches(1);
   return ELFA_OK;
@@ -461,7 +476,7 @@ ELFA_API int elfa_paged_attention_scratch(int N, int page, int H, int Hkv, int h
   if (N <= 0 || page <= 0 || Hkv <= 0 || H % Hkv || max_new <= 0) return 0;
   if (many_rows(max_new, H / Hkv)) return (int)paged_prefill_scratch(hd);
   if (decode_whole(max_new, H / Hkv, (long long)N * page)) return 0;
-  return 2 * decode_grid(hd) * DROWS * ((hd <= 64 ? 64 : 128) + 2);
+  return decode_grid(hd) * (2 * DROWS * ((hd <= 64 ? 64 : 128) + 2) + 8);
 }
 
 // q: rows [T] of H heads, `qs` elements apart, heads packed, 16-byte aligned; out: [T, H * hd] contiguous. max_new: at least the most new tokens of a sequence.
@@ -476,7 +491,7 @@ ELFA_API int elfa_paged_attention(const void* q, long long qs, const void* pages
                "paged_attention: query rows must lie on 16-byte boundaries");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (many_rows(max_new, a.g.rep)) {
-    ELFA_REQUIRE(scratch, "paged_attention: no scratch");
+    ELFA_REQUIRE(scratch && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0, "paged_attention: no scratch, or not 16-byte aligned");
     return paged_prefill(a.g, q, qs, pages, out, scratch, page, scale, st);
   }
   a.q = static_cast<const __nv_bfloat16*>(q);
@@ -488,8 +503,9 @@ ELFA_API int elfa_paged_attention(const void* q, long long qs, const void* pages
   a.whole = decode_whole(max_new, a.g.rep, (long long)N * page);
   a.wide = ((long long)max_new * a.g.rep + DROWS - 1) / DROWS > 4;
   a.min_units = MIN_UNITS;
-  ELFA_REQUIRE(a.whole || scratch, "paged_attention: no scratch");
+  ELFA_REQUIRE(a.whole || (scratch && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0), "paged_attention: no scratch, or not 16-byte aligned");
   a.part = scratch;
   a.stat = scratch + 2LL * decode_grid(hd) * DROWS * (hd <= 64 ? 64 : 128);
+  a.notes = reinterpret_cast<PagedJoin*>(a.stat + 2LL * decode_grid(hd) * DROWS * 2);
   return hd <= 64 ? launch_decode<64>(a, page, st) : launch_decode<128>(a, page, st);
 }

@@ -25,6 +25,7 @@ struct PrefillArgs {
   const __nv_bfloat16 *q, *pages;
   __nv_bfloat16* out;
   float *part, *stat;                  // [2 G][2 tiles][HDP / 4][128] float4, [2 G][2 tiles][128] (maximum, sum)
+  PagedJoin* notes;                    // [G]
   long long qs;
   float scale;
   int tile_toks;                       // tokens of one of the two tiles
@@ -62,6 +63,9 @@ __device__ __forceinline__ Part part_of(const PagedGeom& g, const PagedItem& it,
   }
   return p;
 }
+
+// the lowest n bits, n clamped to 0 .. 32
+__device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 
 template <int HDP>
 __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKV,
@@ -103,8 +107,9 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
   const long long W = prefix[g.B];
   const int G = (int)min(W, (long long)gridDim.x);
   const long long u_begin = (int)blockIdx.x < G ? paged_cut(W, G, blockIdx.x) : 0, u_end = (int)blockIdx.x < G ? paged_cut(W, G, blockIdx.x + 1) : 0;
-  PagedItem it;
+  PagedItem it{};
   if (u_begin < u_end) it = paged_find<PBLK>(g, prefix, u_begin);
+  if (threadIdx.x == 0) paged_join_note(g, a.notes, it, W, G, blockIdx.x, u_begin < u_end, u_begin > it.u0);
   pdl_next();
   tc_fence_before();
   __syncthreads();                                         // the prefix makes room for P
@@ -312,15 +317,16 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
         const uint32_t there = __ballot_sync(0xffffffffu, id >= 0) & 0xffu;
         if (lane == 0) mbar_arrive(bar(PB_SREAD + t));
         bool landed = i == p.i0;                           // whether the product before is known to be complete (an item's end waits for it)
-        if (there != 0xffu || (g.window && key0 < pos_max - g.window + 1 && key0 + PBLK > g.sinks)) {
-          const int far = g.window ? lower : 0, keep = g.window ? g.sinks : 0;
+        if (there != 0xffu || key0 + PBLK - 1 > pos_min || (g.window && key0 < pos_max - g.window + 1 && key0 + PBLK > g.sinks)) {
+          // a word of visible keys per 32 columns, then a select by one bit each: tests of every column in turn took 7 us a block where these take 0.3
 #pragma unroll
-          for (int x = 0; x < 128; ++x)
-            if (key0 + x > pos || (key0 + x < far && key0 + x >= keep) || !(there >> (x / 16) & 1u)) s[x] = 0xff800000u;
-        } else if (key0 + PBLK - 1 > pos_min) {
+          for (int c = 0; c < 4; ++c) {
+            const int base = key0 + c * 32;
+            uint32_t see = first_bits(pos + 1 - base) & ((there >> (2 * c) & 1u ? 0xffffu : 0u) | (there >> (2 * c + 1) & 1u ? 0xffff0000u : 0u));
+            if (g.window) see &= ~first_bits(lower - base) | first_bits(g.sinks - base);
 #pragma unroll
-          for (int x = 0; x < 128; ++x)
-            if (key0 + x > pos) s[x] = 0xff800000u;        // -inf
+            for (int x = 0; x < 32; ++x) s[c * 32 + x] = see >> x & 1u ? s[c * 32 + x] : 0xff800000u;      // -inf
+          }
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -389,6 +395,9 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
         ++oc;
       }
       const bool any = n_t > p.i0, whole = p.i0 == 0 && p.i1 == it.span.n;
+      u = min(u_end, it.u0 + it.span.n);
+      PagedItem next = it;
+      if (u < u_end) paged_next<PBLK>(g, next);            // its lengths arrive while the last product runs
       if (ok && any) {
         ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_OFULL + t), (oc - 1) & 1, abort_flag, g.status));
         tc_fence_after();
@@ -398,7 +407,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
         const long long at = it.s.q0 + tok;
         const int head = it.h * g.rep + r - tok * g.rep;
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        __nv_bfloat16* orow = a.out + (at * g.H + head) * g.hd;
+        const long long orow = (at * g.H + head) * g.hd;
         const long long ps = (2LL * blockIdx.x + (p.i0 == 0)) * 2 + t;
         float4* prow = reinterpret_cast<float4*>(a.part) + ps * (HDP / 4) * 128 + row_local;
         bool finite = true;
@@ -406,31 +415,44 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
         for (int c = 0; c < HDP / 32; ++c) {
           uint32_t o[32];
           if (any) {
-            __syncwarp();
             tmem_ld32(TM_O[t] + lane_addr + c * 32, o);
             tmem_ld_wait();
           } else {
 #pragma unroll
             for (int x = 0; x < 32; ++x) o[x] = 0u;
           }
-          if (!valid) continue;
           if (whole) {
+            // through this warp's rows of P: a row's 16-byte pieces next to each other make whole lines (a thread's row at a time: 32 lines per instruction, 3 us)
 #pragma unroll
-            for (int x = 0; x < 32; ++x) {
-              const float v = __uint_as_float(o[x]) * inv;
-              finite = finite && isfinite(v);
-              o[x] = __float_as_uint(v);
+            for (int x = 0; x < 4; ++x) {
+              uint32_t w[4];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                const float v0 = __uint_as_float(o[x * 8 + 2 * y]) * inv, v1 = __uint_as_float(o[x * 8 + 2 * y + 1]) * inv;
+                finite = finite & isfinite(v0) & isfinite(v1);
+                w[y] = pack_bf16(v0, v1);
+              }
+              const int q8 = c * 4 + x;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p_row + (q8 >> 3) * PSUB + (((q8 & 7) ^ (row_local & 7)) << 4)), "r"(w[0]), "r"(w[1]),
+                           "r"(w[2]), "r"(w[3]) : "memory");
             }
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (c * 32 + x * 8 < g.hd)
-                *reinterpret_cast<uint4*>(orow + c * 32 + x * 8) =
-                    make_uint4(pack_bf16(__uint_as_float(o[x * 8]), __uint_as_float(o[x * 8 + 1])), pack_bf16(__uint_as_float(o[x * 8 + 2]), __uint_as_float(o[x * 8 + 3])),
-                               pack_bf16(__uint_as_float(o[x * 8 + 4]), __uint_as_float(o[x * 8 + 5])), pack_bf16(__uint_as_float(o[x * 8 + 6]), __uint_as_float(o[x * 8 + 7])));
-          } else {
+          } else if (valid) {
 #pragma unroll
             for (int x = 0; x < 8; ++x)
               prow[(c * 8 + x) * 128] = make_float4(__uint_as_float(o[x * 4]), __uint_as_float(o[x * 4 + 1]), __uint_as_float(o[x * 4 + 2]), __uint_as_float(o[x * 4 + 3]));
+          }
+          __syncwarp();
+        }
+        if (whole) {
+          constexpr int PIECES = HDP / 8, AT_ONCE = 32 / PIECES;       // 16-byte pieces of a row, rows of an instruction
+#pragma unroll 4
+          for (int y = 0; y < 32 / AT_ONCE; ++y) {
+            const int x = y * AT_ONCE + lane / PIECES, q8 = lane % PIECES, local = quarter * 32 + x;
+            const long long to = __shfl_sync(0xffffffffu, orow, x);
+            uint4 v;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                         : "r"(sbase + L::P + t * 2 * PSUB + local * 128 + (q8 >> 3) * PSUB + (((q8 & 7) ^ (local & 7)) << 4)) : "memory");
+            if (local < rows && q8 * 8 < g.hd) *reinterpret_cast<uint4*>(a.out + to + q8 * 8) = v;
           }
         }
         if (!whole && valid) reinterpret_cast<float2*>(a.stat)[ps * 128 + row_local] = make_float2(m, l);
@@ -450,8 +472,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
         tc_fence_before();
         __syncwarp();
       }
-      u = min(u_end, it.u0 + it.span.n);
-      if (u < u_end) paged_next<PBLK>(g, it);
+      it = next;
     }
   }
 
@@ -464,75 +485,98 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
   }
 }
 
-// Block (c - 1, y) joins rows y, y + Y, ... of the item that the cut between CTAs c - 1 and c goes through, if no earlier cut does: a warp per row.
+// Block (c - 1, y, z) joins 32 rows (y) of the item that CTA c has noted, a thread per row, its warps taking four columns each in turn (of the z-th share of them).
 template <int HDP>
-__global__ void __launch_bounds__(128) paged_prefill_join_kernel(const __grid_constant__ PrefillArgs a, int grid) {
-  extern __shared__ long long prefix[];
-  __shared__ long long warp_tot[4];
+__global__ void __launch_bounds__(256) paged_prefill_join_kernel(const __grid_constant__ PrefillArgs a) {
+  constexpr int VECS = HDP / 4, TURNS = VECS / 8;
+  __shared__ float most[8][32], sums[8][32], weight[32][32];
+  __shared__ uint2 tile[32][VECS + 1];
+  __shared__ unsigned bad_rows;
   const PagedGeom& g = a.g;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  paged_prefix<PBLK, 128>(g, prefix, warp_tot, true);
-  const long long W = prefix[g.B];
-  const int G = (int)min(W, (long long)grid), c = blockIdx.x + 1;
   pdl_wait();
-  if (c >= G) return;
-  const long long u = paged_cut(W, G, c);
-  const PagedItem it = paged_find<PBLK>(g, prefix, u);
-  if (u == it.u0) return;
-  const int c0 = paged_owner(W, G, it.u0), c1 = paged_owner(W, G, it.u0 + it.span.n - 1);
-  if (c0 != c - 1) return;
-  const int half_rows = g.tile_rows >> 1, r0 = it.t * g.tile_rows, rows = min(g.tile_rows, it.s.n * g.rep - r0);
+  const int c = blockIdx.x + 1;
+  const PagedJoin j = a.notes[c];
+  const int half_rows = g.tile_rows >> 1, t = blockIdx.y >> 2, first = (blockIdx.y & 3) * 32, local = first + lane;
+  if (first >= half_rows || t * half_rows + first >= j.rows) return;
+  const bool live = local < half_rows && t * half_rows + local < j.rows;
   const float2* stat = reinterpret_cast<const float2*>(a.stat);
   const float4* part = reinterpret_cast<const float4*>(a.part);
-  constexpr int VECS = HDP / 4;
-  for (int r = blockIdx.y * 4 + warp; r < rows; r += gridDim.y * 4) {
-    const int t = r >= half_rows, local = r - t * half_rows;
-    auto slot = [&](int i) { return (i == 0 ? 2LL * c0 + 1 : 2LL * (c0 + i)) * 2 + t; };
-    const int n = c1 - c0 + 1;
-    float M = -INFINITY;
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, stat[slot(i) * 128 + local].x);
-    M = warp_max(M);
-    float den = 0.f;
-    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      float w = 0.f, wl = 0.f;
-      if (i0 + lane < n) {
-        const float2 st = stat[slot(i0 + lane) * 128 + local];
-        w = st.x == -INFINITY ? 1.f : fast_exp2(st.x - M);             // without a maximum: sums of zero, or a NaN to hand on
-        wl = w * st.y;
-      }
-      den += wl;
-      const int m = min(32, n - i0);
-#pragma unroll 4
+  const int n = j.last - c + 2;                                        // parts: CTAs c - 1 to last
+  auto slot = [&](int i) { return (i == 0 ? 2LL * c - 1 : 2LL * (c - 1 + i)) * 2 + t; };
+  float M = -INFINITY;
+  for (int i = warp; i < n && live; i += 8) M = fmaxf(M, stat[slot(i) * 128 + local].x);
+  most[warp][lane] = M;
+  if (threadIdx.x == 0) bad_rows = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) M = fmaxf(M, most[w][lane]);
+  float den = 0.f;
+  float4 num[TURNS];
+#pragma unroll
+  for (int k = 0; k < TURNS; ++k) num[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int k0 = blockIdx.z * TURNS / gridDim.z, k1 = (blockIdx.z + 1) * TURNS / gridDim.z;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int m = min(32, n - i0);
+    for (int i = warp; i < m; i += 8) {
+      const float2 st = live ? stat[slot(i0 + i) * 128 + local] : make_float2(-INFINITY, 0.f);
+      const float w = st.x == -INFINITY ? 1.f : fast_exp2(st.x - M);   // without a maximum: sums of zero, or a NaN to hand on
+      weight[i][lane] = w;
+      den += w * st.y;
+    }
+    __syncthreads();
+    if (live)
+#pragma unroll 2
       for (int i = 0; i < m; ++i) {
-        const float f = __shfl_sync(0xffffffffu, w, i);
-        if (lane < VECS) {
-          const float4 v = part[(slot(i0 + i) * VECS + lane) * 128 + local];
-          num.x += f * v.x; num.y += f * v.y; num.z += f * v.z; num.w += f * v.w;
+        const float w = weight[i][lane];
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k) {
+          if (k < k0 || k >= k1) continue;
+          const float4 x = part[(slot(i0 + i) * VECS + k * 8 + warp) * 128 + local];
+          num[k].x += w * x.x; num[k].y += w * x.y; num[k].z += w * x.z; num[k].w += w * x.w;
         }
       }
-    }
-    den = warp_sum(den);
-    const float inv = den == 0.f ? 0.f : 1.f / den;
-    const float v[4] = {num.x * inv, num.y * inv, num.z * inv, num.w * inv};
-    const bool bad = __any_sync(0xffffffffu, !(isfinite(v[0]) && isfinite(v[1]) && isfinite(v[2]) && isfinite(v[3])));
-    const int tok = (r0 + r) / g.rep, head = it.h * g.rep + (r0 + r) - tok * g.rep;
-    const long long at = it.s.q0 + tok;
-    __nv_bfloat16* po = a.out + (at * g.H + head) * g.hd;
-    if (!bad) {
-      if (lane * 4 < g.hd) *reinterpret_cast<uint2*>(po + lane * 4) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-      continue;
-    }
-    float res[HDP / 32];
-    paged_row<HDP>(g, a.q + at * a.qs + head * g.hd, a.pages, it.b, it.h, it.s.kv - it.s.n + tok, a.scale, res);
+    __syncthreads();
+  }
+  sums[warp][lane] = den;
+  __syncthreads();
+  den = 0.f;
 #pragma unroll
-    for (int x = 0; x < HDP / 32; ++x)
-      if (lane + 32 * x < g.hd) po[lane + 32 * x] = __float2bfloat16(res[x]);
+  for (int w = 0; w < 8; ++w) den += sums[w][lane];
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  bool finite = true;
+#pragma unroll
+  for (int k = 0; k < TURNS; ++k) {
+    if (k < k0 || k >= k1) continue;
+    const float x = num[k].x * inv, y = num[k].y * inv, z = num[k].z * inv, w = num[k].w * inv;
+    finite = finite & isfinite(x) & isfinite(y) & isfinite(z) & isfinite(w);
+    tile[lane][k * 8 + warp] = make_uint2(pack_bf16(x, y), pack_bf16(z, w));
+  }
+  if (live && !finite) atomicOr(&bad_rows, 1u << lane);
+  __syncthreads();
+  const unsigned bad = bad_rows;
+  for (int x = warp; x < 32; x += 8) {
+    const int r = j.r0 + t * half_rows + first + x;
+    if (first + x >= half_rows || t * half_rows + first + x >= j.rows) continue;
+    const int tok = r / g.rep, head = j.h * g.rep + r - tok * g.rep;
+    const long long at = j.q0 + tok;
+    __nv_bfloat16* po = a.out + (at * g.H + head) * g.hd;
+    if (bad >> x & 1u) {
+      float res[HDP / 32];
+      paged_row<HDP>(g, a.q + at * a.qs + head * g.hd, a.pages, j.b, j.h, j.pos0 + tok, a.scale, res);
+#pragma unroll
+      for (int k = 0; k < HDP / 32; ++k) {
+        const int col = lane + 32 * k;
+        if (col < g.hd && col / 32 >= k0 && col / 32 < k1) po[col] = __float2bfloat16(res[k]);
+      }
+    } else if (lane < VECS && lane * 4 < g.hd && lane / 8 >= k0 && lane / 8 < k1) {
+      *reinterpret_cast<uint2*>(po + lane * 4) = tile[x][lane];
+    }
   }
 }
 
 template <int HDP>
-int launch_prefill(PrefillArgs& a, int page, int join_y, cudaStream_t st) {
+int launch_prefill(PrefillArgs& a, int page, int join_z, cudaStream_t st) {
   CUtensorMap tmQ, tmKV;
   int rc = make_paged_tmap(&tmKV, a.pages, a.g.P, a.g.Hkv, page, a.g.hd, page < PBLK ? page : PBLK);
   if (rc != ELFA_OK) return rc;
@@ -547,7 +591,7 @@ int launch_prefill(PrefillArgs& a, int page, int join_y, cudaStream_t st) {
   ELFA_CUDA(cudaGetLastError());
   ::elfa::count_launches(1);
   PdlScope scope(true);
-  ELFA_CUDA(launch_chain(paged_prefill_join_kernel<HDP>, dim3(grid - 1, join_y), dim3(128), 8 * (a.g.B + 1), st, 1, a, grid));
+  ELFA_CUDA(launch_chain(paged_prefill_join_kernel<HDP>, dim3(grid - 1, 8, join_z), dim3(256), 0, st, 1, a));
   ELFA_CUDA(cudaGetLastError());
   ::elfa::count_launches(1);
   return ELFA_OK;
@@ -555,7 +599,7 @@ int launch_prefill(PrefillArgs& a, int page, int join_y, cudaStream_t st) {
 
 }  // namespace
 
-long long paged_prefill_scratch(int hd) { return 2LL * 148 * 2 * 128 * ((hd <= 64 ? 64 : 128) + 2); }
+long long paged_prefill_scratch(int hd) { return 148LL * (2 * 2 * 128 * ((hd <= 64 ? 64 : 128) + 2) + 8); }
 
 int paged_prefill(PagedGeom g, const void* q, long long qs, const void* pages, void* out, float* scratch, int page, float scale, cudaStream_t st) {
   PrefillArgs a{};
@@ -569,10 +613,11 @@ int paged_prefill(PagedGeom g, const void* q, long long qs, const void* pages, v
   a.g.tile_rows = 2 * a.tile_toks * g.rep;
   a.part = scratch;
   a.stat = scratch + 2LL * 148 * 2 * 128 * (g.hd <= 64 ? 64 : 128);
-  // items are cut into about 148 / items parts each: more blocks per item where there are many parts to read
+  a.notes = reinterpret_cast<PagedJoin*>(a.stat + 2LL * 148 * 2 * 128 * 2);
+  // few items have many parts each: their columns go to several blocks too (a slice of 32 columns each)
   const long long items = g.Hkv * ((long long)g.T * g.rep / a.g.tile_rows + 1);
-  const int join_y = (int)(items >= 74 ? 8 : (items >= 16 ? 16 : 64));
-  return g.hd <= 64 ? launch_prefill<64>(a, page, join_y, st) : launch_prefill<128>(a, page, join_y, st);
+  const int join_z = items < 16 ? (g.hd <= 64 ? 2 : 4) : 1;
+  return g.hd <= 64 ? launch_prefill<64>(a, page, join_z, st) : launch_prefill<128>(a, page, join_z, st);
 }
 
 }  // namespace elfa
