@@ -48,8 +48,10 @@ __device__ __forceinline__ float value_of(unsigned long long c) {
 struct SampleShared {
   union {
     unsigned int hist[BINS];               // tokens per bin of this CTA's part of the row
-    unsigned long long list[LIST];         // places, in the row's first CTA
+    unsigned long long list[LIST];         // places of its tokens in the window; in the first CTA then of all of them, in order
   };
+  unsigned int merged[BINS];               // tokens per bin of the row, in the first CTA
+  unsigned long long swap[LIST];
   double2 mail[2][8];                      // what the CTAs of the row send each other, by turns
   double2 red[SW];
   double scan[3][SW];
@@ -86,31 +88,51 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
   constexpr int PER = 16 / sizeof(T);
   const int head = min(V, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)));
   const int vecs = (V - head) / PER, v0 = (int)((long long)vecs * rank / C), v1 = (int)((long long)vecs * (rank + 1) / C);
-  auto each = [&](auto&& f) {
-    auto value = [](T v) {
-      float y;
-      if constexpr (std::is_same<T, float>::value) y = v;
-      else y = __bfloat162float(v);
-      return y != y ? -CUDART_INF_F : y;
+  auto value = [](T v) {
+    float y;
+    if constexpr (std::is_same<T, float>::value) y = v;
+    else y = __bfloat162float(v);
+    return fmaxf(y, -CUDART_INF_F);        // of a NaN and -inf the latter
+  };
+  // f(values, first indices, std::integral_constants of the number of runs and of a run's length): up to four vectors of 16 bytes at once
+  auto each_batch = [&](auto runs, auto&& f) {
+    constexpr int U = runs.value;
+    auto single = [&](int i) {
+      const float v[1][1] = {{value(x[i])}};
+      const int at[1] = {i};
+      f(v, at, std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}, 1);
     };
-    if (rank == 0 && tid < head) f(value(x[tid]), tid);
-    const int tail = head + vecs * PER;
-    if (rank == C - 1 && tail + tid < V) f(value(x[tail + tid]), tail + tid);
+    if (rank == 0 && tid < head) single(tid);
     const uint4* xv = reinterpret_cast<const uint4*>(x + head);
-    constexpr int U = 4;
     for (int v = v0 + tid; v < v1; v += U * ST) {
       uint4 w[U];
+      float y[U][PER];
+      int at[U];
+      const int n = min(U, (v1 - v + ST - 1) / ST);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (v + u * ST < v1) w[u] = __ldg(xv + v + u * ST);
+        if (u < n) w[u] = __ldg(xv + v + u * ST);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (v + u * ST >= v1) break;
         const T* e = reinterpret_cast<const T*>(&w[u]);
+        at[u] = head + (v + u * ST) * PER;
 #pragma unroll
-        for (int k = 0; k < PER; ++k) f(value(e[k]), head + (v + u * ST) * PER + k);
+        for (int k = 0; k < PER; ++k) y[u][k] = value(e[k]);
       }
+      f(y, at, std::integral_constant<int, U>{}, std::integral_constant<int, PER>{}, n);
     }
+    const int tail = head + vecs * PER;
+    if (rank == C - 1 && tail + tid < V) single(tail + tid);
+  };
+  auto each = [&](auto&& f) {
+    each_batch(std::integral_constant<int, 4>{}, [&](auto& v, auto& at, auto runs, auto len, int n) {
+#pragma unroll
+      for (int u = 0; u < runs.value; ++u) {
+        if (u >= n) break;
+#pragma unroll
+        for (int k = 0; k < len.value; ++k) f(v[u][k], at[u] + k);
+      }
+    });
   };
   // ---- sums and maxima over the row, the same in every thread of the cluster
   int turn = 0;
@@ -148,30 +170,44 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
   };
 
   const int kr = a.top_k ? a.top_k[b] : a.top_k_all, k = kr > 0 && kr < V ? kr : V;
-  const float temp = a.temperature ? a.temperature[b] : a.temperature_all, p = a.top_p ? a.top_p[b] : a.top_p_all,
+  const float asked = a.temperature ? a.temperature[b] : a.temperature_all, temp = fminf(asked, 1e30f), p = a.top_p ? a.top_p[b] : a.top_p_all,
               min_p = a.min_p ? a.min_p[b] : a.min_p_all;
   if (C > 1) cluster_sync_all();           // every CTA of the row has started
-  unsigned long long best = 0;
-  each([&](float v, int i) { best = max(best, place(v, i)); });
-  best = most(best);
-  const float mx = value_of(best);
-  if (mx == -CUDART_INF_F || !(temp > 0.f)) {
-    if (rank == 0 && tid == 0) a.out[b] = mx == -CUDART_INF_F ? -1 : index_of(best);
+  float mx = -CUDART_INF_F;
+  each([&](float v, int) { mx = fmaxf(mx, v); });
+  mx = value_of(most(place(mx, 0)));
+  if (mx == -CUDART_INF_F || !(asked > 0.f)) {
+    unsigned long long first = 0;          // of the largest, the one with the lowest index
+    if (mx != -CUDART_INF_F)
+      each([&](float v, int i) {
+        if (v == mx) first = max(first, place(v, i));
+      });
+    first = most(first);
+    if (rank == 0 && tid == 0) a.out[b] = index_of(first);             // -1 of 0
     return;
   }
   auto weight = [&](float v) { return v == mx ? 1.f : expf((v - mx) / temp); };
-  const float fast = 1.4426950408889634f / temp;
-  auto rough = [&](float v) { return v == mx ? 1.f : fast_exp2((v - mx) * fast); };       // for the sums: 2^-22 of each, of what weighs little a bit more
-  unsigned long long win = (uint32_t)best;                                                // score 0 of the first largest, should no other compare
+  // y = 256 (mx - v) / T, 0 for the largest whatever it is (inf - inf is a NaN), never falling as v falls; exp(-y / 256) for the sums: 2^-22 of each
+  const float per = fminf(BINS_PER / temp, 1e30f);
+  auto depth = [&](float v) { return fmaxf(mx - v, 0.f) * per; };
+  auto rough = [&](float y) { return fast_exp2(y * (-1.4426950408889634f / BINS_PER)); };
+  unsigned long long win = 0;
   auto race = [&](float w, int i) {
     const float sc = w / noise[i];
     if (sc >= 0.f) win = max(win, (unsigned long long)__float_as_uint(sc) << 32 | (uint32_t)~i);
   };
+  // what is kept: cut and all before it in the order
   unsigned long long cut = 0;
+  float last_value = -CUDART_INF_F;
+  int last_index = V;
+  auto keep_to = [&](unsigned long long c) {
+    if (c == 0) return;
+    last_value = value_of(c);
+    last_index = index_of(c);
+  };
+  auto kept = [&](float v, int i) { return v > last_value || (v == last_value && i <= last_index); };
 
   if (k < V || p < 1.f) {
-    const float per = BINS_PER / temp;
-    auto bin_of = [&](float v) { return v == mx ? 0 : (int)fminf((mx - v) * per, BINS - 1.f); };     // never falls as v falls, whatever it rounds to
     for (int i = tid; i < BINS; i += ST) s.hist[i] = 0;
     if (tid == 0) s.fill = 0;
     __syncthreads();
@@ -179,30 +215,40 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     float sum = 0.f;
     unsigned int rest = 0;                                 // what weighs less than 2^-46, often most of the row, would meet in one word
     each([&](float v, int) {
-      const int bin = bin_of(v);
-      if (bin == BINS - 1) ++rest;
-      else atomicAdd(&s.hist[bin], 1u);
-      if (want_all) sum += rough(v);
+      const float y = depth(v);
+      if (y >= BINS - 1.f) ++rest;
+      else atomicAdd(&s.hist[(int)y], 1u);
+      if (want_all) sum += rough(y);
     });
     if (rest) atomicAdd(&s.hist[BINS - 1], rest);
-    double mass = want_all ? total(sum, 0.0).x : 0.0;      // of what top-k keeps
-    meet();                                                // all of the row is counted
-    // ---- the row's first CTA adds the bins up: 16 neighbouring ones per thread
+    double mass = 0.0;                                     // of what top-k keeps
+    if (want_all) mass = total(sum, 0.0).x;
+    else meet();
+    // all of the row is counted
+    // ---- each CTA adds a share of the bins up, for the row's first one: there 16 neighbouring bins per thread
     constexpr int OWN = BINS / ST;
-    unsigned int cnt[OWN];
-    if (rank == 0) {
+    const int share = BINS / 4 / C;
+    for (int i = rank * share + tid; i < (rank + 1) * share; i += ST) {
+      uint4 h[8];
 #pragma unroll
-      for (int j = 0; j < OWN; ++j) cnt[j] = 0;
-      for (int r = 0; r < C; ++r) {
-        const uint4* h = reinterpret_cast<const uint4*>(peer(s.hist, r)) + tid * (OWN / 4);
+      for (int r = 0; r < 8; ++r)
+        if (r < C) h[r] = reinterpret_cast<const uint4*>(peer(s.hist, r))[i];
+      uint4 sum4 = h[0];
 #pragma unroll
-        for (int j = 0; j < OWN / 4; ++j) {
-          const uint4 v = h[j];
-          cnt[4 * j] += v.x; cnt[4 * j + 1] += v.y; cnt[4 * j + 2] += v.z; cnt[4 * j + 3] += v.w;
+      for (int r = 1; r < 8; ++r)
+        if (r < C) {
+          sum4.x += h[r].x; sum4.y += h[r].y; sum4.z += h[r].z; sum4.w += h[r].w;
         }
-      }
-      __syncthreads();                                     // the list may take the bins' place
+      reinterpret_cast<uint4*>(peer(s.merged, 0))[i] = sum4;
     }
+    meet();                                                // from here on the list may take the bins' place
+    auto load_counts = [&](unsigned int (&cnt)[OWN]) {
+#pragma unroll
+      for (int j = 0; j < OWN / 4; ++j) {
+        const uint4 v = reinterpret_cast<const uint4*>(s.merged)[tid * (OWN / 4) + j];
+        cnt[4 * j] = v.x; cnt[4 * j + 1] = v.y; cnt[4 * j + 2] = v.z; cnt[4 * j + 3] = v.w;
+      }
+    };
     // sums before this thread: v over the first CTA's threads
     auto before_me = [&](double (&v)[3]) {
       double incl[3] = {v[0], v[1], v[2]};
@@ -225,9 +271,12 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
       }
     };
     const int bin0 = tid * OWN;
-    // The window (first CTA): where the number of tokens reaches `want`, or bounds of the mass do. A bin's tokens weigh between exp(-(bin + 1) / 256) and
-    // exp(-bin / 256); those of bin `last`, of which not all may count, between nothing and that.
+    // The window (first CTA): where the number of tokens reaches `want`, or the mass may. A bin's tokens weigh between exp(-(bin + 1) / 256) and
+    // exp(-bin / 256); those of bin `last`, of which not all may count, between nothing and that. `wide` takes the bounds; else the middle of the bin stands for
+    // them, with 2^-11 to either side, which holds nearly always and leaves an eighth of the tokens to sort; what the list then holds shows whether it did.
     auto window_of_count = [&](double want) {
+      unsigned int cnt[OWN];
+      load_counts(cnt);
       double at[3] = {0, 0, 0};
 #pragma unroll
       for (int j = 0; j < OWN; ++j) at[0] += cnt[j];
@@ -243,34 +292,48 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
       }
       __syncthreads();
     };
-    auto window_of_mass = [&](double want, int last) {
-      auto high = [&](int j) { return cnt[j] * (double)expf(-(bin0 + j) / BINS_PER); };
-      auto low = [&](int j) { return bin0 + j < last ? cnt[j] * (double)expf(-(bin0 + j + 1) / BINS_PER) : 0.0; };
-      double at[3] = {0, 0, 0};
+    auto window_of_mass = [&](double want, int last, bool wide) {
+      unsigned int cnt[OWN];
+      load_counts(cnt);
+      constexpr float RATIO = 0.99610137f;                 // exp(-1 / 256)
+      const float edge = expf(-bin0 / BINS_PER) * (wide ? 1.f : 0.99804878f);          // exp(-1 / 512)
+      const double shrink = wide ? RATIO : 1.0, gap = wide ? 1e-5 : 0x1p-11;           // 1e-5: more than the sums' and the weights' rounding
+      float w = edge, sum = 0.f;
+      unsigned int n = 0;
 #pragma unroll
       for (int j = 0; j < OWN; ++j) {
-        if (bin0 + j > last) continue;
-        at[0] += cnt[j];
-        at[1] += high(j);
-        at[2] += low(j);
+        if (bin0 + j <= last) {
+          n += cnt[j];
+          sum += cnt[j] * w;
+        }
+        w *= RATIO;
       }
+      double at[3] = {(double)n, sum, 0};
       before_me(at);
-      const double up = want * (1 - 1e-5), down = want * (1 + 1e-5);         // more than the sums' and the weights' rounding
+      const double up = want * (1 - gap), down = want * (1 + gap);
+      const bool ends_here = bin0 <= last && bin0 + OWN > last;
+      const double behind = (at[1] + sum) * (1 + 1e-6);
+      if ((at[1] < up && behind >= up) || (at[1] * shrink < down && behind * shrink >= down) || ends_here) {
+        w = edge;
+        double high = at[1], count = at[0];
 #pragma unroll
-      for (int j = 0; j < OWN; ++j) {
-        const int bin = bin0 + j;
-        if (bin > last) continue;
-        if (at[1] < up && (at[1] + high(j) >= up || bin == last)) {
-          s.b1 = bin;
-          s.before = (long long)at[0];
+        for (int j = 0; j < OWN; ++j) {
+          const int bin = bin0 + j;
+          if (bin > last) continue;
+          double next = high + cnt[j] * w;
+          if (j == OWN - 1 || bin == last) next = fmax(next, at[1] + sum);   // what the next thread starts from
+          if (high < up && (next >= up || bin == last)) {
+            s.b1 = bin;
+            s.before = (long long)count;
+          }
+          if (high * shrink < down && (next * shrink >= down || bin == last)) {
+            s.b2 = bin;
+            s.upto = (long long)(count + cnt[j]);
+          }
+          count += cnt[j];
+          high = next;
+          w *= RATIO;
         }
-        if (at[2] < down && (at[2] + low(j) >= down || bin == last)) {
-          s.b2 = bin;
-          s.upto = (long long)(at[0] + cnt[j]);
-        }
-        at[0] += cnt[j];
-        at[1] += high(j);
-        at[2] += low(j);
       }
       __syncthreads();
     };
@@ -284,41 +347,84 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
       }
     };
     // the window's tokens (those not behind `least`) to the list; the mass of the ones before the window
-    auto collect = [&](unsigned long long least) {
-      const int b1 = s.b1, b2 = s.b2;
-      int* fill = peer(&s.fill, 0);
-      unsigned long long* list = peer(s.list, 0);
+    auto collect = [&]() {
+      const float from = (float)s.b1, to = s.b2 == BINS - 1 ? CUDART_INF_F : (float)(s.b2 + 1);
       float sum = 0.f;
       each([&](float v, int i) {
-        const int bin = bin_of(v);
-        if (bin < b1) sum += rough(v);
-        else if (bin <= b2 && place(v, i) >= least) {
-          const int at = atomicAdd(fill, 1);
-          if (at < LIST) list[at] = place(v, i);
-        }
+        const float y = depth(v), w = rough(y);
+        if (y < from) sum += w;
+        else if ((y < to || to == CUDART_INF_F) && kept(v, i)) s.list[atomicAdd(&s.fill, 1)] = place(v, i);      // the window's count fits
       });
-      return total(sum, 0.0).x;
+      __syncthreads();
+      const int fill = s.fill;
+      const double2 all = total(sum, tid == 0 ? fill : 0);
+      if (C > 1) {                                         // behind those of the CTAs before, in the first one
+        int at = 0;
+        for (int r = 0; r < rank; ++r) at += (int)s.mail[turn ^ 1][r].y;
+        unsigned long long* to0 = peer(s.swap, 0);
+        for (int i = tid; i < fill; i += ST) to0[at + i] = s.list[i];
+        cluster_sync_all();
+      } else {
+        for (int i = tid; i < fill; i += ST) s.swap[i] = s.list[i];
+        __syncthreads();
+      }
+      return all;
     };
-    // first CTA: the list in order
-    auto sort = [&]() {
-      const int n = min(s.fill, LIST);
-      int m = 2;
-      while (m < n) m <<= 1;
-      for (int i = n + tid; i < m; i += ST) s.list[i] = 0;
+    // first CTA: all lists to one, in order: a bitonic network, E neighbouring entries per thread in registers, exchanges between warps through shared memory
+    auto order = [&](auto per_thread, int m) {
+      constexpr int E = per_thread.value;
+      unsigned long long e[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) e[j] = s.swap[tid * E + j];
+      unsigned long long* buf = s.list;
       for (int size = 2; size <= m; size <<= 1)
         for (int step = size >> 1; step > 0; step >>= 1) {
-          __syncthreads();
-          for (int i = tid; i < m / 2; i += ST) {
-            const int l = 2 * i - (i & (step - 1)), h = l + step;
-            const unsigned long long u = s.list[l], v = s.list[h];
-            if ((u < v) == ((l & size) == 0)) {            // falling
-              s.list[l] = v;
-              s.list[h] = u;
+          if (step < E) {
+#pragma unroll
+            for (int st = 1; st < E; st <<= 1) {
+              if (st != step) continue;
+#pragma unroll
+              for (int j = 0; j < E; ++j)
+                if (!(j & st)) {
+                  const bool fall = ((tid * E + j) & size) == 0;
+                  const unsigned long long u = e[j], v = e[j | st];
+                  if ((u < v) == fall) {
+                    e[j] = v;
+                    e[j | st] = u;
+                  }
+                }
             }
+          } else {
+            if (step >= 32 * E) {
+#pragma unroll
+              for (int j = 0; j < E; ++j) buf[j * ST + tid] = e[j];
+              __syncthreads();
+            }
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+              const int i = tid * E + j;
+              const unsigned long long o = step >= 32 * E ? buf[j * ST + (tid ^ (step / E))] : __shfl_xor_sync(0xffffffffu, e[j], step / E);
+              const bool larger = ((i & step) == 0) == ((i & size) == 0);
+              e[j] = larger ? max(e[j], o) : min(e[j], o);
+            }
+            if (step >= 32 * E) buf = buf == s.swap ? s.list : s.swap;       // the next exchange's place: nobody reads it any more behind its barrier
           }
         }
       __syncthreads();
-      return n;
+#pragma unroll
+      for (int j = 0; j < E; ++j) s.list[tid * E + j] = e[j];
+      __syncthreads();
+    };
+    auto sort = [&](int n) {
+      int m = 2;
+      while (m < n) m <<= 1;
+      const int room = max(m, ST);
+      for (int i = n + tid; i < room; i += ST) s.swap[i] = 0;
+      __syncthreads();
+      if (m <= ST) order(std::integral_constant<int, 1>{}, m);
+      else if (m <= 2 * ST) order(std::integral_constant<int, 2>{}, m);
+      else if (m <= 4 * ST) order(std::integral_constant<int, 4>{}, m);
+      else order(std::integral_constant<int, 8>{}, m);
     };
     // first CTA: the mass of the first n of the list, and how many of them it takes until base + mass >= want (n, if that is not reached) in s.pos
     auto prefix = [&](int n, double base, double want) {
@@ -373,14 +479,16 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         cut = search(k, [](float) { return 1.0; });
         if (p < 1.f) {
           double m = 0;
-          each([&](float v, int i) { m += place(v, i) >= cut ? (double)rough(v) : 0.0; });
+          each([&](float v, int i) { m += place(v, i) >= cut ? (double)rough(depth(v)) : 0.0; });
           mass = total(m, 0.0).x;
         }
       } else {
-        const double above = collect(0);
+        const double2 got = collect();
+        const double above = got.x;
         if (mode == SORT_ALL) {                            // the list holds all that can be kept
           if (rank != 0) return;
-          int n = min(sort(), k);
+          sort((int)got.y);
+          int n = min((int)got.y, k);
           if (p < 1.f) {
             const double m = prefix(n, 0.0, -1.0);
             prefix(n, 0.0, fmax((double)p * m, 1e-30));
@@ -402,7 +510,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
           return;
         }
         if (rank == 0) {
-          sort();
+          sort((int)got.y);
           const int n = (int)(k - s.before);
           const double m = p < 1.f ? prefix(n, above, 1e300) : 0.0;
           if (tid < C) {
@@ -410,59 +518,106 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
             d->cut = s.list[n - 1];
             d->mass = m;
           }
-          __syncthreads();
-          if (tid == 0) s.fill = 0;
         }
         meet();
         cut = s.cut;
         mass = s.mass;
+        __syncthreads();
+        if (tid == 0) s.fill = 0;          // for the next window; read and counted on behind the barriers before that
       }
       if (rank == 0 && tid == 0) s.b2 = last;
     }
     if (p < 1.f) {
       const double want = fmax((double)p * mass, 1e-30);   // a share of nothing still takes the first token
-      if (rank == 0) {
+      int last = BINS - 1;
+      if (k < V) {
         __syncthreads();
-        const int last = k < V ? s.b2 : BINS - 1;
+        last = s.b2;
         __syncthreads();
-        window_of_mass(want, last);
-        if (tid == 0) tell(s.upto - s.before <= LIST ? SORT_WINDOW : SEARCH);
       }
-      meet();
-      const double above = s.mode == SEARCH ? 0.0 : collect(cut);
-      int found = 0;
-      if (s.mode != SEARCH) {
+      bool found = false;
+      for (int wide = 0; wide < 2 && !found; ++wide) {
         if (rank == 0) {
-          const int n = sort();
-          if (n > 0) prefix(n, above, want);
-          if (tid < C) {
-            SampleShared* d = peer(&s, tid);
-            d->cut = n > 0 ? s.list[s.pos - 1] : 0;
-          }
+          window_of_mass(want, last, wide);
+          if (tid == 0) tell(s.upto - s.before <= LIST ? SORT_WINDOW : SEARCH);
         }
+        meet();
+        if (s.mode == SEARCH) break;
+        keep_to(cut);
+        const double2 got = collect();
+        if (rank == 0) {
+          const int n = (int)got.y;
+          sort(n);
+          bool holds = n > 0;
+          if (n > 0) {
+            const double m = prefix(n, got.x, want);
+            holds = wide || (got.x < want && m >= want);
+          }
+          if (tid < C) peer(&s, tid)->cut = holds ? s.list[s.pos - 1] : 0;
+          __syncthreads();
+        }
+        if (tid == 0) s.fill = 0;
         meet();
         if (s.cut) {
           cut = s.cut;
-          found = 1;
+          found = true;
         }
       }
-      if (!found) cut = max(cut, search(want, [&](float v) { return (double)rough(v); }));
+      if (!found) cut = max(cut, search(want, [&](float v) { return (double)rough(depth(v)); }));
     }
   }
-  each([&](float v, int i) {
-    if (place(v, i) < cut) return;
-    const float w = weight(v);
-    if (w >= min_p) race(w, i);
+  // A rough score of every token, the exact one of the best of each thread; of all of its tokens where another one (or the line of min_p) was within 10^-4, more than
+  // the rough scores are off. The variates of a batch are asked for at once.
+  keep_to(cut);
+  float bar = -1.f;
+  int bar_at = 0;
+  bool close = false;
+  float bar_value = 0.f;
+  const float least = fmaxf(min_p, 0.f) * (1.f - 1e-5f), sure = min_p * (1.f + 1e-5f);
+  each_batch(std::integral_constant<int, 16 / PER>{}, [&](auto& v, auto& at, auto runs, auto len, int n) {
+    float w[runs.value][len.value], e[runs.value][len.value];
+#pragma unroll
+    for (int u = 0; u < runs.value; ++u)
+#pragma unroll
+      for (int q = 0; q < len.value; ++q) {
+        w[u][q] = u < n && kept(v[u][q], at[u] + q) ? rough(depth(v[u][q])) : -1.f;
+        e[u][q] = 1.f;
+        if (w[u][q] >= least) e[u][q] = __ldg(noise + at[u] + q);
+      }
+#pragma unroll
+    for (int u = 0; u < runs.value; ++u)
+#pragma unroll
+      for (int q = 0; q < len.value; ++q) {
+        if (!(w[u][q] >= least)) continue;
+        const float sc = __fdividef(w[u][q], e[u][q]);
+        close = close | (w[u][q] < sure) | !(fabsf(sc - bar) > 1e-4f * fmaxf(sc, bar));            // equal infinities and NaN too
+        if (sc > bar) {
+          bar = sc;
+          bar_at = at[u] + q;
+          bar_value = v[u][q];
+        }
+      }
   });
+  if (close) {
+    each([&](float v, int i) {
+      if (!kept(v, i)) return;
+      const float w = weight(v);
+      if (w >= min_p) race(w, i);
+    });
+  } else if (bar >= 0.f) {
+    race(weight(bar_value), bar_at);
+  }
   win = most(win);
   if (rank == 0 && tid == 0) a.out[b] = index_of(win);
 }
 
 template <typename T>
 int launch_sample(const SampleArgs& a, int B, cudaStream_t st) {
-  // CTAs per row: a part of 16384 logits or less each, and while the rows leave SMs idle, down to 4096
+  // CTAs per row: as many as run at once (two per SM; half a wave more is still faster: 96 rows of 131072 take 190, 125, 117 and 147 us on 1, 2, 4 and 8), none
+  // with less than 4096 logits (a row of 32000: 22.7, 22.5, 20.5 and 18.5 us)
   int C = 1;
-  while (C < 8 && ((long long)a.V > 16384LL * C || (B * C * 2 <= 148 && (long long)a.V > 4096LL * C))) C *= 2;
+  while (C < 8 && a.V > 4096LL * C && (long long)B * C * 2 <= 444) C *= 2;
+  ELFA_CUDA(allow_shared<sample_kernel<T>>((int)sizeof(SampleShared)));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)B * C);
   cfg.blockDim = dim3(ST);
