@@ -4,10 +4,11 @@
 // heads that share a key head read its keys once: with rep heads per group a tile holds 128 / rep tokens, one TMA box {64 columns, rep heads, 128 / rep tokens}
 // per 64 columns. A CTA walks its share of the line of units (paged.cuh) with everything in flight across items: per pair of tiles and block of 128 keys
 //   warp 0      : TMA: queries once per item, keys one block ahead in two stages, values; a box per page
-//   warp 1      : every tcgen05.mma: S = Q K^T of the next block before O += P V of this one, also over the end of an item
+//   warp 1      : S = Q K^T, block by block, tile 0 then tile 1, into one S buffer: a product is issued when the rows of the one before have been read
+//   warp 3      : O += P V as the rows of P arrive (of its own, so that neither waits for the other's barriers)
 //   warp 2      : clears the value rows behind a sequence's last token before they are multiplied (what lies there may be anything)
 //   warps 4-11  : softmax and sums of tile 0 and tile 1, a thread per row, as in attention_fwd.cu: the whole S row in registers, P to shared memory in
-//                 bf16, O in tensor memory, scaled again when a row's maximum grows by more than 2^8
+//                 O in tensor memory, scaled again when a row's maximum grows by more than 2^8
 // Parts of items go to scratch in fp32 and are joined by a second launch. Every wait is bounded.
 #include "elfa_native.h"
 #include "paged.cuh"
@@ -31,16 +32,16 @@ struct PrefillArgs {
   int tile_toks;                       // tokens of one of the two tiles
 };
 
-enum { PB_Q = 0, PB_QFREE, PB_KFULL, PB_KFREE = PB_KFULL + 2, PB_VFULL = PB_KFREE + 2, PB_VFREE, PB_VTAIL, PB_SFULL, PB_SREAD = PB_SFULL + 2,
-       PB_PREADY = PB_SREAD + 2, PB_OFULL = PB_PREADY + 2, PB_COUNT = PB_OFULL + 2 };
+enum { PB_Q = 0, PB_QFREE, PB_KFULL, PB_KFREE = PB_KFULL + 2, PB_VFULL = PB_KFREE + 2, PB_VFREE = PB_VFULL + 2, PB_VTAIL = PB_VFREE + 2,
+       PB_SFULL = PB_VTAIL + 2, PB_SREAD = PB_SFULL + 2, PB_PREADY, PB_OFULL = PB_PREADY + 2, PB_COUNT = PB_OFULL + 2 };
 
 template <int HDP>
 struct PrefillSmem {
   static constexpr int NSUB = HDP / 64;
-  static constexpr int Q = 0, K = Q + 2 * NSUB * PSUB, V = K + 2 * NSUB * PSUB, P = V + NSUB * PSUB, BAR = P + 4 * PSUB;
+  static constexpr int Q = 0, K = Q + 2 * NSUB * PSUB, V = K + 2 * NSUB * PSUB, OUT = V + 2 * NSUB * PSUB, BAR = OUT + 8 * 4096;
   static constexpr int TOTAL = BAR + PB_COUNT * 8 + 16 + 8 * (PTHREADS / 32);
   static constexpr int DYN = TOTAL + 1024;
-  static_assert(8 * (PAGED_MAX_SEQS + 1) <= 4 * PSUB, "the prefix lies where P will");
+  static_assert(8 * (PAGED_MAX_SEQS + 1) <= 8 * 4096, "the prefix lies where outputs will");
 };
 
 // what a CTA does of an item: blocks i0 .. i1 of its list; tile 0 takes part up to n0, tile 1 up to n1
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
     prefetch_tmap(&tmQ);
     prefetch_tmap(&tmKV);
     for (int i = 0; i < PB_COUNT; ++i)
-      mbar_init(bar(i), i == PB_SREAD || i == PB_SREAD + 1 || i == PB_PREADY || i == PB_PREADY + 1 ? 4 : 1);
+      mbar_init(bar(i), i == PB_SREAD || i == PB_PREADY || i == PB_PREADY + 1 ? 4 : 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -102,7 +103,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
     for (int s = 0; s < 2 * NSUB; ++s)
       asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sbase + L::Q + s * PSUB + i * 16), "r"(0) : "memory");
   fence_proxy_async();
-  long long* prefix = reinterpret_cast<long long*>(smem + L::P);
+  long long* prefix = reinterpret_cast<long long*>(smem + L::OUT);
   paged_prefix<PBLK, PTHREADS>(g, prefix, warp_tot, true);
   const long long W = prefix[g.B];
   const int G = (int)min(W, (long long)gridDim.x);
@@ -112,10 +113,10 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
   if (threadIdx.x == 0) paged_join_note(g, a.notes, it, W, G, blockIdx.x, u_begin < u_end, u_begin > it.u0);
   pdl_next();
   tc_fence_before();
-  __syncthreads();                                         // the prefix makes room for P
+  __syncthreads();                                         // the prefix makes room for outputs
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
-  const uint32_t TM_S[2] = {tmem_base + 0, tmem_base + 128};
+  const uint32_t TM_S = tmem_base, TM_P[2] = {tmem_base + 128, tmem_base + 192};
   const uint32_t TM_O[2] = {tmem_base + 256, tmem_base + 256 + HDP};
 
   if (warp < 4) {
@@ -172,111 +173,96 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
             if (fresh) load_q(it);
             load_k(it, (int)(u + 1 - it.u0), next_id);
           }
-          if (vc) wait(PB_VFREE, (vc - 1) & 1);
+          const int st = vc & 1;
+          if (vc >= 2) wait(PB_VFREE + st, ((vc >> 1) - 1) & 1);
           ++vc;
-          if (ok) load(cur, i, id, 1, sbase + L::V, (cur.span.block(i) + 1) * PBLK > cur.s.kv ? PB_VTAIL : PB_VFULL);
+          if (ok) load(cur, i, id, 1, sbase + L::V + st * NSUB * PSUB, ((cur.span.block(i) + 1) * PBLK > cur.s.kv ? PB_VTAIL : PB_VFULL) + st);
           id = next_id;
         }
       }
-    } else if (warp == 1) {
-      // ---------------------------------------------------------------- products
-      constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false), idesc_o = make_idesc_bf16(128, HDP, false, true);
+    } else if (warp == 1 || warp == 3) {
+      // ---------------------------------------------------------------- products: S from warp 1, O from warp 3
       bool ok = true;
-      uint32_t kc = 0, vc = 0, qc = 0, sI[2] = {0, 0}, pI[2] = {0, 0};
       auto wait = [&](int b, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(b), parity, abort_flag, g.status)); };
       auto commit = [&](int b) {
         if (elect_one()) tc_commit(bar(b));
         __syncwarp();
       };
-      const uint64_t dq = make_smem_desc(sbase + L::Q, 16, 1024, 2), dk = make_smem_desc(sbase + L::K, 16, 1024, 2);
-      const uint64_t dp = make_smem_desc(sbase + L::P, 16, 1024, 2), dv = make_smem_desc(sbase + L::V, PSUB, 1024, 2);
-      const uint32_t q_lo = (uint32_t)dq, q_hi = (uint32_t)(dq >> 32), k_lo = (uint32_t)dk, k_hi = (uint32_t)(dk >> 32);
-      const uint32_t p_lo = (uint32_t)dp, p_hi = (uint32_t)(dp >> 32), v_lo = (uint32_t)dv, v_hi = (uint32_t)(dv >> 32);
-      auto scores = [&](const Part& p, int i) {            // S of block i for the tiles that take part
-        const int st = kc & 1;
-        wait(PB_KFULL + st, (kc >> 1) & 1);
-        if (i == p.i0) {
-          wait(PB_Q, qc & 1);
-          ++qc;
-        }
+      uint32_t blocks = 0, parts = 0, done = 0, pI[2] = {0, 0};
+      for (long long u = u_begin; u < u_end && ok;) {
+        const Part p = part_of(g, it, u, u_end);
+        for (int i = p.i0; i < p.i1 && ok; ++i, ++blocks) {
+          const int st = blocks & 1;
+          const uint32_t parity = (blocks >> 1) & 1;
+          if (warp == 1) {
+            constexpr uint32_t idesc = make_idesc_bf16(128, 128, false, false);
+            const uint64_t dq = make_smem_desc(sbase + L::Q, 16, 1024, 2), dk = make_smem_desc(sbase + L::K + st * NSUB * PSUB, 16, 1024, 2);
+            const uint32_t q_lo = (uint32_t)dq, q_hi = (uint32_t)(dq >> 32), k_lo = (uint32_t)dk, k_hi = (uint32_t)(dk >> 32);
+            wait(PB_KFULL + st, parity);
+            if (i == p.i0) wait(PB_Q, parts++ & 1);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (i >= (t ? p.n1 : p.n0)) continue;
-          if (sI[t]) wait(PB_SREAD + t, (sI[t] - 1) & 1);
-          ++sI[t];
-          if (!ok) return;
-          tc_fence_after();
-          if (elect_one()) {
+            for (int t = 0; t < 2; ++t) {
+              if (i >= (t ? p.n1 : p.n0)) continue;
+              if (done) wait(PB_SREAD, (done - 1) & 1);    // the one S buffer: the rows of the product before have been read
+              ++done;
+              if (!ok) break;
+              tc_fence_after();
+              if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < HDP / 16; ++kk) {
-              const uint32_t off = ((kk / 4) * PSUB + (kk % 4) * 32) >> 4;
-              tc_mma_f16_lh(TM_S[t], q_lo + ((t * NSUB * PSUB) >> 4) + off, q_hi, k_lo + ((st * NSUB * PSUB) >> 4) + off, k_hi, idesc_s, kk != 0);
-            }
-            tc_commit(bar(PB_SFULL + t));
-          }
-          __syncwarp();
-        }
-        commit(PB_KFREE + st);
-        ++kc;
-        if (i + 1 == p.i1) commit(PB_QFREE);
-      };
-      if (u_begin < u_end) {
-        Part p = part_of(g, it, u_begin, u_end);
-        scores(p, p.i0);
-        for (long long u = u_begin; u < u_end && ok; ++u) {
-          const Part c = p;
-          const int i = (int)(u - it.u0);
-          if (u + 1 < u_end) {
-            int ni = i + 1;
-            if (ni >= c.i1) {
-              paged_next<PBLK>(g, it);
-              p = part_of(g, it, u + 1, u_end);
-              ni = p.i0;
-            }
-            scores(p, ni);
-            if (!ok) break;
-          }
-          wait(PB_VFULL, vc & 1);
-          ++vc;
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (i >= (t ? c.n1 : c.n0)) continue;
-            wait(PB_PREADY + t, pI[t] & 1);
-            ++pI[t];
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-              for (int kk = 0; kk < 8; ++kk) {
-                const uint32_t off = ((kk / 4) * PSUB + (kk % 4) * 32) >> 4;
-                tc_mma_f16_lh(TM_O[t], p_lo + ((t * 2 * PSUB) >> 4) + off, p_hi, v_lo + ((kk * 2048) >> 4), v_hi, idesc_o, i != c.i0 || kk != 0);
+                for (int kk = 0; kk < HDP / 16; ++kk) {
+                  const uint32_t off = ((kk / 4) * PSUB + (kk % 4) * 32) >> 4;
+                  tc_mma_f16_lh(TM_S, q_lo + ((t * NSUB * PSUB) >> 4) + off, q_hi, k_lo + off, k_hi, idesc, kk != 0);
+                }
+                tc_commit(bar(PB_SFULL + t));
               }
-              tc_commit(bar(PB_OFULL + t));
+              __syncwarp();
             }
-            __syncwarp();
+            if (ok) commit(PB_KFREE + st);
+            if (ok && i + 1 == p.i1) commit(PB_QFREE);
+          } else {
+            constexpr uint32_t idesc = make_idesc_bf16(128, HDP, false, true);
+            const uint64_t dv = make_smem_desc(sbase + L::V + st * NSUB * PSUB, PSUB, 1024, 2);
+            const uint32_t v_lo = (uint32_t)dv, v_hi = (uint32_t)(dv >> 32);
+            wait(PB_VFULL + st, parity);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (i >= (t ? p.n1 : p.n0)) continue;
+              wait(PB_PREADY + t, pI[t]++ & 1);
+              if (!ok) break;
+              tc_fence_after();
+              if (elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk) tc_mma_f16_ts_lh(TM_O[t], TM_P[t] + kk * 8, v_lo + ((kk * 2048) >> 4), v_hi, idesc, i != p.i0 || kk != 0);
+                tc_commit(bar(PB_OFULL + t));
+              }
+              __syncwarp();
+            }
+            if (ok) commit(PB_VFREE + st);
           }
-          if (ok) commit(PB_VFREE);
         }
+        u = it.u0 + p.i1;
+        if (u < u_end) paged_next<PBLK>(g, it);
       }
     } else if (warp == 2) {
       // ---------------------------------------------------------------- value rows that hold no token
-      uint32_t tails = 0;
+      uint32_t tails[2] = {0, 0}, blocks = 0;
       for (long long u = u_begin; u < u_end;) {
         const long long ue = min(u_end, it.u0 + it.span.n);
         bool ok = true;
         for (int i = (int)(u - it.u0); i < (int)(ue - it.u0) && ok; ++i) {
-          const int key0 = it.span.block(i) * PBLK;
+          const int key0 = it.span.block(i) * PBLK, st = blocks++ & 1;
           if (key0 + PBLK <= it.s.kv) continue;
-          ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_VTAIL), tails & 1, abort_flag, g.status));
-          ++tails;
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_VTAIL + st), (st ? tails[1] : tails[0]) & 1, abort_flag, g.status));
+          if (st) ++tails[1];
+          else ++tails[0];
           if (!ok) break;
           for (int x = max(it.s.kv - key0, 0) * 8 + lane; x < PBLK * 8; x += 32)
 #pragma unroll
             for (int s = 0; s < NSUB; ++s)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sbase + L::V + s * PSUB + x * 16), "r"(0) : "memory");
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sbase + L::V + (st * NSUB + s) * PSUB + x * 16), "r"(0) : "memory");
           fence_proxy_async();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(PB_VFULL));
+          if (lane == 0) mbar_arrive(bar(PB_VFULL + st));
         }
         if (!ok) break;
         u = ue;
@@ -288,7 +274,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
     // ---------------------------------------------------------------- softmax and sums
     const int t = (warp - 4) >> 2, quarter = warp & 3, row_local = quarter * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-    const uint32_t p_row = sbase + L::P + t * 2 * PSUB + row_local * 128;
+    const uint32_t stage = sbase + L::OUT + (warp - 4) * 4096;             // this warp's 32 rows of 64 columns on their way out
     const float sl2 = a.scale * 1.4426950408889634f;
     uint32_t sc = 0, oc = 0;                               // S rows taken, P tiles handed over
     bool ok = true;
@@ -301,21 +287,28 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
       const int pos_min = pos0 + first_row / g.rep, pos_max = pos0 + (first_row + max(rows, 1) - 1) / g.rep;
       const int lower = g.window ? pos - g.window + 1 : 0;
       float m = -INFINITY, l = 0.f;
+      // the pages of each 16 keys, read a block ahead and looked at when it is their turn
+      const int* pages_of = g.table + (long long)it.b * g.N;
+      auto look = [&](int i) {
+        const int key = it.span.block(i) * PBLK + lane * 16;
+        return lane < 8 && key < it.s.kv ? __ldg(pages_of + (key >> g.page_shift)) : -1;
+      };
+      int id = p.i0 < n_t ? look(p.i0) : -1;
       for (int i = p.i0; i < n_t; ++i) {
         const int key0 = it.span.block(i) * PBLK;
-        const int col_key = key0 + lane * 16;              // whether the page of each 16 keys is there
-        const int id = lane < 8 && col_key < it.s.kv ? paged_page(g, it.b, col_key) : -1;
         ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_SFULL + t), sc & 1, abort_flag, g.status));
         ++sc;
         if (!ok) break;
         tc_fence_after();
         uint32_t s[128];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(TM_S[t] + lane_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+        for (int c = 0; c < 4; ++c) tmem_ld32(TM_S + lane_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
         tmem_ld_wait();
         tc_fence_before();
-        const uint32_t there = __ballot_sync(0xffffffffu, id >= 0) & 0xffu;
-        if (lane == 0) mbar_arrive(bar(PB_SREAD + t));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(PB_SREAD));
+        const uint32_t there = __ballot_sync(0xffffffffu, id >= 0 && id < g.P) & 0xffu;
+        if (i + 1 < n_t) id = look(i + 1);
         bool landed = i == p.i0;                           // whether the product before is known to be complete (an item's end waits for it)
         if (there != 0xffu || key0 + PBLK - 1 > pos_min || (g.window && key0 < pos_max - g.window + 1 && key0 + PBLK > g.sinks)) {
           // a word of visible keys per 32 columns, then a select by one bit each: tests of every column in turn took 7 us a block where these take 0.3
@@ -373,22 +366,14 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
           if (c == 0 && !landed) {                         // P is still the operand of the product before
             ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_OFULL + t), (oc - 1) & 1, abort_flag, g.status));
           }
-          if (ok) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int q8 = c * 4 + x;
-              const uint32_t addr = p_row + (q8 >> 3) * PSUB + (((q8 & 7) ^ (row_local & 7)) << 4);
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[x * 4]), "r"(w[x * 4 + 1]), "r"(w[x * 4 + 2]),
-                           "r"(w[x * 4 + 3]) : "memory");
-            }
-          }
+          if (ok) tmem_st16(TM_P[t] + lane_addr + c * 16, w);
         }
         if (!ok) break;
         float a0, a1, a2, a3;
         unpack_f32x2(ls[0], a0, a1);
         unpack_f32x2(ls[1], a2, a3);
         l += (a0 + a1) + (a2 + a3);
-        fence_proxy_async();
+        tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(PB_PREADY + t));
@@ -422,7 +407,8 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
             for (int x = 0; x < 32; ++x) o[x] = 0u;
           }
           if (whole) {
-            // through this warp's rows of P: a row's 16-byte pieces next to each other make whole lines (a thread's row at a time: 32 lines per instruction, 3 us)
+            // through shared memory, 64 columns at a time: the 16-byte pieces of a row next to each other make whole lines (a thread's row at a time: 32 lines per
+            // instruction, 3 us an item)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               uint32_t w[4];
@@ -432,9 +418,20 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
                 finite = finite & isfinite(v0) & isfinite(v1);
                 w[y] = pack_bf16(v0, v1);
               }
-              const int q8 = c * 4 + x;
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p_row + (q8 >> 3) * PSUB + (((q8 & 7) ^ (row_local & 7)) << 4)), "r"(w[0]), "r"(w[1]),
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((((c & 1) * 4 + x) ^ (lane & 7)) << 4)), "r"(w[0]), "r"(w[1]),
                            "r"(w[2]), "r"(w[3]) : "memory");
+            }
+            if (c & 1) {
+              __syncwarp();
+#pragma unroll
+              for (int y = 0; y < 8; ++y) {
+                const int x = y * 4 + (lane >> 3), piece = lane & 7, col = (c >> 1) * 64 + piece * 8;
+                const long long to = __shfl_sync(0xffffffffu, orow, x);
+                uint4 v;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                             : "r"(stage + x * 128 + ((piece ^ (x & 7)) << 4)) : "memory");
+                if (quarter * 32 + x < rows && col < g.hd) *reinterpret_cast<uint4*>(a.out + to + col) = v;
+              }
             }
           } else if (valid) {
 #pragma unroll
@@ -442,18 +439,6 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
               prow[(c * 8 + x) * 128] = make_float4(__uint_as_float(o[x * 4]), __uint_as_float(o[x * 4 + 1]), __uint_as_float(o[x * 4 + 2]), __uint_as_float(o[x * 4 + 3]));
           }
           __syncwarp();
-        }
-        if (whole) {
-          constexpr int PIECES = HDP / 8, AT_ONCE = 32 / PIECES;       // 16-byte pieces of a row, rows of an instruction
-#pragma unroll 4
-          for (int y = 0; y < 32 / AT_ONCE; ++y) {
-            const int x = y * AT_ONCE + lane / PIECES, q8 = lane % PIECES, local = quarter * 32 + x;
-            const long long to = __shfl_sync(0xffffffffu, orow, x);
-            uint4 v;
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                         : "r"(sbase + L::P + t * 2 * PSUB + local * 128 + (q8 >> 3) * PSUB + (((q8 & 7) ^ (local & 7)) << 4)) : "memory");
-            if (local < rows && q8 * 8 < g.hd) *reinterpret_cast<uint4*>(a.out + to + q8 * 8) = v;
-          }
         }
         if (!whole && valid) reinterpret_cast<float2*>(a.stat)[ps * 128 + row_local] = make_float2(m, l);
         __syncwarp();
