@@ -15,12 +15,25 @@ namespace elfa {
 
 constexpr int PAGED_MAX_SEQS = 1024;       // per launch; the Python side cuts larger batches
 
+// x / d for 0 <= x < 2^31 and a d that the host knows: with 2^s the power of two from d on and m = floor(2^32 (2^s - d) / d) + 1, (mulhi(x, m) + x) >> s
+// (the round-up method for invariant divisors). A division costs some 40 instructions, and the walk over items is made of them.
+struct DivBy {
+  unsigned d, m, s;
+  __device__ __forceinline__ int operator()(int x) const { return (int)((__umulhi((unsigned)x, m) + (unsigned)x) >> s); }
+};
+inline DivBy div_by(unsigned d) {
+  unsigned s = 0;
+  while ((1u << s) < d) ++s;
+  return {d, (unsigned)((((unsigned long long)1 << 32) * ((1ull << s) - d)) / d + 1), s};
+}
+
 struct PagedGeom {
   const int *table, *q_start, *kv_len;
   int B, N, P, page_shift, T, max_new;     // T: rows of q; max_new: the most new tokens that the host has planned for
   int H, Hkv, rep, hd;
   int window, sinks;                       // window 0: none
   int tile_rows;                           // query rows of a tile
+  DivBy by_rep, by_tile;                   // / rep, / tile_rows
   unsigned int* status;
 };
 
@@ -39,7 +52,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedGeom& g, int b) {
   return s;
 }
 __device__ __forceinline__ int paged_tiles(const PagedGeom& g, const PagedSeq& s) {
-  return (s.n * g.rep + g.tile_rows - 1) / g.tile_rows;
+  return g.by_tile(s.n * g.rep + g.tile_rows - 1);
 }
 
 // key blocks that the rows of a tile see: i < ns is block i (sinks), later ones are w0 + i - ns. A tile that sees nothing still has one block.
@@ -49,7 +62,7 @@ struct PagedSpan {
 };
 template <int BLK>
 __device__ __forceinline__ PagedSpan paged_span(const PagedGeom& g, const PagedSeq& s, int t) {
-  const int r0 = t * g.tile_rows, lo_tok = r0 / g.rep, hi_tok = (min(r0 + g.tile_rows, s.n * g.rep) - 1) / g.rep;
+  const int r0 = t * g.tile_rows, lo_tok = g.by_rep(r0), hi_tok = g.by_rep(min(r0 + g.tile_rows, s.n * g.rep) - 1);
   const int pos0 = s.kv - s.n, hi = max(pos0 + hi_tok + 1, 0);
   const int lo = g.window ? max(0, pos0 + lo_tok - g.window + 1) : 0;
   PagedSpan p;

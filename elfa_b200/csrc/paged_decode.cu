@@ -127,8 +127,8 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
     const long long ue = min(u_end, it.u0 + it.span.n);
     const int r0 = it.t * DROWS, rows = min(DROWS, it.s.n * g.rep - r0), pos0 = it.s.kv - it.s.n;
     // rows behind the last one repeat it
-    const int ra = r0 + min(gr, rows - 1), rb = r0 + min(gr + 8, rows - 1), ta = ra / g.rep, tb = rb / g.rep;
-    const int pa = pos0 + ta, pb = pos0 + tb, pos_min = pos0 + r0 / g.rep, pos_max = pos0 + (r0 + rows - 1) / g.rep;
+    const int ra = r0 + min(gr, rows - 1), rb = r0 + min(gr + 8, rows - 1), ta = g.by_rep(ra), tb = g.by_rep(rb);
+    const int pa = pos0 + ta, pb = pos0 + tb, pos_min = pos0 + g.by_rep(r0), pos_max = pos0 + g.by_rep(r0 + rows - 1);
     uint32_t qf[HDP / 16][4];
     {
       const __nv_bfloat16* qa = a.q + (it.s.q0 + ta) * a.qs + (it.h * g.rep + ra - ta * g.rep) * g.hd;
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
         while (bad) {                                                  // all lanes hold the same word
           const int r = __ffs(bad) - 1;
           bad &= bad - 1;
-          const int tok = (r0 + r) / g.rep, head = it.h * g.rep + (r0 + r) % g.rep;
+          const int tok = g.by_rep(r0 + r), head = it.h * g.rep + r0 + r - tok * g.rep;
           const long long at = it.s.q0 + tok;
           float res[HDP / 32];
           paged_row<HDP>(g, a.q + at * a.qs + head * g.hd, a.pages, it.b, it.h, pos0 + tok, a.scale, res);
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(const __grid_con
       const float inv = den == 0.f ? 0.f : 1.f / den;
       num.x *= inv; num.y *= inv; num.z *= inv; num.w *= inv;
       if (v * 4 < g.hd) {
-        const int tok = (j.r0 + r) / g.rep, head = j.h * g.rep + (j.r0 + r) - tok * g.rep;
+        const int tok = g.by_rep(j.r0 + r), head = j.h * g.rep + (j.r0 + r) - tok * g.rep;
         *reinterpret_cast<uint2*>(a.out + ((long long)(j.q0 + tok) * g.H + head) * g.hd + v * 4) = make_uint2(pack_bf16(num.x, num.y), pack_bf16(num.z, num.w));
         if (!(isfinite(num.x) && isfinite(num.y) && isfinite(num.z) && isfinite(num.w))) atomicOr(&bad, 1u << r);
       }
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(const __grid_con
   }
   for (int r = warp; r < j.rows; r += 8) {
     if (!(bad >> r & 1u)) continue;
-    const int tok = (j.r0 + r) / g.rep, head = j.h * g.rep + (j.r0 + r) % g.rep;
+    const int tok = g.by_rep(j.r0 + r), head = j.h * g.rep + (j.r0 + r) - tok * g.rep;
     const long long at = j.q0 + tok;
     float res[HDP / 32];
     paged_row<HDP>(g, a.q + at * a.qs + head * g.hd, a.pages, j.b, j.h, j.pos0 + tok, a.scale, res);
@@ -455,6 +455,7 @@ int paged_geom(PagedGeom* g, const void* pages, const int* table, const int* q_s
   g->B = B; g->N = N; g->P = P; g->T = T; g->max_new = max_new;
   g->page_shift = __builtin_ctz((unsigned)page);
   g->H = H; g->Hkv = Hkv; g->rep = H / Hkv; g->hd = hd;
+  g->by_rep = div_by((unsigned)g->rep);
   g->window = window > (1 << 30) ? 0 : window;
   g->sinks = sinks > (1 << 30) ? 1 << 30 : sinks;
   return ELFA_OK;
@@ -500,6 +501,7 @@ ELFA_API int elfa_paged_attention(const void* q, long long qs, const void* pages
   a.qs = qs;
   a.scale = scale;
   a.g.tile_rows = DROWS;
+  a.g.by_tile = div_by(DROWS);
   a.whole = decode_whole(max_new, a.g.rep, (long long)N * page);
   a.wide = ((long long)max_new * a.g.rep + DROWS - 1) / DROWS > 4;
   a.min_units = MIN_UNITS;

@@ -57,7 +57,7 @@ __device__ __forceinline__ Part part_of(const PagedGeom& g, const PagedItem& it,
     p.n0 = p.i1;
     p.n1 = p.i0;
   } else {
-    const int hi = max(it.s.kv - it.s.n + (r0 + half - 1) / g.rep + 1, 0), b = (hi + PBLK - 1) / PBLK;      // blocks up to tile 0's last row
+    const int hi = max(it.s.kv - it.s.n + g.by_rep(r0 + half - 1) + 1, 0), b = (hi + PBLK - 1) / PBLK;      // blocks up to tile 0's last row
     const int n = b >= it.span.w0 ? it.span.ns + b - it.span.w0 : min(it.span.ns, b);
     p.n0 = min(max(n, p.i0), p.i1);
     p.n1 = p.i1;
@@ -283,8 +283,8 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
       const int n_t = t ? p.n1 : p.n0;
       const int first_row = it.t * g.tile_rows + t * half_rows, rows = min(half_rows, it.s.n * g.rep - first_row);   // rows <= 0: no such tile
       const int pos0 = it.s.kv - it.s.n;
-      const int r = first_row + min(row_local, max(rows, 1) - 1), tok = min(r / g.rep, it.s.n - 1), pos = pos0 + tok;
-      const int pos_min = pos0 + first_row / g.rep, pos_max = pos0 + (first_row + max(rows, 1) - 1) / g.rep;
+      const int r = first_row + min(row_local, max(rows, 1) - 1), tok = min(g.by_rep(r), it.s.n - 1), pos = pos0 + tok;
+      const int pos_min = pos0 + g.by_rep(first_row), pos_max = pos0 + g.by_rep(first_row + max(rows, 1) - 1);
       const int lower = g.window ? pos - g.window + 1 : 0;
       float m = -INFINITY, l = 0.f;
       // the pages of each 16 keys, read a block ahead and looked at when it is their turn
@@ -395,7 +395,8 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
         const long long orow = (at * g.H + head) * g.hd;
         const long long ps = (2LL * blockIdx.x + (p.i0 == 0)) * 2 + t;
         float4* prow = reinterpret_cast<float4*>(a.part) + ps * (HDP / 4) * 128 + row_local;
-        bool finite = true;
+        const uint64_t inv2 = pack_f32x2(inv, inv), zero2 = 0ull;
+        uint64_t odd = 0ull;
 #pragma unroll 1
         for (int c = 0; c < HDP / 32; ++c) {
           uint32_t o[32];
@@ -414,8 +415,10 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
               uint32_t w[4];
 #pragma unroll
               for (int y = 0; y < 4; ++y) {
-                const float v0 = __uint_as_float(o[x * 8 + 2 * y]) * inv, v1 = __uint_as_float(o[x * 8 + 2 * y + 1]) * inv;
-                finite = finite & isfinite(v0) & isfinite(v1);
+                const uint64_t v = mul_f32x2(pack_f32x2(__uint_as_float(o[x * 8 + 2 * y]), __uint_as_float(o[x * 8 + 2 * y + 1])), inv2);
+                odd = fma_f32x2(v, zero2, odd);            // infinity and NaN times zero
+                float v0, v1;
+                unpack_f32x2(v, v0, v1);
                 w[y] = pack_bf16(v0, v1);
               }
               asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((((c & 1) * 4 + x) ^ (lane & 7)) << 4)), "r"(w[0]), "r"(w[1]),
@@ -442,9 +445,11 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
         }
         if (!whole && valid) reinterpret_cast<float2*>(a.stat)[ps * 128 + row_local] = make_float2(m, l);
         __syncwarp();
-        unsigned bad = __ballot_sync(0xffffffffu, whole && valid && !finite);
+        float odd0, odd1;
+        unpack_f32x2(odd, odd0, odd1);
+        unsigned bad = __ballot_sync(0xffffffffu, whole && valid && (odd0 != 0.f || odd1 != 0.f));
         while (bad) {
-          const int x = __ffs(bad) - 1, rx = first_row + quarter * 32 + x, tx = rx / g.rep;
+          const int x = __ffs(bad) - 1, rx = first_row + quarter * 32 + x, tx = g.by_rep(rx);
           bad &= bad - 1;
           const int hx = it.h * g.rep + rx - tx * g.rep;
           const long long ax = it.s.q0 + tx;
@@ -543,7 +548,7 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const __grid_co
   for (int x = warp; x < 32; x += 8) {
     const int r = j.r0 + t * half_rows + first + x;
     if (first + x >= half_rows || t * half_rows + first + x >= j.rows) continue;
-    const int tok = r / g.rep, head = j.h * g.rep + r - tok * g.rep;
+    const int tok = g.by_rep(r), head = j.h * g.rep + r - tok * g.rep;
     const long long at = j.q0 + tok;
     __nv_bfloat16* po = a.out + (at * g.H + head) * g.hd;
     if (bad >> x & 1u) {
@@ -596,6 +601,7 @@ int paged_prefill(PagedGeom g, const void* q, long long qs, const void* pages, v
   a.scale = scale;
   a.tile_toks = 128 / g.rep;
   a.g.tile_rows = 2 * a.tile_toks * g.rep;
+  a.g.by_tile = div_by((unsigned)a.g.tile_rows);
   a.part = scratch;
   a.stat = scratch + 2LL * 148 * 2 * 128 * (g.hd <= 64 ? 64 : 128);
   a.notes = reinterpret_cast<PagedJoin*>(a.stat + 2LL * 148 * 2 * 128 * 2);
