@@ -5,8 +5,8 @@
 // `pos` sees the keys that lie in pages that are there and for which key <= pos and (key > pos - window or key < sinks).
 //
 // Work is counted in units: one tile of query rows (rows are (token, head of the group) pairs, token first, so a key is read once for all heads
-// that share it) against one block of keys. The units of all (sequence, tile, key head) items stand in one line, blocks innermost, and CTA c
-// of G takes c W / G up to (c + 1) W / G of them: every CTA gets the same number whatever the sequences' lengths are, and the host needs to know none of
+// that share it) against one block of keys. The units of all (sequence, tile, key head) items stand in one line, blocks innermost, and each of G
+// CTAs takes W / G of them (the first ones one more each): the same number whatever the sequences' lengths are, and the host needs to know none of
 // them. An item that a CTA does not hold whole leaves a partial result: slot 2 c + 1 for the part that begins it, slot 2 c for a later part.
 #pragma once
 #include "common.cuh"
@@ -72,52 +72,75 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedGeom& g, const PagedS
   return p;
 }
 
-// units of a sequence (all tiles, all key heads); `lane` of `lanes` threads adds up every lanes-th tile
+// units of a sequence (all tiles, all key heads); `lane` of `lanes` threads adds up every lanes-th tile. The host has seen to it that all units of a call fit 32 bits.
 template <int BLK>
-__device__ __forceinline__ long long paged_units(const PagedGeom& g, const PagedSeq& s, int lane, int lanes) {
+__device__ __forceinline__ unsigned paged_units(const PagedGeom& g, const PagedSeq& s, int lane, int lanes) {
   const int tiles = paged_tiles(g, s);
-  long long u = 0;
+  unsigned u = 0;
   for (int t = lane; t < tiles; t += lanes) u += paged_span<BLK>(g, s, t).n;
   return u * g.Hkv;
 }
 
-// prefix[b] = units before sequence b, prefix[B] = W, by all threads of the block (ends with a barrier). wide: a warp per sequence (many tiles each).
+// What every CTA works out for itself, in shared memory: prefix[b] = units before sequence b, prefix[B] = W, and the sequences.
+struct PagedLine {
+  unsigned* prefix;                        // [B + 1]
+  PagedSeq* seqs;                          // [B]
+  unsigned* warp_tot;                      // [warps]
+};
+constexpr int paged_line_bytes(int B) { return 4 * (B + 1) + (int)sizeof(PagedSeq) * B; }
+__device__ __forceinline__ PagedLine paged_line(void* at, int B, unsigned* warp_tot) {
+  unsigned* p = static_cast<unsigned*>(at);
+  return {p, reinterpret_cast<PagedSeq*>(p + B + 1), warp_tot};
+}
+// By all threads of the block (ends with a barrier). wide: a warp per sequence (many tiles each).
 template <int BLK, int THREADS>
-__device__ __forceinline__ void paged_prefix(const PagedGeom& g, long long* prefix, long long* warp_tot, bool wide) {
+__device__ __forceinline__ void paged_prefix(const PagedGeom& g, const PagedLine& line, bool wide) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int WARPS = THREADS / 32;
   if (wide) {
     for (int b = warp; b < g.B; b += WARPS) {
       const PagedSeq s = paged_seq(g, b);
-      long long u = paged_units<BLK>(g, s, lane, 32);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-      if (lane == 0) prefix[b + 1] = u;
+      const unsigned u = __reduce_add_sync(0xffffffffu, paged_units<BLK>(g, s, lane, 32));
+      if (lane == 0) {
+        line.prefix[b + 1] = u;
+        line.seqs[b] = s;
+      }
     }
     __syncthreads();
   }
-  long long run = 0;
+  unsigned run = 0;
   for (int b0 = 0; b0 < g.B; b0 += THREADS) {
     const int b = b0 + threadIdx.x;
-    long long u = 0;
-    if (b < g.B) u = wide ? prefix[b + 1] : paged_units<BLK>(g, paged_seq(g, b), 0, 1);
+    unsigned u = 0;
+    if (b < g.B) {
+      if (wide) {
+        u = line.prefix[b + 1];
+      } else {
+        const PagedSeq s = paged_seq(g, b);
+        line.seqs[b] = s;
+        u = paged_units<BLK>(g, s, 0, 1);
+      }
+    }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, u, o);
+      const unsigned v = __shfl_up_sync(0xffffffffu, u, o);
       if (lane >= o) u += v;
     }
-    if (lane == 31) warp_tot[warp] = u;
-    __syncthreads();
-    long long before = run;
+    if (g.B > 32) {                        // else the first warp has all of them
+      if (lane == 31) line.warp_tot[warp] = u;
+      __syncthreads();
+      unsigned before = run;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) before += warp_tot[w];
-      run += warp_tot[w];
+      for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) before += line.warp_tot[w];
+        run += line.warp_tot[w];
+      }
+      u += before;
+      if (b0 + THREADS < g.B) __syncthreads();
     }
-    if (b < g.B) prefix[b + 1] = before + u;
-    __syncthreads();
+    if (b < g.B) line.prefix[b + 1] = u;
   }
-  if (threadIdx.x == 0) prefix[0] = 0;
+  if (threadIdx.x == 0) line.prefix[0] = 0;
   __syncthreads();
 }
 
@@ -125,34 +148,34 @@ struct PagedItem {
   int b, t, h;
   PagedSeq s;
   PagedSpan span;
-  long long u0;                            // unit of its block 0
+  unsigned u0;                             // unit of its block 0
   int tiles;
 };
 
 // the item that unit u belongs to; all lanes of a warp call it together
 template <int BLK>
-__device__ __forceinline__ PagedItem paged_find(const PagedGeom& g, const long long* prefix, long long u) {
+__device__ __forceinline__ PagedItem paged_find(const PagedGeom& g, const PagedLine& line, unsigned u) {
   int lo = 0, hi = g.B;                    // prefix[lo] <= u < prefix[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (prefix[mid] <= u) lo = mid;
+    if (line.prefix[mid] <= u) lo = mid;
     else hi = mid;
   }
   PagedItem it;
   it.b = lo;
-  it.s = paged_seq(g, lo);
+  it.s = line.seqs[lo];
   it.tiles = paged_tiles(g, it.s);
   const int lane = threadIdx.x & 31;
-  long long base = prefix[lo];
+  unsigned base = line.prefix[lo];
   it.t = 0;
   if (it.tiles > 1) {
     for (int t0 = 0;; t0 += 32) {
       const int t = t0 + lane;
-      const long long mine = t < it.tiles ? (long long)paged_span<BLK>(g, it.s, t).n * g.Hkv : 0;
-      long long incl = mine;
+      const unsigned mine = t < it.tiles ? (unsigned)paged_span<BLK>(g, it.s, t).n * g.Hkv : 0;
+      unsigned incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+        const unsigned v = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += v;
       }
       const unsigned hit = __ballot_sync(0xffffffffu, base + incl > u && t < it.tiles);
@@ -166,8 +189,8 @@ __device__ __forceinline__ PagedItem paged_find(const PagedGeom& g, const long l
     }
   }
   it.span = paged_span<BLK>(g, it.s, it.t);
-  it.h = (int)((u - base) / it.span.n);
-  it.u0 = base + (long long)it.h * it.span.n;
+  it.h = (int)((u - base) / (unsigned)it.span.n);
+  it.u0 = base + (unsigned)it.h * it.span.n;
   return it;
 }
 // the next item in line (there is one as long as its first unit is below W)
@@ -190,20 +213,27 @@ __device__ __forceinline__ void paged_next(const PagedGeom& g, PagedItem& it) {
   it.span = paged_span<BLK>(g, it.s, it.t);
 }
 
-__device__ __forceinline__ long long paged_cut(long long W, int G, int c) { return c * W / G; }
-// the CTA that holds unit u
-__device__ __forceinline__ int paged_owner(long long W, int G, long long u) { return (int)(((u + 1) * G - 1) / W); }
+// The shares of G CTAs (G <= W).
+struct PagedShares {
+  unsigned each, more;                     // units of a CTA; how many of them have one more
+  __device__ __forceinline__ PagedShares(unsigned W, unsigned G) : each(G ? W / G : 0), more(G ? W - each * G : 0) {}
+  __device__ __forceinline__ unsigned first(unsigned c) const { return c * each + min(c, more); }
+  __device__ __forceinline__ int owner(unsigned u) const {
+    const unsigned front = more * (each + 1);
+    return (int)(u < front ? u / (each + 1) : more + (u - front) / each);
+  }
+};
 
 // What joins an item that several CTAs have parts of, written by the CTA that the item's first cut lies in front of: its parts are slot 2 first + 1 and
 // slots 2 c for first < c <= last. rows 0: nothing to join here.
 struct alignas(16) PagedJoin {
   int rows, last, b, h, r0, q0, pos0, unused;
 };
-__device__ __forceinline__ void paged_join_note(const PagedGeom& g, PagedJoin* notes, const PagedItem& it, long long W, int G, int c, bool has_units, bool cut) {
+__device__ __forceinline__ void paged_join_note(const PagedGeom& g, PagedJoin* notes, const PagedItem& it, const PagedShares& shares, int c, bool cut) {
   PagedJoin j{};
-  if (has_units && cut && paged_owner(W, G, it.u0) == c - 1) {
+  if (cut && shares.owner(it.u0) == c - 1) {
     j.rows = min(g.tile_rows, it.s.n * g.rep - it.t * g.tile_rows);
-    j.last = paged_owner(W, G, it.u0 + it.span.n - 1);
+    j.last = shares.owner(it.u0 + it.span.n - 1);
     j.b = it.b;
     j.h = it.h;
     j.r0 = it.t * g.tile_rows;

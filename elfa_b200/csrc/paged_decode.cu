@@ -38,14 +38,11 @@ struct DecodeSmem {
   static constexpr int STAT = MERGE + 2 * DROWS * HDP * 4;           // [4][16][2]
   static constexpr int BAR = STAT + DWARPS * DROWS * 8;
   static constexpr int TOT = BAR + DWARPS * DST * 8;                 // warp totals, abort flag
-  static constexpr int PREFIX = TOT + DWARPS * 8 + 16;
-  static constexpr int bytes(int B) { return PREFIX + 8 * (B + 1) + 1024; }
+  static constexpr int LINE = TOT + DWARPS * 4 + 16;
+  static constexpr int bytes(int B) { return LINE + paged_line_bytes(B) + 1024; }
 };
 
-__device__ __forceinline__ int decode_ctas(long long W, int grid, int min_units) {
-  const long long most = (W + min_units - 1) / min_units;
-  return (int)(most < grid ? most : grid);
-}
+__device__ __forceinline__ int decode_ctas(unsigned W, int grid, int min_units) { return (int)min((W + min_units - 1) / min_units, (unsigned)grid); }
 
 template <int HDP>
 __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ DecodeArgs a) {
@@ -55,9 +52,7 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* merge = reinterpret_cast<float*>(smem + L::MERGE);
   float2* stat = reinterpret_cast<float2*>(smem + L::STAT);
-  long long* prefix = reinterpret_cast<long long*>(smem + L::PREFIX);
-  long long* warp_tot = reinterpret_cast<long long*>(smem + L::TOT);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::TOT + DWARPS * 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::TOT + DWARPS * 4);
   const PagedGeom& g = a.g;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, qd = lane & 3;
   const uint32_t ring = smem_u32(smem) + warp * DST * L::UNIT, bars = smem_u32(smem + L::BAR) + warp * DST * 8;
@@ -68,7 +63,7 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
   }
   if (lane < DST) mbar_init(bars + 8 * lane, 1);
   fence_barrier_init();
-  long long u_begin, u_end;
+  unsigned u_begin, u_end;
   PagedItem first{};
   if (a.whole) {
     first.b = blockIdx.x / g.Hkv;
@@ -81,50 +76,75 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
     u_end = first.tiles ? first.span.n : 0;
     __syncthreads();
   } else {
-    paged_prefix<DBLK, DWARPS * 32>(g, prefix, warp_tot, a.wide);
-    const long long W = prefix[g.B];
+    const PagedLine line = paged_line(smem + L::LINE, g.B, reinterpret_cast<unsigned*>(smem + L::TOT));
+    paged_prefix<DBLK, DWARPS * 32>(g, line, a.wide);
+    const unsigned W = line.prefix[g.B];
     const int G = decode_ctas(W, gridDim.x, a.min_units);
-    u_begin = (int)blockIdx.x < G ? paged_cut(W, G, blockIdx.x) : 0;
-    u_end = (int)blockIdx.x < G ? paged_cut(W, G, blockIdx.x + 1) : 0;
-    if (u_begin < u_end) first = paged_find<DBLK>(g, prefix, u_begin);
-    if (threadIdx.x == 0) paged_join_note(g, a.notes, first, W, G, blockIdx.x, u_begin < u_end, u_begin > first.u0);
+    const PagedShares shares(W, G);
+    u_begin = (int)blockIdx.x < G ? shares.first(blockIdx.x) : 0;
+    u_end = (int)blockIdx.x < G ? shares.first(blockIdx.x + 1) : 0;
+    if (u_begin < u_end) first = paged_find<DBLK>(g, line, u_begin);
+    if (threadIdx.x == 0) paged_join_note(g, a.notes, first, shares, blockIdx.x, u_begin < u_end && u_begin > first.u0);
   }
   pdl_next();
   if (u_begin >= u_end) return;
 
-  // ---- the warp's own loads: unit u_begin + warp, then every fourth
+  // ---- the warp's own loads: unit u_begin + warp, then every fourth; the page of the next one is looked up a turn ahead
   PagedItem pi = first;
-  long long pu = u_begin + warp;
+  unsigned pu = u_begin + warp;
   const int rows_per_box = min(1 << g.page_shift, DBLK), boxes = DBLK / rows_per_box;
+  const int box = lane / (2 * NSUB), sub = (lane >> 1) % NSUB, kv = lane & 1;
   uint32_t there = 0;                                    // two bits per ring slot: which half's page is there
-  auto issue = [&](int slot) {
+  struct Ahead {
+    int id, row, h;
+  };
+  auto look = [&]() {
+    Ahead n{-1, 0, 0};
+    if (pu < u_end) {
+      while (pu >= pi.u0 + pi.span.n) paged_next<DBLK>(g, pi);
+      const int key = pi.span.block((int)(pu - pi.u0)) * DBLK + box * rows_per_box;
+      n.row = key & ((1 << g.page_shift) - 1);
+      n.h = pi.h;
+      if (box < boxes && key < pi.s.kv) n.id = __ldg(g.table + (long long)pi.b * g.N + (key >> g.page_shift));
+    }
+    return n;
+  };
+  auto issue = [&](int slot, const Ahead& n) {
     if (pu >= u_end) return;
-    while (pu >= pi.u0 + pi.span.n) paged_next<DBLK>(g, pi);
-    const int key0 = pi.span.block((int)(pu - pi.u0)) * DBLK;
     const uint32_t bar = bars + 8 * slot, dst = ring + slot * L::UNIT;
     if (lane == 0) mbar_expect_tx(bar, L::UNIT);
-    const int box = lane / (2 * NSUB), sub = (lane >> 1) % NSUB, kv = lane & 1;
-    const int key = key0 + box * rows_per_box;
-    const int id = box < boxes && key < pi.s.kv ? paged_page(g, pi.b, key) : -1;
+    const bool ok = n.id >= 0 && n.id < g.P;
+    if (n.id >= g.P) atomicOr(g.status, (unsigned)ELFA_ST_BAD_PAGE);
     __syncwarp();
     if (box < boxes)                                     // an absent page is read past the pool's end, which gives zeros
-      tma_load_3d(dst + kv * L::HALF + (sub * DBLK + box * rows_per_box) * 128, &tm, sub * 64, key & ((1 << g.page_shift) - 1),
-                  id < 0 ? 2 * g.P * g.Hkv : (2 * id + kv) * g.Hkv + pi.h, bar);
-    const unsigned ok = __ballot_sync(0xffffffffu, id >= 0);
-    const uint32_t two = (ok & 1u) | ((boxes > 1 ? ok >> (2 * NSUB) & 1u : ok & 1u) << 1);
+      tma_load_3d(dst + kv * L::HALF + (sub * DBLK + box * rows_per_box) * 128, &tm, sub * 64, n.row,
+                  ok ? (2 * n.id + kv) * g.Hkv + n.h : 2 * g.P * g.Hkv, bar);
+    const unsigned who = __ballot_sync(0xffffffffu, ok);
+    const uint32_t two = (who & 1u) | ((boxes > 1 ? who >> (2 * NSUB) & 1u : who & 1u) << 1);
     there = (there & ~(3u << (2 * slot))) | two << (2 * slot);
     pu += DWARPS;
   };
+  Ahead ahead;
+  {
+    Ahead n[DST];                                        // the first ones asked for together
 #pragma unroll
-  for (int s = 0; s < DST; ++s) issue(s);
+    for (int s = 0; s < DST; ++s) {
+      n[s] = look();
+      pu += DWARPS;
+    }
+    ahead = look();
+    pu -= DST * DWARPS;
+#pragma unroll
+    for (int s = 0; s < DST; ++s) issue(s, n[s]);
+  }
 
   const float sl2 = a.scale * 1.4426950408889634f;
   PagedItem it = first;
   int slot = 0;
   uint32_t phase = 0;
   bool ok = true;
-  for (long long u = u_begin; u < u_end;) {
-    const long long ue = min(u_end, it.u0 + it.span.n);
+  for (unsigned u = u_begin; u < u_end;) {
+    const unsigned ue = min(u_end, it.u0 + it.span.n);
     const int r0 = it.t * DROWS, rows = min(DROWS, it.s.n * g.rep - r0), pos0 = it.s.kv - it.s.n;
     // rows behind the last one repeat it
     const int ra = r0 + min(gr, rows - 1), rb = r0 + min(gr + 8, rows - 1), ta = g.by_rep(ra), tb = g.by_rep(rb);
@@ -147,8 +167,8 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
     for (int d = 0; d < HDP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-    const int lead = (int)((warp - (u - u_begin)) & (DWARPS - 1));     // this warp's first unit of the item
-    for (long long x = u + lead; x < ue; x += DWARPS) {
+    const unsigned lead = (warp - (u - u_begin)) & (DWARPS - 1);       // this warp's first unit of the item
+    for (unsigned x = u + lead; x < ue; x += DWARPS) {
       const int key0 = it.span.block((int)(x - it.u0)) * DBLK;
       ok = ok && __all_sync(0xffffffffu, mbar_wait(bars + 8 * slot, phase, abort_flag, g.status));
       if (!ok) break;
@@ -227,7 +247,8 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
         }
       }
       __syncwarp();                                                    // every lane has read the slot
-      issue(slot);
+      issue(slot, ahead);
+      ahead = look();
       if (++slot == DST) {
         slot = 0;
         phase ^= 1;
@@ -465,6 +486,12 @@ int paged_geom(PagedGeom* g, const void* pages, const int* table, const int* q_s
 long long paged_prefill_scratch(int hd);
 int paged_prefill(PagedGeom g, const void* q, long long qs, const void* pages, void* out, float* scratch, int page, float scale, cudaStream_t st);
 
+// Units are counted in 32 bits.
+bool paged_units_fit(const PagedGeom& g, int block) {
+  const double tiles = (double)g.T * g.rep / g.tile_rows + g.B, blocks = ((double)g.N * (1 << g.page_shift)) / block + 2;
+  return tiles * blocks * g.Hkv < 4.0e9;
+}
+
 // Which calls go to the tiles of 2 x 128 rows.
 static bool many_rows(int max_new, int rep) { return (long long)max_new * rep > PREFILL_ROWS && rep <= 128; }
 
@@ -505,6 +532,7 @@ ELFA_API int elfa_paged_attention(const void* q, long long qs, const void* pages
   a.whole = decode_whole(max_new, a.g.rep, (long long)N * page);
   a.wide = ((long long)max_new * a.g.rep + DROWS - 1) / DROWS > 4;
   a.min_units = MIN_UNITS;
+  ELFA_REQUIRE(paged_units_fit(a.g, DBLK), "paged_attention: too much work for one call (2^32 tiles of 16 rows by 32 keys)");
   ELFA_REQUIRE(a.whole || (scratch && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0), "paged_attention: no scratch, or not 16-byte aligned");
   a.part = scratch;
   a.stat = scratch + 2LL * decode_grid(hd) * DROWS * (hd <= 64 ? 64 : 128);

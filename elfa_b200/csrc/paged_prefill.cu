@@ -16,6 +16,7 @@
 namespace elfa {
 
 int make_paged_tmap(CUtensorMap* tm, const void* pages, long long P, int Hkv, int page, int hd, int box_rows);
+bool paged_units_fit(const PagedGeom& g, int block);
 
 namespace {
 
@@ -39,16 +40,16 @@ template <int HDP>
 struct PrefillSmem {
   static constexpr int NSUB = HDP / 64;
   static constexpr int Q = 0, K = Q + 2 * NSUB * PSUB, V = K + 2 * NSUB * PSUB, OUT = V + 2 * NSUB * PSUB, BAR = OUT + 8 * 4096;
-  static constexpr int TOTAL = BAR + PB_COUNT * 8 + 16 + 8 * (PTHREADS / 32);
+  static constexpr int TOTAL = BAR + PB_COUNT * 8 + 16 + 4 * (PTHREADS / 32);
   static constexpr int DYN = TOTAL + 1024;
-  static_assert(8 * (PAGED_MAX_SEQS + 1) <= 8 * 4096, "the prefix lies where outputs will");
+  static_assert(paged_line_bytes(PAGED_MAX_SEQS) <= 8 * 4096, "the line of units lies where outputs will");
 };
 
 // what a CTA does of an item: blocks i0 .. i1 of its list; tile 0 takes part up to n0, tile 1 up to n1
 struct Part {
   int i0, i1, n0, n1;
 };
-__device__ __forceinline__ Part part_of(const PagedGeom& g, const PagedItem& it, long long u, long long u_end) {
+__device__ __forceinline__ Part part_of(const PagedGeom& g, const PagedItem& it, unsigned u, unsigned u_end) {
   Part p;
   p.i0 = (int)(u - it.u0);
   p.i1 = (int)(min(u_end, it.u0 + it.span.n) - it.u0);
@@ -78,7 +79,6 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + PB_COUNT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  long long* warp_tot = reinterpret_cast<long long*>(tmem_holder + 4);
   const uint32_t sbase = smem_u32(smem), bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * i; };
   const PagedGeom& g = a.g;
@@ -103,14 +103,15 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
     for (int s = 0; s < 2 * NSUB; ++s)
       asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sbase + L::Q + s * PSUB + i * 16), "r"(0) : "memory");
   fence_proxy_async();
-  long long* prefix = reinterpret_cast<long long*>(smem + L::OUT);
-  paged_prefix<PBLK, PTHREADS>(g, prefix, warp_tot, true);
-  const long long W = prefix[g.B];
-  const int G = (int)min(W, (long long)gridDim.x);
-  const long long u_begin = (int)blockIdx.x < G ? paged_cut(W, G, blockIdx.x) : 0, u_end = (int)blockIdx.x < G ? paged_cut(W, G, blockIdx.x + 1) : 0;
+  const PagedLine line = paged_line(smem + L::OUT, g.B, tmem_holder + 4);
+  paged_prefix<PBLK, PTHREADS>(g, line, true);
+  const unsigned W = line.prefix[g.B];
+  const int G = (int)min(W, gridDim.x);
+  const PagedShares shares(W, G);
+  const unsigned u_begin = (int)blockIdx.x < G ? shares.first(blockIdx.x) : 0, u_end = (int)blockIdx.x < G ? shares.first(blockIdx.x + 1) : 0;
   PagedItem it{};
-  if (u_begin < u_end) it = paged_find<PBLK>(g, prefix, u_begin);
-  if (threadIdx.x == 0) paged_join_note(g, a.notes, it, W, G, blockIdx.x, u_begin < u_end, u_begin > it.u0);
+  if (u_begin < u_end) it = paged_find<PBLK>(g, line, u_begin);
+  if (threadIdx.x == 0) paged_join_note(g, a.notes, it, shares, blockIdx.x, u_begin < u_end && u_begin > it.u0);
   pdl_next();
   tc_fence_before();
   __syncthreads();                                         // the prefix makes room for outputs
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
         int id = page_of(it, (int)(u_begin - it.u0));
         load_q(it);
         load_k(it, (int)(u_begin - it.u0), id);
-        for (long long u = u_begin; u < u_end && ok; ++u) {
+        for (unsigned u = u_begin; u < u_end && ok; ++u) {
           const PagedItem cur = it;
           const int i = (int)(u - cur.u0);
           int next_id = -1;
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
         __syncwarp();
       };
       uint32_t blocks = 0, parts = 0, done = 0, pI[2] = {0, 0};
-      for (long long u = u_begin; u < u_end && ok;) {
+      for (unsigned u = u_begin; u < u_end && ok;) {
         const Part p = part_of(g, it, u, u_end);
         for (int i = p.i0; i < p.i1 && ok; ++i, ++blocks) {
           const int st = blocks & 1;
@@ -246,8 +247,8 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
     } else if (warp == 2) {
       // ---------------------------------------------------------------- value rows that hold no token
       uint32_t tails[2] = {0, 0}, blocks = 0;
-      for (long long u = u_begin; u < u_end;) {
-        const long long ue = min(u_end, it.u0 + it.span.n);
+      for (unsigned u = u_begin; u < u_end;) {
+        const unsigned ue = min(u_end, it.u0 + it.span.n);
         bool ok = true;
         for (int i = (int)(u - it.u0); i < (int)(ue - it.u0) && ok; ++i) {
           const int key0 = it.span.block(i) * PBLK, st = blocks++ & 1;
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
     const float sl2 = a.scale * 1.4426950408889634f;
     uint32_t sc = 0, oc = 0;                               // S rows taken, P tiles handed over
     bool ok = true;
-    for (long long u = u_begin; u < u_end && ok;) {
+    for (unsigned u = u_begin; u < u_end && ok;) {
       const Part p = part_of(g, it, u, u_end);
       const int n_t = t ? p.n1 : p.n0;
       const int first_row = it.t * g.tile_rows + t * half_rows, rows = min(half_rows, it.s.n * g.rep - first_row);   // rows <= 0: no such tile
@@ -575,6 +576,7 @@ int launch_prefill(PrefillArgs& a, int page, int join_z, cudaStream_t st) {
   const uint32_t box[3] = {64, (uint32_t)a.g.rep, (uint32_t)a.tile_toks};
   rc = make_tmap_nd_bf16(&tmQ, a.q, 3, dims, strides, box);
   if (rc != ELFA_OK) return rc;
+  ELFA_REQUIRE(paged_units_fit(a.g, PBLK), "paged_attention: too much work for one call (2^32 tiles of 256 rows by 128 keys)");
   ELFA_CUDA(allow_shared<paged_prefill_kernel<HDP>>(PrefillSmem<HDP>::DYN));
   const int grid = 148;
   paged_prefill_kernel<HDP><<<grid, PTHREADS, PrefillSmem<HDP>::DYN, st>>>(tmQ, tmKV, a);
