@@ -6,6 +6,7 @@ handlers)::
     train --config F [--resume P] [--data P] [--checkpoint-dir D]
     evaluate --checkpoint P --data P [--config F] [--max-tokens N]
     generate --checkpoint P [--prompt S] [--max-tokens 256] [--temperature 1.0] [--top-p 0.9] [--config F]
+             [--samples N] [--top-k K] [--min-p M] [--window W] [--sinks S]     (softmax-attention family: paged cache, draws on the device)
     smoke-test [--config configs/smoke.yaml]
     checkpoint list [--dir checkpoints] | validate --path P | convert --input P --output P [--format efla_native|safetensors|pytorch]
     tokenizer train --corpus F [--output tokenizer.bin] [--vocab-size 65536] [--type bpe]
@@ -122,6 +123,11 @@ def cmd_generate(a) -> int:
     tr, cfg = _load_for_inference(a.checkpoint, a.config)
     tok = Tokenizer.load(cfg.data.tokenizer_path) if os.path.exists(cfg.data.tokenizer_path) else None
     g = Generator(tr.model, tok, tr.device)
+    if a.samples > 1 or a.top_k or a.min_p or a.window or a.sinks:
+        ids = tok.encode(a.prompt) if tok is not None else [min(b, cfg.model.vocab_size - 1) for b in a.prompt.encode()]
+        for out in g.generate_batch([ids], a.max_tokens, a.temperature, a.top_k, a.top_p, a.min_p, samples=a.samples, window=a.window or None, sinks=a.sinks)[0]:
+            print(tok.decode(out) if tok is not None else ",".join(str(i) for i in out))
+        return 0
     if tok is not None:
         print(g.generate(a.prompt, a.max_tokens, a.temperature, a.top_p))
     else:
@@ -279,6 +285,11 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--max-tokens", type=int, default=256)
     g.add_argument("--temperature", type=float, default=1.0)
     g.add_argument("--top-p", type=float, default=0.9)
+    g.add_argument("--samples", type=int, default=1, help="continuations of the prompt, which runs once")
+    g.add_argument("--top-k", type=int, default=0)
+    g.add_argument("--min-p", type=float, default=0.0)
+    g.add_argument("--window", type=int, default=0, help="tokens see the last W ones ...")
+    g.add_argument("--sinks", type=int, default=0, help="... and the first S")
     g.add_argument("--config")
     g.set_defaults(fn=cmd_generate)
     s = sub.add_parser("smoke-test", allow_abbrev=False)

@@ -16,6 +16,7 @@ from typing import Dict, List, Optional
 
 import torch
 
+from .. import ops
 from ..data import BinaryDataset, DataLoader
 
 
@@ -101,6 +102,76 @@ class Generator:
                 logits, states = self.model.forward_with_states(torch.tensor([[nxt]], device=self.device), states)
                 last = logits[0, -1]
         return ids
+
+    @torch.no_grad()
+    def generate_batch(self, prompts: List[List[int]], max_new_tokens: int = 256, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                       min_p: float = 0.0, samples: int = 1, seed: Optional[int] = None, eos_id: Optional[int] = None, window: Optional[int] = None,
+                       sinks: int = 0, page_size: int = 64, chunk: int = 2048) -> List[List[List[int]]]:
+        """``samples`` continuations of each prompt, all at once, from a cache of pages (softmax-attention family): a prompt runs once, in pieces of at most ``chunk``
+        tokens, its samples fork off and share its pages, every step brings one token of each unfinished sequence, and tokens are drawn on the device
+        (:func:`elfa_b200.ops.sample`). With a ``window`` tokens see the last ``window`` ones and the first ``sinks``, and pages out of sight are used again. Ends a
+        sequence behind ``eos_id``, or before the model's positions run out. Returns prompt and continuation of ``[prompt][sample]``."""
+        if not hasattr(self.model, "forward_paged"):
+            raise ValueError("generate_batch wants a model with a paged cache (the softmax-attention family)")
+        if samples < 1 or chunk < 1:
+            raise ValueError("at least one sample, and at least one token in a piece of a prompt")
+        self.model.eval()
+        dev = self.device
+        prompts = [list(p) or [0] for p in prompts]
+        limit = self.model.pos_embed.shape[0] if self.model.pos_embed is not None else 1 << 62
+        longest = [min(len(p) + max_new_tokens, limit) for p in prompts]
+        if any(len(p) > limit for p in prompts):
+            raise ValueError(f"a prompt is longer than the model's {limit} positions")
+        live = -(-min(max(longest, default=0), (window or limit) + sinks + chunk) // page_size) + 2        # pages of one sequence that are in use
+        pages = sum(-(-len(p) // page_size) + samples * min(-(-n // page_size) - len(p) // page_size + 1, live) for p, n in zip(prompts, longest))
+        cache = self.model.new_paged_cache(max(pages, 1), page_size, window, sinks)
+        gen = torch.Generator(device=dev)
+        if seed is not None:
+            gen.manual_seed(seed)
+        else:
+            gen.seed()
+        roots, last = [cache.add() for _ in prompts], [None] * len(prompts)
+        done = [0] * len(prompts)
+        while any(d < len(p) for d, p in zip(done, prompts)):                     # prompts, up to `chunk` tokens of them in a call
+            part, room = [], chunk
+            for i, p in enumerate(prompts):
+                n = min(len(p) - done[i], room)
+                if n > 0:
+                    part.append((i, n))
+                    room -= n
+            ids = torch.tensor([t for i, n in part for t in prompts[i][done[i]:done[i] + n]], device=dev)
+            logits = self.model.forward_paged(ids, [roots[i] for i, _ in part], [n for _, n in part], cache)
+            for row, (i, n) in zip(logits, part):
+                done[i] += n
+                last[i] = row
+        out = [[list(p) for _ in range(samples)] for p in prompts]
+        seqs = [(i, j, s) for i, r in enumerate(roots) for j, s in enumerate([r] + cache.fork(r, samples - 1))]
+        logits = torch.stack([last[i] for i, _, _ in seqs]) if seqs else None
+        for step in range(max_new_tokens):
+            seqs_left = [x for x in range(len(seqs)) if len(out[seqs[x][0]][seqs[x][1]]) < limit]
+            if len(seqs_left) < len(seqs):
+                for x in set(range(len(seqs))) - set(seqs_left):
+                    cache.free(seqs[x][2])
+                seqs, logits = [seqs[x] for x in seqs_left], logits[seqs_left]
+            if not seqs:
+                break
+            noise = torch.empty(logits.shape, dtype=torch.float32, device=dev).exponential_(generator=gen) if temperature > 0 else None
+            ids = ops.sample(logits, noise, temperature, top_k, top_p, min_p)
+            keep = []
+            for x, ((i, j, s), t) in enumerate(zip(seqs, ids.tolist())):
+                if t < 0:
+                    raise FloatingPointError("logits without a finite number: nothing to draw from")
+                out[i][j].append(t)
+                if t == eos_id:
+                    cache.free(s)
+                else:
+                    keep.append(x)
+            if len(keep) < len(seqs):
+                seqs, ids = [seqs[x] for x in keep], ids[keep]
+            if not seqs or step + 1 == max_new_tokens:
+                break
+            logits = self.model.forward_paged(ids, [s for _, _, s in seqs], [1] * len(seqs), cache)
+        return out
 
     def generate_greedy(self, prompt_ids, max_new_tokens=256):
         return self.generate_ids(prompt_ids, max_new_tokens, temperature=0.0)

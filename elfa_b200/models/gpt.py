@@ -20,7 +20,8 @@ Parameter names (checkpoint keys) extend the reference's naming style
 from __future__ import annotations
 
 import math
-from typing import Optional
+from dataclasses import dataclass
+from typing import Optional, Sequence
 
 import torch
 import torch.nn as nn
@@ -30,6 +31,7 @@ from ..config import Config
 from ..parallel.mesh import ParallelContext
 from ..parallel import tp as tpl
 from ..quant.qat import QuantSpec
+from ..runtime.paged_cache import PagedBatch, PagedCache
 from . import streaming
 
 
@@ -68,6 +70,14 @@ def _attend_cached(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.T
     return o.reshape(s_, B, H * hd).to(q.dtype)
 
 
+@dataclass
+class PagedLayer:
+    """What one layer's attention needs of a paged cache in one call."""
+    pages: PagedCache
+    layer: int
+    batch: PagedBatch
+
+
 @streaming.stands_in_for("forward")
 class Attention(nn.Module):
     def __init__(self, cfg: Config, pc: ParallelContext, dtype, device, init_std: float, out_std: float):
@@ -97,6 +107,11 @@ class Attention(nn.Module):
         else:
             qkv = h.view(S, B, 3, H, hd)
             q, k, v = qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2]
+        if isinstance(cache, PagedLayer):                         # rows of many sequences, keys and values in pages
+            rows = [t.reshape(S * B, t.shape[2], hd) for t in (q, k, v)]
+            cache.pages.write(cache.layer, rows[1], rows[2], cache.batch)
+            o = cache.pages.attend(cache.layer, rows[0], cache.batch).view(S, B, H * hd)
+            return tpl.row_parallel_linear(o, self.w_o, self.pc, quant=self.quant)
         if cache is not None and cache.get("k") is not None:
             # incremental decoding: the new rows attend to the cached keys / values and, causally, to each other
             if ops.attention_decode_native(q, k, v, cache["k"], cache["v"]):
@@ -350,6 +365,37 @@ class GPTModel(nn.Module):
         states["pos"] += ids.shape[1]
         head = self.lm_head if self.lm_head is not None else self.embed_tokens
         return tpl.vocab_parallel_logits(n, head, self.pc, gather=True).transpose(0, 1), states
+
+    def new_paged_cache(self, pages: int, page_size: int = 64, window: Optional[int] = None, sinks: int = 0) -> PagedCache:
+        """A cache of ``pages`` pages of ``page_size`` tokens for this model's layers (see :meth:`forward_paged`)."""
+        at = self.blocks[0].attn
+        return PagedCache(len(self.blocks), pages, page_size, at.n_kv_heads, at.head_dim, self.dtype, self.embed_tokens.device, window, sinks)
+
+    @torch.no_grad()
+    def forward_paged(self, ids: torch.Tensor, seqs: Sequence[int], new: Sequence[int], cache: PagedCache, all_logits: bool = False) -> torch.Tensor:
+        """The next ``new[i]`` tokens of sequence ``seqs[i]`` of ``cache`` for all ``i`` at once, one after the other in ``ids [T]``: prompts or pieces of them,
+        single tokens of sequences that are being generated, in any mixture. Returns the logits behind each sequence's last new token ``[B, V]``, or of all
+        tokens ``[T, V]`` (a sequence without a new token has no logits of its own then: its row is that of the token before in ``ids``). One rank, without gradients."""
+        assert self.pc.tp_size == 1 and self.pc.cp_size == 1, "a paged cache runs on one rank"
+        if ids.dim() != 1 or ids.shape[0] != sum(new):
+            raise ValueError(f"ids must hold the new tokens of all sequences, [{sum(new)}], got {tuple(ids.shape)}")
+        if len(cache.pool) != len(self.blocks):
+            raise ValueError(f"the cache has {len(cache.pool)} layers, the model {len(self.blocks)}")
+        if self.pos_embed is not None:
+            end = max(cache.length(s) + n for s, n in zip(seqs, new))
+            if end > self.pos_embed.shape[0]:
+                raise ValueError(f"position {end} is past the model's {self.pos_embed.shape[0]} learned positions")
+        batch = cache.append(seqs, new)
+        x = ops.embedding(ids.view(-1, 1), self.embed_tokens, None, 0, self.vocab_lo, seq_first=True, vocab_total=self.cfg.model.vocab_size)   # [T, 1, D]
+        if self.pos_embed is not None:
+            x = x + self.pos_embed[batch.positions].unsqueeze(1)
+        pending = None
+        for i, blk in enumerate(self.blocks):
+            x, pending = blk(x, pending, PagedLayer(cache, i, batch))
+        n, _ = self.final_norm(x, pending)
+        n = n[:, 0] if all_logits else n[batch.last.clamp_min(0), 0]
+        head = self.lm_head if self.lm_head is not None else self.embed_tokens
+        return tpl.vocab_parallel_logits(n.unsqueeze(1), head, self.pc, gather=True)[:, 0]
 
     def forward(self, ids: torch.Tensor, targets: Optional[torch.Tensor] = None, pos0: int = 0,
                 loss_denominator: Optional[float] = None, grad_scale: float = 1.0, doc_start: Optional[torch.Tensor] = None):

@@ -14,6 +14,7 @@ reference: ``src/eval/evaluator.zig:419-470`` (generation runs the whole context
 from __future__ import annotations
 
 import array
+import functools
 import math
 from typing import Optional, Sequence
 
@@ -60,34 +61,41 @@ def paged_attention_ref(q: torch.Tensor, pages: torch.Tensor, table: torch.Tenso
     return out.reshape(T, H * hd).to(q.dtype)
 
 
-def _check(pages: torch.Tensor, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, what: str) -> None:
-    if pages.dim() != 5 or pages.shape[1] != 2:
-        raise ValueError(f"{what}: pages must be [P, 2, Hkv, page, hd], got {tuple(pages.shape)}")
-    B = kv_len.shape[0] if kv_len.dim() == 1 else -1
-    if B < 0 or table.dim() != 2 or table.shape[0] != B or q_start.shape != (B + 1,):
+def _check(pages: torch.Tensor, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, what: str):
+    """The shapes ``(P, Hkv, page, hd, B, N)`` of arguments that fit each other. A decoding step is issued in the time that its kernel takes: the tests of
+    good arguments are few and cheap."""
+    ps, ts = pages.shape, table.shape
+    if len(ps) != 5 or ps[1] != 2:
+        raise ValueError(f"{what}: pages must be [P, 2, Hkv, page, hd], got {tuple(ps)}")
+    if len(ts) != 2 or kv_len.shape != ts[:1] or q_start.shape != (ts[0] + 1,):
         raise ValueError(f"{what}: table [B, N], q_start [B + 1] and kv_len [B] do not fit each other: "
-                         f"{tuple(table.shape)}, {tuple(q_start.shape)}, {tuple(kv_len.shape)}")
-    dev = pages.device
-    if table.device != dev or q_start.device != dev or kv_len.device != dev:
-        raise ValueError(f"{what}: table, q_start and kv_len must be on the pages' device, {dev}")
-    if table.dtype != torch.int32 or q_start.dtype != torch.int32 or kv_len.dtype != torch.int32:
+                         f"{tuple(ts)}, {tuple(q_start.shape)}, {tuple(kv_len.shape)}")
+    dev = pages.get_device()
+    if not table.get_device() == q_start.get_device() == kv_len.get_device() == dev:
+        raise ValueError(f"{what}: table, q_start and kv_len must be on the pages' device, {pages.device}")
+    if not (table.dtype is q_start.dtype is kv_len.dtype is torch.int32):
         raise TypeError(f"{what}: table, q_start and kv_len must be int32")
+    if dev >= 0:
+        if pages.dtype is not torch.bfloat16:
+            raise TypeError(f"{what}: bf16 required on CUDA, got {pages.dtype}")
+        if ps[3] not in PAGE_SIZES or ps[4] % 8 or not 8 <= ps[4] <= 128:
+            raise ValueError(f"{what}: pages of {PAGE_SIZES} tokens and head dimensions that are multiples of 8 up to 128, got {ps[3]} and {ps[4]}")
+        if not pages.is_contiguous() or pages.data_ptr() % 16:
+            raise ValueError(f"{what}: pages must be contiguous and 16-byte aligned")
+    return ps[0], ps[2], ps[3], ps[4], ts[0], ts[1]
 
 
-def _check_cuda(pages: torch.Tensor, what: str) -> None:
-    if pages.dtype != torch.bfloat16:
-        raise TypeError(f"{what}: bf16 required on CUDA, got {pages.dtype}")
-    if pages.shape[3] not in PAGE_SIZES or pages.shape[4] % 8 or not 8 <= pages.shape[4] <= 128:
-        raise ValueError(f"{what}: pages of {PAGE_SIZES} tokens and head dimensions that are multiples of 8 up to 128, got {pages.shape[3]} and {pages.shape[4]}")
-    if not pages.is_contiguous() or pages.data_ptr() % 16:
-        raise ValueError(f"{what}: pages must be contiguous and 16-byte aligned")
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
+def _rows(t: torch.Tensor, hd: int) -> torch.Tensor:
     """``t [T, heads, hd]`` with packed heads on 16-byte boundaries: itself (a slice of a fused projection is), or a copy."""
-    if t.stride(2) == 1 and t.stride(1) == t.shape[2] and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
+    st = t.stride()
+    if st[2] == 1 and st[1] == hd and st[0] % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+@functools.lru_cache(maxsize=256)
+def _scratch_floats(N: int, page: int, H: int, Hkv: int, hd: int, max_new: int) -> int:
+    return lib.raw("elfa_paged_attention_scratch")(N, page, H, Hkv, hd, max_new)
 
 
 def paged_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
@@ -96,10 +104,12 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q
     (:func:`paged_write`). A query at position ``p`` sees the keys up to ``p``; with a ``window`` the last ``window`` of them and the first ``sinks``; never those of
     pages that are not there. A row that sees nothing (or only scores of -inf) is zero, and what a row does not see cannot reach it whatever it holds. ``H`` is a
     multiple of ``Hkv``. ``max_new``: an upper bound of the new tokens of one sequence, known to the host; without it the number of rows. Returns ``[T, H * hd]``."""
-    _check(pages, table, q_start, kv_len, "paged_attention")
-    if q.dim() != 3 or q.shape[2] != pages.shape[4] or q.shape[1] < 1 or q.shape[1] % pages.shape[2]:
-        raise ValueError(f"paged_attention: q must be [T, H, {pages.shape[4]}] with H a multiple of {pages.shape[2]}, got {tuple(q.shape)}")
-    if q.dtype != pages.dtype or q.device != pages.device:
+    P, Hkv, page, hd, B, N = _check(pages, table, q_start, kv_len, "paged_attention")
+    qs = q.shape
+    if len(qs) != 3 or qs[2] != hd or qs[1] < 1 or qs[1] % Hkv:
+        raise ValueError(f"paged_attention: q must be [T, H, {hd}] with H a multiple of {Hkv}, got {tuple(qs)}")
+    dev = q.get_device()
+    if q.dtype is not pages.dtype or dev != pages.get_device():
         raise TypeError("paged_attention: q and pages differ in type or device")
     if window is not None and window < 1:
         raise ValueError("paged_attention: a window holds at least the token itself")
@@ -107,51 +117,45 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q
         raise ValueError("paged_attention: negative sinks")
     if torch.is_grad_enabled() and (q.requires_grad or pages.requires_grad):
         raise RuntimeError("paged_attention has no backward pass: call it without gradients")
-    T, H, hd = q.shape
-    B, N = table.shape
-    if not q.is_cuda:
+    T, H = qs[0], qs[1]
+    if dev < 0:
         return paged_attention_ref(q, pages, table, q_start, kv_len, window, sinks, scale)
-    _check_cuda(pages, "paged_attention")
-    out = torch.empty((T, H * hd), dtype=q.dtype, device=q.device)
+    out = torch.empty((T, H * hd), dtype=torch.bfloat16, device=q.device)
     if T == 0:
         return out
     if B == 0 or N == 0:
         return out.zero_()
-    q, table = _rows(q), table.contiguous()
-    P, _, Hkv, page, _ = pages.shape
     max_new = T if max_new is None else min(int(max_new), T)
     if max_new < 1:
         raise ValueError("paged_attention: max_new must be positive where there are new tokens")
-    if not q_start.is_contiguous() or not kv_len.is_contiguous():
-        q_start, kv_len = q_start.contiguous(), kv_len.contiguous()
-    n = lib.raw("elfa_paged_attention_scratch")(N, page, H, Hkv, hd, max_new)
+    q = _rows(q, hd)
+    if not (table.is_contiguous() and q_start.is_contiguous() and kv_len.is_contiguous()):
+        table, q_start, kv_len = table.contiguous(), q_start.contiguous(), kv_len.contiguous()
+    n = _scratch_floats(N, page, H, Hkv, hd, max_new)
     scratch = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
-    sc = scale if scale is not None else hd ** -0.5
-    stream = stream_ptr(q)
+    pt, pq, pk = table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr()
     for b in range(0, B, _MAX_SEQS):           # q_start counts from the first row of the whole call in every part
-        m = min(_MAX_SEQS, B - b)
-        lib.call("elfa_paged_attention", q, q.stride(0), pages, table.data_ptr() + 4 * b * N, q_start.data_ptr() + 4 * b, kv_len.data_ptr() + 4 * b, out,
-                 scratch, m, N, P, page, T, H, Hkv, hd, max_new, min(window or 0, 1 << 30), min(sinks, 1 << 30), sc, stream)
+        lib.call("elfa_paged_attention", q, q.stride(0), pages, pt + 4 * b * N, pq + 4 * b, pk + 4 * b, out, scratch, min(_MAX_SEQS, B - b), N, P, page, T, H,
+                 Hkv, hd, max_new, min(window or 0, 1 << 30), min(sinks, 1 << 30), scale if scale is not None else hd ** -0.5, stream_ptr(q))
     return out
 
 
 def paged_write(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor) -> None:
     """Writes the new tokens' keys and values ``k, v [T, Hkv, hd]`` (rows may be strided) into their places, in place. Every new token needs a page."""
-    _check(pages, table, q_start, kv_len, "paged_write")
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (pages.shape[2], pages.shape[4]):
-        raise ValueError(f"paged_write: k and v must be [T, {pages.shape[2]}, {pages.shape[4]}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    if k.dtype != pages.dtype or v.dtype != pages.dtype or k.device != pages.device or v.device != pages.device:
+    P, Hkv, page, hd, B, N = _check(pages, table, q_start, kv_len, "paged_write")
+    ks, dev = k.shape, k.get_device()
+    if len(ks) != 3 or ks != v.shape or ks[1] != Hkv or ks[2] != hd:
+        raise ValueError(f"paged_write: k and v must be [T, {Hkv}, {hd}], got {tuple(ks)} and {tuple(v.shape)}")
+    if not (k.dtype is v.dtype is pages.dtype) or not dev == v.get_device() == pages.get_device():
         raise TypeError("paged_write: k, v and pages differ in type or device")
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or pages.requires_grad):
         raise RuntimeError("paged_write has no backward pass: call it without gradients")
-    T, Hkv, hd = k.shape
-    B, N = table.shape
+    T = ks[0]
     if T == 0:
         return
     if B == 0 or N == 0:
         raise ValueError("paged_write: new tokens without a sequence or a page")
-    if not k.is_cuda:
-        page = pages.shape[3]
+    if dev < 0:
         starts = q_start.tolist()
         for b, kv in enumerate(kv_len.tolist()):
             n = starts[b + 1] - starts[b]
@@ -162,11 +166,10 @@ def paged_write(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, table: to
             pages[ids, 0, :, pos % page] = k[starts[b]:starts[b + 1]]
             pages[ids, 1, :, pos % page] = v[starts[b]:starts[b + 1]]
         return
-    _check_cuda(pages, "paged_write")
-    k, v, table = _rows(k), _rows(v), table.contiguous()
-    if not q_start.is_contiguous() or not kv_len.is_contiguous():
-        q_start, kv_len = q_start.contiguous(), kv_len.contiguous()
-    lib.call("elfa_paged_write", k, k.stride(0), v, v.stride(0), pages, table, q_start, kv_len, B, N, pages.shape[0], pages.shape[3], T, Hkv, hd, stream_ptr(k))
+    k, v = _rows(k, hd), _rows(v, hd)
+    if not (table.is_contiguous() and q_start.is_contiguous() and kv_len.is_contiguous()):
+        table, q_start, kv_len = table.contiguous(), q_start.contiguous(), kv_len.contiguous()
+    lib.call("elfa_paged_write", k, k.stride(0), v, v.stride(0), pages, table, q_start, kv_len, B, N, P, page, T, Hkv, hd, stream_ptr(k))
 
 
 def copy_pages(pages: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> None:

@@ -47,9 +47,11 @@ def _setting(value: _Setting, name: str, dtype: torch.dtype, logits: torch.Tenso
     """(tensor or None, number) of a setting that is one number for all rows or a tensor with one per row."""
     if not isinstance(value, torch.Tensor):
         return None, value
-    if value.shape != (logits.shape[0],) or value.device != logits.device:
+    if value.shape != logits.shape[:1] or value.get_device() != logits.get_device():
         raise ValueError(f"sample: {name} must be a number or one per row, [{logits.shape[0]}] on {logits.device}")
-    return value.to(dtype).contiguous(), 0
+    if value.dtype is not dtype or not value.is_contiguous():
+        value = value.to(dtype).contiguous()
+    return value, 0
 
 
 def sample(logits: torch.Tensor, noise: Optional[torch.Tensor], temperature: _Setting = 1.0, top_k: _Setting = 0, top_p: _Setting = 1.0,
@@ -64,26 +66,29 @@ def sample(logits: torch.Tensor, noise: Optional[torch.Tensor], temperature: _Se
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"sample: logits must be [B, V], got {tuple(logits.shape)}")
     B, V = logits.shape
+    dev = logits.get_device()
     if noise is None:
         if isinstance(temperature, torch.Tensor) or temperature > 0:
             raise ValueError("sample: noise may be left out where temperature is 0 for all rows")
-    elif noise.shape != logits.shape or noise.dtype != torch.float32 or noise.device != logits.device:
+    elif noise.shape != logits.shape or noise.dtype is not torch.float32 or noise.get_device() != dev:
         raise ValueError(f"sample: noise must be fp32 {tuple(logits.shape)} on {logits.device}")
-    settings = [_setting(temperature, "temperature", torch.float32, logits), _setting(top_k, "top_k", torch.int32, logits),
-                _setting(top_p, "top_p", torch.float32, logits), _setting(min_p, "min_p", torch.float32, logits)]
+    t, tn = _setting(temperature, "temperature", torch.float32, logits)
+    k, kn = _setting(top_k, "top_k", torch.int32, logits)
+    p, pn = _setting(top_p, "top_p", torch.float32, logits)
+    m, mn = _setting(min_p, "min_p", torch.float32, logits)
     if B == 0:
         return torch.empty(0, dtype=torch.int64, device=logits.device)
-    if not logits.is_cuda:
-        rows = [t if t is not None else torch.full((B,), n, dtype=d) for (t, n), d in zip(settings, (torch.float32, torch.int32, torch.float32, torch.float32))]
+    if dev < 0:
+        rows = [s if s is not None else torch.full((B,), n, dtype=d)
+                for s, n, d in ((t, tn, torch.float32), (k, kn, torch.int32), (p, pn, torch.float32), (m, mn, torch.float32))]
         return sample_ref(logits, noise, *rows)
-    if logits.dtype not in (torch.bfloat16, torch.float32):
+    if logits.dtype is not torch.bfloat16 and logits.dtype is not torch.float32:
         logits = logits.float()
     if logits.stride(1) != 1:
         logits = logits.contiguous()
     if noise is not None and noise.stride(1) != 1:
         noise = noise.contiguous()
     out = torch.empty(B, dtype=torch.int64, device=logits.device)
-    (t, tn), (k, kn), (p, pn), (m, mn) = settings
     lib.call("elfa_sample", logits, int(logits.dtype == torch.float32), logits.stride(0), noise, noise.stride(0) if noise is not None else 0, t, k, p, m, tn,
              max(0, min(int(kn), V)), pn, mn, out, B, V, stream_ptr(logits))
     return out
