@@ -322,58 +322,71 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
             for (int x = 0; x < 32; ++x) s[c * 32 + x] = see >> x & 1u ? s[c * 32 + x] : 0xff800000u;      // -inf
           }
         }
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto row_max = [&]() {
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int x = 0; x < 128; x += 2) mx4[(x >> 1) & 3] = max3(mx4[(x >> 1) & 3], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
-        if (i == p.i0) {
-          m = mx;
-        } else {
-          const bool grow = mx - m > 8.f;
-          if (__any_sync(0xffffffffu, grow)) {
-            ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_OFULL + t), (oc - 1) & 1, abort_flag, g.status));
-            if (!ok) break;
-            landed = true;
-            tc_fence_after();
-            const float m_new = grow ? mx : m, alpha = m_new == m ? 1.f : fast_exp2(m - m_new);
+          for (int x = 0; x < 128; x += 2) mx4[(x >> 1) & 3] = max3(mx4[(x >> 1) & 3], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
+          return fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
+        };
+        // The exponentials do not wait for the row's maximum. Their reference may lag behind it: as long as a block's sum stays below 2^8 none of them is above that.
+        // Where it does not (rare behind an item's first blocks), or nothing has been seen yet, the maximum is found, the sums are scaled and the row is done again.
+        bool fresh = i == p.i0;
+        for (;;) {
+          if (fresh) {
+            const float mx = row_max();
+            const bool grow = mx > m;
+            const float m_new = grow ? mx : m, alpha = grow ? fast_exp2(m - m_new) : 1.f;
+            if (i > p.i0) {
+              if (!landed) ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_OFULL + t), (oc - 1) & 1, abort_flag, g.status));
+              if (!ok) break;
+              landed = true;
+              tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < HDP / 16; ++c) {           // narrow pieces: the S row stays in registers meanwhile
-              uint32_t o[16];
-              tmem_ld16(TM_O[t] + lane_addr + c * 16, o);
-              tmem_ld_wait();
+              for (int c = 0; c < HDP / 16; ++c) {         // narrow pieces: the S row stays in registers meanwhile
+                uint32_t o[16];
+                tmem_ld16(TM_O[t] + lane_addr + c * 16, o);
+                tmem_ld_wait();
 #pragma unroll
-              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
-              tmem_st16(TM_O[t] + lane_addr + c * 16, o);
+                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+                tmem_st16(TM_O[t] + lane_addr + c * 16, o);
+              }
+              tmem_st_wait();
             }
-            tmem_st_wait();
             l *= alpha;
             m = m_new;
           }
-        }
-        const float neg_m = m == -INFINITY ? 0.f : -m;
-        const uint64_t sc2 = pack_f32x2(sl2, sl2), neg2 = pack_f32x2(neg_m, neg_m);
-        uint64_t ls[2] = {0ull, 0ull};
+          const float neg_m = m == -INFINITY ? 0.f : -m;
+          const uint64_t sc2 = pack_f32x2(sl2, sl2), neg2 = pack_f32x2(neg_m, neg_m);
+          uint64_t ls[2] = {0ull, 0ull};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[16];
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[16];
 #pragma unroll
-          for (int x = 0; x < 32; x += 2) {
-            float x0, x1;
-            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[c * 32 + x]), __uint_as_float(s[c * 32 + x + 1])), sc2, neg2), x0, x1);
-            const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
-            ls[(x >> 1) & 1] = add_f32x2(ls[(x >> 1) & 1], pack_f32x2(e0, e1));
-            w[x >> 1] = pack_bf16(e0, e1);
+            for (int x = 0; x < 32; x += 2) {
+              float x0, x1;
+              unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[c * 32 + x]), __uint_as_float(s[c * 32 + x + 1])), sc2, neg2), x0, x1);
+              const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
+              ls[(x >> 1) & 1] = add_f32x2(ls[(x >> 1) & 1], pack_f32x2(e0, e1));
+              w[x >> 1] = pack_bf16(e0, e1);
+            }
+            if (c == 0 && !landed) {                       // P is still the operand of the product before
+              ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_OFULL + t), (oc - 1) & 1, abort_flag, g.status));
+              landed = true;
+            }
+            if (ok) tmem_st16(TM_P[t] + lane_addr + c * 16, w);
           }
-          if (c == 0 && !landed) {                         // P is still the operand of the product before
-            ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_OFULL + t), (oc - 1) & 1, abort_flag, g.status));
+          if (!ok) break;
+          float a0, a1, a2, a3;
+          unpack_f32x2(ls[0], a0, a1);
+          unpack_f32x2(ls[1], a2, a3);
+          const float block = (a0 + a1) + (a2 + a3);
+          if (fresh || !__any_sync(0xffffffffu, block > 256.f || m == -INFINITY)) {
+            l += block;
+            break;
           }
-          if (ok) tmem_st16(TM_P[t] + lane_addr + c * 16, w);
+          fresh = true;
         }
         if (!ok) break;
-        float a0, a1, a2, a3;
-        unpack_f32x2(ls[0], a0, a1);
-        unpack_f32x2(ls[1], a2, a3);
-        l += (a0 + a1) + (a2 + a3);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
