@@ -36,6 +36,8 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 constexpr int ST = 512, SW = ST / 32;      // threads of a CTA
 constexpr int BINS = 8192, LIST = 4096;    // bins of width T / 256 below the maximum; tokens that are sorted
 constexpr float BINS_PER = 256.f;
+// Vectors of 16 bytes that a thread asks for at once, tokens of it whose variates it does: what 64 registers hold (twice as many of either cost 7 to 20 %).
+constexpr int EACH = 2, RACE = 8;
 
 // (key, index) as one number: larger is earlier in the order of falling logits, equal ones by index. Never 0.
 __device__ __forceinline__ unsigned long long place(float x, int i) { return (unsigned long long)order_key(x) << 32 | (uint32_t)~i; }
@@ -54,7 +56,7 @@ struct SampleShared {
   unsigned long long swap[LIST];
   double2 mail[2][8];                      // what the CTAs of the row send each other, by turns
   double2 red[SW];
-  double scan[3][SW];
+  double2 scan[SW];
   unsigned long long cut;                  // the last token that is kept
   double mass, target;
   long long before, upto;                  // tokens before and up to the end of the window
@@ -63,9 +65,10 @@ struct SampleShared {
 };
 enum { SORT_ALL, SORT_WINDOW, SEARCH };
 
-// A row belongs to a cluster of C CTAs: CTA r reads the r-th part of it, in every pass. Passes: the maximum; tokens per bin (and the whole mass); the tokens of
-// the few bins that the line runs through, which the first CTA sorts; and the race over what is kept, or over the sorted list alone where it holds all of it.
-// The row is read again from the L2 in each (a row of 131072 fp32 logits is 512 KB). What does not fit the list (many equal logits) is searched bit by bit.
+// A row belongs to a cluster of C CTAs: CTA r reads the r-th part of it, in every pass. Passes: the maximum; tokens per bin (and the whole mass); the race over
+// the tokens in front of the few bins that a filter's line runs through, whose tokens the first CTA sorts to find out which of them race too. Where the sorted list
+// holds all that can be kept, it races alone. The row is read again from the L2 in each pass (a row of 131072 fp32 logits is 512 KB). What does not fit the
+// list (many equal logits) is searched bit by bit, and then races in a pass of its own.
 template <typename T>
 __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ SampleArgs a, int C) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -104,14 +107,14 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     };
     if (rank == 0 && tid < head) single(tid);
     const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+    uint4 w[U];                            // asked for a batch ahead
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v0 + tid + u * ST < v1) w[u] = __ldg(xv + v0 + tid + u * ST);
     for (int v = v0 + tid; v < v1; v += U * ST) {
-      uint4 w[U];
       float y[U][PER];
       int at[U];
       const int n = min(U, (v1 - v + ST - 1) / ST);
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u < n) w[u] = __ldg(xv + v + u * ST);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const T* e = reinterpret_cast<const T*>(&w[u]);
@@ -119,13 +122,16 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
 #pragma unroll
         for (int k = 0; k < PER; ++k) y[u][k] = value(e[k]);
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (v + (U + u) * ST < v1) w[u] = __ldg(xv + v + (U + u) * ST);
       f(y, at, std::integral_constant<int, U>{}, std::integral_constant<int, PER>{}, n);
     }
     const int tail = head + vecs * PER;
     if (rank == C - 1 && tail + tid < V) single(tail + tid);
   };
   auto each = [&](auto&& f) {
-    each_batch(std::integral_constant<int, 4>{}, [&](auto& v, auto& at, auto runs, auto len, int n) {
+    each_batch(std::integral_constant<int, EACH>{}, [&](auto& v, auto& at, auto runs, auto len, int n) {
 #pragma unroll
       for (int u = 0; u < runs.value; ++u) {
         if (u >= n) break;
@@ -207,6 +213,72 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
   };
   auto kept = [&](float v, int i) { return v > last_value || (v == last_value && i <= last_index); };
 
+  // The race of the tokens for which in(value, index, depth) holds; out(value, index, depth, weight) is told of the others. A rough score of every token, the
+  // exact one (settle) of the best of each thread, or of all of its tokens where another one (or the line of min_p) was within 10^-4, more than the rough
+  // scores are off. The variates of a batch are asked for at once.
+  float bar = -1.f, second = -1.f;         // of this thread's rough scores
+  int bar_at = 0;
+  bool close = false, raced = false;
+  const float least = fmaxf(min_p, 0.f) * (1.f - 1e-5f), sure = min_p * (1.f + 1e-5f);
+  auto run_race = [&](auto&& in, auto&& out) {
+    bar = second = -1.f;
+    close = false;
+    float sum = 0.f;
+    each_batch(std::integral_constant<int, RACE / PER>{}, [&](auto& v, auto& at, auto runs, auto len, int n) {
+      if constexpr (len.value > 1) {       // the variates of the next batch on their way to the L2
+#pragma unroll
+        for (int u = 0; u < runs.value; ++u) {
+          const int next = at[u] + RACE * ST;
+          if (lane % (32 / PER) == 0 && next < V) asm volatile("prefetch.global.L2 [%0];" ::"l"(noise + next));
+        }
+      }
+      float w[runs.value][len.value], e[runs.value][len.value];
+#pragma unroll
+      for (int u = 0; u < runs.value; ++u)
+#pragma unroll
+        for (int q = 0; q < len.value; ++q) {
+          w[u][q] = -1.f;
+          e[u][q] = 1.f;
+          if (u >= n) continue;
+          const float y = depth(v[u][q]), r = rough(y);
+          if (in(v[u][q], at[u] + q, y)) {
+            sum += r;
+            if (r >= least) {
+              w[u][q] = r;
+              e[u][q] = __ldg(noise + at[u] + q);
+            }
+          } else {
+            out(v[u][q], at[u] + q, y, r);
+          }
+        }
+#pragma unroll
+      for (int u = 0; u < runs.value; ++u)
+#pragma unroll
+        for (int q = 0; q < len.value; ++q) {
+          float inv;
+          asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(e[u][q]));
+          const float sc = w[u][q] * inv;  // -1 of what does not race
+          if (sc > bar) bar_at = at[u] + q;
+          second = fmaxf(second, fminf(sc, bar));
+          bar = fmaxf(bar, sc);
+          if (min_p > 0.f) close = close | (w[u][q] >= 0.f && w[u][q] < sure);
+        }
+    });
+    close = close || (bar >= 0.f && !(second < bar * (1.f - 1e-4f)));
+    return sum;                            // the mass of those that raced, and of those that min_p keeps out
+  };
+  auto settle = [&](auto&& in) {
+    if (close) {
+      each([&](float v, int i) {
+        if (!in(v, i, depth(v))) return;
+        const float w = weight(v);
+        if (w >= min_p) race(w, i);
+      });
+    } else if (bar >= 0.f) {
+      race(weight(value(x[bar_at])), bar_at);
+    }
+  };
+
   if (k < V || p < 1.f) {
     for (int i = tid; i < BINS; i += ST) s.hist[i] = 0;
     if (tid == 0) s.fill = 0;
@@ -217,7 +289,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     each([&](float v, int) {
       const float y = depth(v);
       if (y >= BINS - 1.f) ++rest;
-      else atomicAdd(&s.hist[(int)y], 1u);
+      else atomicAdd(&s.hist[__float_as_uint(__fadd_rd(y, 8388608.f)) - 0x4b000000u], 1u);           // its whole part
       if (want_all) sum += rough(y);
     });
     if (rest) atomicAdd(&s.hist[BINS - 1], rest);
@@ -227,8 +299,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     // all of the row is counted
     // ---- each CTA adds a share of the bins up, for the row's first one: there 16 neighbouring bins per thread
     constexpr int OWN = BINS / ST;
-    const int share = BINS / 4 / C;
-    for (int i = rank * share + tid; i < (rank + 1) * share; i += ST) {
+    for (int i = BINS / 4 * rank / C + tid; i < BINS / 4 * (rank + 1) / C; i += ST) {
       uint4 h[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r)
@@ -250,25 +321,23 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
       }
     };
     // sums before this thread: v over the first CTA's threads
-    auto before_me = [&](double (&v)[3]) {
-      double incl[3] = {v[0], v[1], v[2]};
+    auto before_me = [&](double& u, double& v) {
+      auto scan = [&](double a, int upto) {                // inclusive, over `upto` lanes
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1)
-#pragma unroll
-        for (int q = 0; q < 3; ++q) {
-          const double u = __shfl_up_sync(0xffffffffu, incl[q], o);
-          if (lane >= o) incl[q] += u;
+        for (int o = 1; o < 32; o <<= 1) {
+          const double b = __shfl_up_sync(0xffffffffu, a, o);
+          if (o < upto && lane >= o) a += b;
         }
+        return a;
+      };
+      const double iu = scan(u, 32), iv = scan(v, 32);
       __syncthreads();
-      if (lane == 31)
-#pragma unroll
-        for (int q = 0; q < 3; ++q) s.scan[q][warp] = incl[q];
+      if (lane == 31) s.scan[warp] = make_double2(iu, iv);
       __syncthreads();
-#pragma unroll
-      for (int q = 0; q < 3; ++q) {
-        v[q] = incl[q] - v[q];
-        for (int w = 0; w < warp; ++w) v[q] += s.scan[q][w];
-      }
+      const double2 all = lane < SW ? s.scan[lane] : make_double2(0.0, 0.0);
+      const double wu = __shfl_sync(0xffffffffu, scan(all.x, SW), warp ? warp - 1 : 0), wv = __shfl_sync(0xffffffffu, scan(all.y, SW), warp ? warp - 1 : 0);
+      u = iu - u + (warp ? wu : 0.0);
+      v = iv - v + (warp ? wv : 0.0);
     };
     const int bin0 = tid * OWN;
     // The window (first CTA): where the number of tokens reaches `want`, or the mass may. A bin's tokens weigh between exp(-(bin + 1) / 256) and
@@ -277,18 +346,18 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     auto window_of_count = [&](double want) {
       unsigned int cnt[OWN];
       load_counts(cnt);
-      double at[3] = {0, 0, 0};
+      double at = 0.0, none = 0.0;
 #pragma unroll
-      for (int j = 0; j < OWN; ++j) at[0] += cnt[j];
-      before_me(at);
+      for (int j = 0; j < OWN; ++j) at += cnt[j];
+      before_me(at, none);
 #pragma unroll
       for (int j = 0; j < OWN; ++j) {
-        if (at[0] < want && at[0] + cnt[j] >= want) {
+        if (at < want && at + cnt[j] >= want) {
           s.b1 = s.b2 = bin0 + j;
-          s.before = (long long)at[0];
-          s.upto = (long long)(at[0] + cnt[j]);
+          s.before = (long long)at;
+          s.upto = (long long)(at + cnt[j]);
         }
-        at[0] += cnt[j];
+        at += cnt[j];
       }
       __syncthreads();
     };
@@ -308,20 +377,20 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         }
         w *= RATIO;
       }
-      double at[3] = {(double)n, sum, 0};
-      before_me(at);
+      double front = n, ahead = sum;                       // tokens and mass before this thread's bins
+      before_me(front, ahead);
       const double up = want * (1 - gap), down = want * (1 + gap);
       const bool ends_here = bin0 <= last && bin0 + OWN > last;
-      const double behind = (at[1] + sum) * (1 + 1e-6);
-      if ((at[1] < up && behind >= up) || (at[1] * shrink < down && behind * shrink >= down) || ends_here) {
+      const double behind = (ahead + sum) * (1 + 1e-6);
+      if ((ahead < up && behind >= up) || (ahead * shrink < down && behind * shrink >= down) || ends_here) {
         w = edge;
-        double high = at[1], count = at[0];
+        double high = ahead, count = front;
 #pragma unroll
         for (int j = 0; j < OWN; ++j) {
           const int bin = bin0 + j;
           if (bin > last) continue;
           double next = high + cnt[j] * w;
-          if (j == OWN - 1 || bin == last) next = fmax(next, at[1] + sum);   // what the next thread starts from
+          if (j == OWN - 1 || bin == last) next = fmax(next, ahead + sum);   // what the next thread starts from
           if (high < up && (next >= up || bin == last)) {
             s.b1 = bin;
             s.before = (long long)count;
@@ -346,15 +415,24 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         d->mode = mode;
       }
     };
-    // the window's tokens (those not behind `least`) to the list; the mass of the ones before the window
-    auto collect = [&]() {
+    // The window's tokens (those that are kept so far) to the list; the mass of the ones before it, which race here if this filter is the last one.
+    auto before_window = [&](float, int, float y) { return y < s.b1; };
+    auto collect = [&](bool last) {
       const float from = (float)s.b1, to = s.b2 == BINS - 1 ? CUDART_INF_F : (float)(s.b2 + 1);
+      auto in = [&](float, int, float y) { return y < from; };
+      auto list = [&](float v, int i, float y, float) {
+        if ((y < to || to == CUDART_INF_F) && kept(v, i)) s.list[atomicAdd(&s.fill, 1)] = place(v, i);           // the window's count fits
+      };
       float sum = 0.f;
-      each([&](float v, int i) {
-        const float y = depth(v), w = rough(y);
-        if (y < from) sum += w;
-        else if ((y < to || to == CUDART_INF_F) && kept(v, i)) s.list[atomicAdd(&s.fill, 1)] = place(v, i);      // the window's count fits
-      });
+      if (last) {
+        sum = run_race(in, list);
+      } else {
+        each([&](float v, int i) {
+          const float y = depth(v);
+          if (in(v, i, y)) sum += rough(y);
+          else list(v, i, y, 0.f);
+        });
+      }
       __syncthreads();
       const int fill = s.fill;
       const double2 all = total(sum, tid == 0 ? fill : 0);
@@ -429,11 +507,11 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     // first CTA: the mass of the first n of the list, and how many of them it takes until base + mass >= want (n, if that is not reached) in s.pos
     auto prefix = [&](int n, double base, double want) {
       const int each_n = (n + ST - 1) / ST, i0 = min(n, tid * each_n), i1 = min(n, i0 + each_n);
-      double at[3] = {0, 0, 0};
-      for (int i = i0; i < i1; ++i) at[0] += weight(value_of(s.list[i]));
+      double at = 0.0, none = 0.0;
+      for (int i = i0; i < i1; ++i) at += weight(value_of(s.list[i]));
       if (tid == 0) s.pos = n;
-      before_me(at);
-      double run = base + at[0];
+      before_me(at, none);
+      double run = base + at;
       for (int i = i0; i < i1; ++i) {
         const double next = run + weight(value_of(s.list[i]));
         if (run < want && next >= want) s.pos = i + 1;
@@ -442,6 +520,12 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
       if (i1 == n && i1 > i0) s.mass = run;
       __syncthreads();
       return s.mass;
+    };
+    auto race_list = [&](int n) {
+      for (int i = tid; i < n; i += ST) {
+        const float w = weight(value_of(s.list[i]));
+        if (w >= min_p) race(w, index_of(s.list[i]));
+      }
     };
     // bit by bit: the last token that is kept when `reach(least)` of them have to be: the largest place with reach(place) >= want
     auto search = [&](double want, auto&& count) {
@@ -483,7 +567,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
           mass = total(m, 0.0).x;
         }
       } else {
-        const double2 got = collect();
+        const double2 got = collect(mode == SORT_WINDOW && p >= 1.f);
         const double above = got.x;
         if (mode == SORT_ALL) {                            // the list holds all that can be kept
           if (rank != 0) return;
@@ -494,10 +578,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
             prefix(n, 0.0, fmax((double)p * m, 1e-30));
             n = s.pos;
           }
-          for (int i = tid; i < n; i += ST) {
-            const float w = weight(value_of(s.list[i]));
-            if (w >= min_p) race(w, index_of(s.list[i]));
-          }
+          race_list(n);
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) win = max(win, __shfl_xor_sync(0xffffffffu, win, o));
           __syncthreads();
@@ -513,6 +594,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
           sort((int)got.y);
           const int n = (int)(k - s.before);
           const double m = p < 1.f ? prefix(n, above, 1e300) : 0.0;
+          if (p >= 1.f) race_list(n);
           if (tid < C) {
             SampleShared* d = peer(&s, tid);
             d->cut = s.list[n - 1];
@@ -522,6 +604,10 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         meet();
         cut = s.cut;
         mass = s.mass;
+        if (p >= 1.f) {
+          settle(before_window);
+          raced = true;
+        }
         __syncthreads();
         if (tid == 0) s.fill = 0;          // for the next window; read and counted on behind the barriers before that
       }
@@ -536,7 +622,8 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         __syncthreads();
       }
       bool found = false;
-      for (int wide = 0; wide < 2 && !found; ++wide) {
+      // bf16 logits of one bin are one or two numbers: its middle says too little of them
+      for (int wide = std::is_same<T, float>::value ? 0 : 1; wide < 2 && !found; ++wide) {
         if (rank == 0) {
           window_of_mass(want, last, wide);
           if (tid == 0) tell(s.upto - s.before <= LIST ? SORT_WINDOW : SEARCH);
@@ -544,7 +631,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         meet();
         if (s.mode == SEARCH) break;
         keep_to(cut);
-        const double2 got = collect();
+        const double2 got = collect(true);
         if (rank == 0) {
           const int n = (int)got.y;
           sort(n);
@@ -554,58 +641,25 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
             holds = wide || (got.x < want && m >= want);
           }
           if (tid < C) peer(&s, tid)->cut = holds ? s.list[s.pos - 1] : 0;
+          if (holds) race_list(s.pos);
           __syncthreads();
         }
         if (tid == 0) s.fill = 0;
         meet();
         if (s.cut) {
-          cut = s.cut;
-          found = true;
+          found = raced = true;
+          settle(before_window);
         }
       }
       if (!found) cut = max(cut, search(want, [&](float v) { return (double)rough(depth(v)); }));
     }
   }
-  // A rough score of every token, the exact one of the best of each thread; of all of its tokens where another one (or the line of min_p) was within 10^-4, more than
-  // the rough scores are off. The variates of a batch are asked for at once.
-  keep_to(cut);
-  float bar = -1.f;
-  int bar_at = 0;
-  bool close = false;
-  float bar_value = 0.f;
-  const float least = fmaxf(min_p, 0.f) * (1.f - 1e-5f), sure = min_p * (1.f + 1e-5f);
-  each_batch(std::integral_constant<int, 16 / PER>{}, [&](auto& v, auto& at, auto runs, auto len, int n) {
-    float w[runs.value][len.value], e[runs.value][len.value];
-#pragma unroll
-    for (int u = 0; u < runs.value; ++u)
-#pragma unroll
-      for (int q = 0; q < len.value; ++q) {
-        w[u][q] = u < n && kept(v[u][q], at[u] + q) ? rough(depth(v[u][q])) : -1.f;
-        e[u][q] = 1.f;
-        if (w[u][q] >= least) e[u][q] = __ldg(noise + at[u] + q);
-      }
-#pragma unroll
-    for (int u = 0; u < runs.value; ++u)
-#pragma unroll
-      for (int q = 0; q < len.value; ++q) {
-        if (!(w[u][q] >= least)) continue;
-        const float sc = __fdividef(w[u][q], e[u][q]);
-        close = close | (w[u][q] < sure) | !(fabsf(sc - bar) > 1e-4f * fmaxf(sc, bar));            // equal infinities and NaN too
-        if (sc > bar) {
-          bar = sc;
-          bar_at = at[u] + q;
-          bar_value = v[u][q];
-        }
-      }
-  });
-  if (close) {
-    each([&](float v, int i) {
-      if (!kept(v, i)) return;
-      const float w = weight(v);
-      if (w >= min_p) race(w, i);
-    });
-  } else if (bar >= 0.f) {
-    race(weight(bar_value), bar_at);
+  if (!raced) {
+    keep_to(cut);
+    auto all = [&](float v, int i, float) { return kept(v, i); };
+    auto ignore = [](float, int, float, float) {};
+    run_race(all, ignore);
+    settle(all);
   }
   win = most(win);
   if (rank == 0 && tid == 0) a.out[b] = index_of(win);
@@ -613,10 +667,11 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
 
 template <typename T>
 int launch_sample(const SampleArgs& a, int B, cudaStream_t st) {
-  // CTAs per row: as many as run at once (two per SM; half a wave more is still faster: 96 rows of 131072 take 190, 125, 117 and 147 us on 1, 2, 4 and 8), none
-  // with less than 4096 logits (a row of 32000: 22.7, 22.5, 20.5 and 18.5 us)
+  // CTAs per row: while all rows' run at once (two per SM) and keep 8192 logits each, twice as many, and of long parts half a wave more. Measured, us on 1, 2, 4, 8
+  // (top-p, but for the 8192): 1 row of 131072: 87, 70, 50, 39; 64 of 32000 bf16: 38, 36, 38, 67; 150 of 50000: 75, 86, 106, 166; 96 of 131072: 168, 131, 108, 149;
+  // 32 of 8192: 15, 19, 19, 25.
   int C = 1;
-  while (C < 8 && a.V > 4096LL * C && (long long)B * C * 2 <= 444) C *= 2;
+  while (C < 8 && a.V > 8192LL * C && ((long long)B * C * 2 <= 256 || (a.V > 60000LL * C && (long long)B * C * 2 <= 444))) C *= 2;
   ELFA_CUDA(allow_shared<sample_kernel<T>>((int)sizeof(SampleShared)));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)B * C);
