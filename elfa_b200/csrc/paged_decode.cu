@@ -425,10 +425,14 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(const __grid_con
   }
 }
 
-constexpr int WHOLE_KEYS = 256, MIN_UNITS = 4, PREFILL_ROWS = 32;
+constexpr int MIN_UNITS = 4;
 
 int decode_grid(int hd) { return 148 * (hd <= 64 ? 2 : 1); }
-bool decode_whole(int max_new, int rep, long long most_keys) { return (long long)max_new * rep <= DROWS && most_keys <= WHOLE_KEYS; }
+// A CTA per item, no line and no join, where an item cannot be long. us, cut against whole: 1 sequence of 500, 16 heads of 64 10.6, 9.7; of 1000 10.6, 13.4; 4 of 500 11.4, 10.4;
+// 4 of 1000 14.8, 13.6; 16 of 500 17.1, 11.0; of 1000 21.4, 15.7; of 2000 34.5, 28.6, but then one long sequence among short ones would hold up the others.
+bool decode_whole(int B, int Hkv, int max_new, int rep, long long most_keys) {
+  return (long long)max_new * rep <= DROWS && (most_keys <= 512 || (most_keys <= 1024 && (long long)B * Hkv >= 64));
+}
 
 template <int HDP>
 int launch_decode(DecodeArgs& a, int page, cudaStream_t st) {
@@ -492,18 +496,20 @@ bool paged_units_fit(const PagedGeom& g, int block) {
   return tiles * blocks * g.Hkv < 4.0e9;
 }
 
-// Which calls go to the tiles of 2 x 128 rows.
-static bool many_rows(int max_new, int rep) { return (long long)max_new * rep > PREFILL_ROWS && rep <= 128; }
+// Which calls go to the tiles of 2 x 128 rows, by the rows of a key head. 16-row tiles read the keys again for every 16 rows, 128-row tiles take as long for one row as for
+// all. us, 16-row tiles against 128-row tiles: 8 sequences of 3000, 16 heads of 128: 16 rows 48, 60; 24 rows 69, 60; 48 rows 94, 61. Heads of 64: 32 rows 40, 51; 48 rows 53, 52.
+// 32 of 2000, 32 heads on 8 of 128: 16 rows 60, 76; 24 rows 99, 77. One of 100000: 16 rows 89, 99; 24 rows 114, 101.
+static bool many_rows(int max_new, int rep, int hd) { return (long long)max_new * rep > (hd > 64 ? 16 : 48) && rep <= 128; }
 
 }  // namespace elfa
 
 using namespace elfa;
 
 // Floats of scratch that elfa_paged_attention wants for a call of these sizes.
-ELFA_API int elfa_paged_attention_scratch(int N, int page, int H, int Hkv, int hd, int max_new) {
-  if (N <= 0 || page <= 0 || Hkv <= 0 || H % Hkv || max_new <= 0) return 0;
-  if (many_rows(max_new, H / Hkv)) return (int)paged_prefill_scratch(hd);
-  if (decode_whole(max_new, H / Hkv, (long long)N * page)) return 0;
+ELFA_API int elfa_paged_attention_scratch(int B, int N, int page, int H, int Hkv, int hd, int max_new) {
+  if (B <= 0 || N <= 0 || page <= 0 || Hkv <= 0 || H % Hkv || max_new <= 0) return 0;
+  if (many_rows(max_new, H / Hkv, hd)) return (int)paged_prefill_scratch(hd);
+  if (decode_whole(B, Hkv, max_new, H / Hkv, (long long)N * page)) return 0;
   return decode_grid(hd) * (2 * DROWS * ((hd <= 64 ? 64 : 128) + 2) + 8);
 }
 
@@ -518,7 +524,7 @@ ELFA_API int elfa_paged_attention(const void* q, long long qs, const void* pages
   ELFA_REQUIRE(qs % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
                "paged_attention: query rows must lie on 16-byte boundaries");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (many_rows(max_new, a.g.rep)) {
+  if (many_rows(max_new, a.g.rep, hd)) {
     ELFA_REQUIRE(scratch && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0, "paged_attention: no scratch, or not 16-byte aligned");
     return paged_prefill(a.g, q, qs, pages, out, scratch, page, scale, st);
   }
@@ -529,7 +535,7 @@ ELFA_API int elfa_paged_attention(const void* q, long long qs, const void* pages
   a.scale = scale;
   a.g.tile_rows = DROWS;
   a.g.by_tile = div_by(DROWS);
-  a.whole = decode_whole(max_new, a.g.rep, (long long)N * page);
+  a.whole = decode_whole(B, Hkv, max_new, a.g.rep, (long long)N * page);
   a.wide = ((long long)max_new * a.g.rep + DROWS - 1) / DROWS > 4;
   a.min_units = MIN_UNITS;
   ELFA_REQUIRE(paged_units_fit(a.g, DBLK), "paged_attention: too much work for one call (2^32 tiles of 16 rows by 32 keys)");

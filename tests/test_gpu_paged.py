@@ -37,6 +37,9 @@ CASES = [
     ([(300, 2500)], 16, 2, 128, 16, 700, 17),
     ([(9, 100)], 40, 1, 64, 16, None, 0),
     ([(2, 300)], 128, 1, 128, 16, None, 0),
+    ([(1, 100), (2, 33)], 200, 1, 64, 16, None, 0),
+    ([(1, 900 + 7 * i) for i in range(20)], 8, 4, 64, 16, None, 0),
+    ([(8, 600)], 2, 1, 128, 32, 33, 5),
 ]
 
 
