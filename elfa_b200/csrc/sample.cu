@@ -339,34 +339,63 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
       u = iu - u + (warp ? wu : 0.0);
       v = iv - v + (warp ? wv : 0.0);
     };
+    // Of tokens (exact) and mass (fp32, its error far below the windows' margins): what lies before this thread and what up to its end, which is where the next one starts.
+    struct Span {
+      unsigned before, upto;
+      float front, back;
+    };
+    auto spans = [&](unsigned n, float mass) {
+      auto scan = [&](auto v) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const auto u = __shfl_up_sync(0xffffffffu, v, o);
+          if (lane >= o) v += u;
+        }
+        return v;
+      };
+      const unsigned in = scan(n);
+      const float im = scan(mass);
+      __syncthreads();
+      if (lane == 31) s.scan[warp] = make_double2(in, im);
+      __syncthreads();
+      const double2 all = lane < SW ? s.scan[lane] : make_double2(0.0, 0.0);
+      const unsigned wn = scan((unsigned)all.x);
+      const float wm = scan((float)all.y);
+      const unsigned n0 = __shfl_sync(0xffffffffu, wn, warp ? warp - 1 : 0), n1 = __shfl_sync(0xffffffffu, wn, warp);
+      const float m0 = __shfl_sync(0xffffffffu, wm, warp ? warp - 1 : 0), m1 = __shfl_sync(0xffffffffu, wm, warp);
+      const unsigned bn = warp ? n0 : 0u;
+      const float bm = warp ? m0 : 0.f;
+      const unsigned pn = __shfl_up_sync(0xffffffffu, in, 1);
+      const float pm = __shfl_up_sync(0xffffffffu, im, 1);
+      return Span{lane ? bn + pn : bn, lane == 31 ? n1 : bn + in, lane ? bm + pm : bm, lane == 31 ? m1 : bm + im};
+    };
     const int bin0 = tid * OWN;
     // The window (first CTA): where the number of tokens reaches `want`, or the mass may. A bin's tokens weigh between exp(-(bin + 1) / 256) and
     // exp(-bin / 256); those of bin `last`, of which not all may count, between nothing and that. `wide` takes the bounds; else the middle of the bin stands for
     // them, with 2^-11 to either side, which holds nearly always and leaves an eighth of the tokens to sort; what the list then holds shows whether it did.
-    auto window_of_count = [&](double want) {
-      unsigned int cnt[OWN];
+    auto window_of_count = [&](unsigned want) {
+      unsigned int cnt[OWN], n = 0;
       load_counts(cnt);
-      double at = 0.0, none = 0.0;
 #pragma unroll
-      for (int j = 0; j < OWN; ++j) at += cnt[j];
-      before_me(at, none);
+      for (int j = 0; j < OWN; ++j) n += cnt[j];
+      unsigned at = spans(n, 0.f).before;
 #pragma unroll
       for (int j = 0; j < OWN; ++j) {
         if (at < want && at + cnt[j] >= want) {
           s.b1 = s.b2 = bin0 + j;
-          s.before = (long long)at;
-          s.upto = (long long)(at + cnt[j]);
+          s.before = at;
+          s.upto = at + cnt[j];
         }
         at += cnt[j];
       }
       __syncthreads();
     };
-    auto window_of_mass = [&](double want, int last, bool wide) {
+    auto window_of_mass = [&](double target, int last, bool wide) {
       unsigned int cnt[OWN];
       load_counts(cnt);
       constexpr float RATIO = 0.99610137f;                 // exp(-1 / 256)
       const float edge = expf(-bin0 / BINS_PER) * (wide ? 1.f : 0.99804878f);          // exp(-1 / 512)
-      const double shrink = wide ? RATIO : 1.0, gap = wide ? 1e-5 : 0x1p-11;           // 1e-5: more than the sums' and the weights' rounding
+      const float shrink = wide ? RATIO : 1.f, gap = wide ? 2e-5f : 0x1p-11f, want = (float)target;       // 2e-5: more than the sums' and the weights' rounding
       float w = edge, sum = 0.f;
       unsigned int n = 0;
 #pragma unroll
@@ -377,27 +406,30 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         }
         w *= RATIO;
       }
-      double front = n, ahead = sum;                       // tokens and mass before this thread's bins
-      before_me(front, ahead);
-      const double up = want * (1 - gap), down = want * (1 + gap);
+      if (tid == 0) {                                      // should rounding hide the line: more than a list holds
+        s.b1 = s.b2 = last;
+        s.before = 0;
+        s.upto = 1LL << 40;
+      }
+      const Span at = spans(n, sum);                       // (with a barrier)
+      const float up = want * (1.f - gap), down = want * (1.f + gap);
       const bool ends_here = bin0 <= last && bin0 + OWN > last;
-      const double behind = (ahead + sum) * (1 + 1e-6);
-      if ((ahead < up && behind >= up) || (ahead * shrink < down && behind * shrink >= down) || ends_here) {
+      if ((at.front < up && at.back >= up) || (at.front * shrink < down && at.back * shrink >= down) || ends_here) {
         w = edge;
-        double high = ahead, count = front;
+        float high = at.front;
+        unsigned count = at.before;
 #pragma unroll
         for (int j = 0; j < OWN; ++j) {
           const int bin = bin0 + j;
           if (bin > last) continue;
-          double next = high + cnt[j] * w;
-          if (j == OWN - 1 || bin == last) next = fmax(next, ahead + sum);   // what the next thread starts from
+          const float next = j == OWN - 1 || bin == last ? fmaxf(high, at.back) : high + cnt[j] * w;
           if (high < up && (next >= up || bin == last)) {
             s.b1 = bin;
-            s.before = (long long)count;
+            s.before = count;
           }
           if (high * shrink < down && (next * shrink >= down || bin == last)) {
             s.b2 = bin;
-            s.upto = (long long)(count + cnt[j]);
+            s.upto = count + cnt[j];
           }
           count += cnt[j];
           high = next;
@@ -421,7 +453,10 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
       const float from = (float)s.b1, to = s.b2 == BINS - 1 ? CUDART_INF_F : (float)(s.b2 + 1);
       auto in = [&](float, int, float y) { return y < from; };
       auto list = [&](float v, int i, float y, float) {
-        if ((y < to || to == CUDART_INF_F) && kept(v, i)) s.list[atomicAdd(&s.fill, 1)] = place(v, i);           // the window's count fits
+        if ((y < to || to == CUDART_INF_F) && kept(v, i)) {
+          const int at = atomicAdd(&s.fill, 1);            // the window's count fits
+          if (at < LIST) s.list[at] = place(v, i);
+        }
       };
       float sum = 0.f;
       if (last) {
@@ -434,7 +469,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         });
       }
       __syncthreads();
-      const int fill = s.fill;
+      const int fill = min(s.fill, LIST);
       const double2 all = total(sum, tid == 0 ? fill : 0);
       if (C > 1) {                                         // behind those of the CTAs before, in the first one
         int at = 0;
@@ -638,7 +673,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
           bool holds = n > 0;
           if (n > 0) {
             const double m = prefix(n, got.x, want);
-            holds = wide || (got.x < want && m >= want);
+            holds = got.x < want && m >= want;
           }
           if (tid < C) peer(&s, tid)->cut = holds ? s.list[s.pos - 1] : 0;
           if (holds) race_list(s.pos);
