@@ -5,11 +5,15 @@
 // per 64 columns. A CTA walks its share of the line of units (paged.cuh) with everything in flight across items: per pair of tiles and block of 128 keys
 //   warp 0      : TMA: queries once per item, keys one block ahead in two stages, values; a box per page
 //   warp 1      : S = Q K^T, block by block, tile 0 then tile 1, into one S buffer: a product is issued when the rows of the one before have been read
-//   warp 3      : O += P V as the rows of P arrive (of its own, so that neither waits for the other's barriers)
+//   warp 3      : O += P V as the rows of P arrive (a warp of its own: one that issued both waited for one tile's barriers while the other's were ready)
 //   warp 2      : clears the value rows behind a sequence's last token before they are multiplied (what lies there may be anything)
-//   warps 4-11  : softmax and sums of tile 0 and tile 1, a thread per row, as in attention_fwd.cu: the whole S row in registers, P to shared memory in
-//                 O in tensor memory, scaled again when a row's maximum grows by more than 2^8
-// Parts of items go to scratch in fp32 and are joined by a second launch. Every wait is bounded.
+//   warps 4-11  : softmax and sums of tile 0 and tile 1, a thread per row: the whole S row in registers, P as packed bf16 in tensor memory, where the product takes
+//                 it from (through shared memory P cost 160 of the 384 KB that a block moves there, 128 bytes a cycle), O in tensor memory
+// Tensor memory: S 128 | P 2 x 64 | O 2 x HDP columns. Parts of items go to scratch in fp32 and are joined by a second launch. Every wait is bounded.
+//
+// 2048 tokens over 16384, 32 heads on 8 of 128: 443 to 520 us (box and power), 1000 to 1160 TFLOP/s; prompts of six users with a window of 1024, 40 heads on 8 of 128:
+// 139 us, 450 TFLOP/s of what is visible. A block takes a pair of tiles 3.3 to 3.6 thousand cycles, of which the tensor cores need 2048 and the exponentials 2048; the
+// softmax warps never wait for a product. An item's end (last product, output, the next item's rows) costs about 9 thousand more, masked blocks half again as long.
 #include "elfa_native.h"
 #include "paged.cuh"
 
