@@ -241,7 +241,7 @@ int elfa_efla_stream_work(const long long* dims, int step_tokens);
 int elfa_efla_stream(const unsigned long long* p, const long long* dims, const float* forget, float eps, int step_tokens, void* stream);
 
 // ---- paged_decode.cu, pages.cu, sample.cu --------------------------------------------------------
-int elfa_paged_attention_scratch(int B, int N, int page, int H, int Hkv, int hd, int max_new);
+int elfa_paged_attention_scratch(int B, int N, int page, int H, int Hkv, int hd, int max_new, int window, int sinks);
 int elfa_paged_attention(const void* q, long long qs, const void* pages, const int* table, const int* q_start, const int* kv_len, void* out,
                          float* scratch, int B, int N, int P, int page, int T, int H, int Hkv, int hd, int max_new, int window, int sinks,
                          float scale, void* stream);

@@ -4,11 +4,12 @@
 // memory: every key and value is read once and meets 16 rows, 16 x 4 operations per element where the tensor cores would take hundreds. So
 // a warp fetches for itself: blocks of 32 keys by TMA into a ring of its own, three blocks deep (12 x 16 KB in flight per SM at 128-wide heads),
 // no barrier between the warps until an item ends, where their four partial results meet in shared memory. What a CTA leaves of an item
-// that others share goes to scratch in fp32; a second small launch joins those (in the order of the CTAs, so one call's result does not depend on timing).
+// that others share goes to scratch in fp32; a second small launch joins those (in the order of the CTAs, so one call's result does not depend on timing). Where items are
+// alike, a cluster of up to eight CTAs takes each instead and joins its parts through distributed shared memory: no line to count, no second launch.
 // The exponent's reference may lag behind the row's maximum by up to 2^8 before sums are scaled again.
 // Probabilities are rounded to bf16 for the second product (relative 2^-8 at most, as the result will be); their sum is taken before that.
 // 48 sequences of up to 8191 tokens, 32 heads on 8 of 128: 867 MB in 165 us, 5.2 TB/s (about 145 us of it at 6 TB/s; the first keys arrive after 4.5 us, the join takes 5).
-// 16 sequences, a window of 4096: 65 MB in 24 us. One sequence of 129 tokens: a 4 us kernel in a call that the host takes 15 us to issue.
+// 16 sequences, a window of 4096: 65 MB in 20.5 us (in clusters of four; as a line of units 24). One sequence of 129 tokens: a 4 us kernel in a call that the host takes 15 us to issue.
 #include "elfa_native.h"
 #include "mma_sync.cuh"
 #include "paged.cuh"
@@ -29,7 +30,7 @@ struct DecodeArgs {
   PagedJoin* notes;                    // [G]
   long long qs;                        // elements from a token's queries to the next one's
   float scale;
-  int wide, whole;                     // a warp per sequence for the prefix; whole: CTA c takes item c, nothing is shared
+  int wide, whole;                     // a warp per sequence for the prefix; whole: that many CTAs (a cluster) take an item, 0: the line of units
   int min_units;
 };
 
@@ -45,6 +46,63 @@ struct DecodeSmem {
 };
 
 __device__ __forceinline__ int decode_ctas(unsigned W, int grid, int min_units) { return (int)min((W + min_units - 1) / min_units, (unsigned)grid); }
+
+// The CTAs of a cluster have an item's parts in shared memory, [16][HDP] and (maximum, sum): row r is joined by CTA r mod their number, in their order.
+template <int HDP>
+__device__ __noinline__ void join_cluster(const DecodeArgs& a, PagedItem it, float* part, float2* stat, bool any) {
+  constexpr int VEC = HDP / 4, SIDE = DWARPS * 32 / VEC;               // threads of a row, rows side by side
+  __shared__ unsigned bad;
+  const PagedGeom& g = a.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = a.whole, rank = (int)cluster_ctarank();
+  const int r0 = it.t * DROWS, rows = min(DROWS, it.s.n * g.rep - r0);
+  if (!any) {                                                          // fewer blocks than CTAs
+    for (int i = threadIdx.x; i < DROWS * HDP; i += DWARPS * 32) part[i] = 0.f;
+    if (threadIdx.x < DROWS) stat[threadIdx.x] = make_float2(-INFINITY, 0.f);
+  }
+  if (threadIdx.x == 0) bad = 0;
+  cluster_sync_all();
+  const int v = threadIdx.x % VEC;
+  const uint32_t part_at = smem_u32(part), stat_at = smem_u32(stat);
+  for (int r = rank + n * (threadIdx.x / VEC); r < rows; r += n * SIDE) {
+    float2 st[8];
+    float M = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < n) {
+        st[c] = ld_cluster_f2(map_to_cta(stat_at + r * 8, c));
+        M = fmaxf(M, st[c].x);
+      }
+    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+    float den = 0.f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < n) {
+        const float4 x = ld_cluster_f4(map_to_cta(part_at + (r * HDP + v * 4) * 4, c));
+        const float w = st[c].x == -INFINITY ? 1.f : fast_exp2(st[c].x - M);           // without a maximum: sums of zero, or a NaN to hand on
+        den += w * st[c].y;
+        num.x += w * x.x; num.y += w * x.y; num.z += w * x.z; num.w += w * x.w;
+      }
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    num.x *= inv; num.y *= inv; num.z *= inv; num.w *= inv;
+    if (v * 4 < g.hd) {
+      const int tok = g.by_rep(r0 + r), head = it.h * g.rep + r0 + r - tok * g.rep;
+      *reinterpret_cast<uint2*>(a.out + ((long long)(it.s.q0 + tok) * g.H + head) * g.hd + v * 4) = make_uint2(pack_bf16(num.x, num.y), pack_bf16(num.z, num.w));
+      if (!(isfinite(num.x) && isfinite(num.y) && isfinite(num.z) && isfinite(num.w))) atomicOr(&bad, 1u << r);
+    }
+  }
+  __syncthreads();
+  for (int r = warp; r < rows; r += DWARPS) {
+    if (!(bad >> r & 1u)) continue;
+    const int tok = g.by_rep(r0 + r), head = it.h * g.rep + r0 + r - tok * g.rep;
+    const long long at = it.s.q0 + tok;
+    float res[HDP / 32];
+    paged_row<HDP>(g, a.q + at * a.qs + head * g.hd, a.pages, it.b, it.h, it.s.kv - it.s.n + tok, a.scale, res);
+#pragma unroll
+    for (int x = 0; x < HDP / 32; ++x)
+      if (lane + 32 * x < g.hd) a.out[(at * g.H + head) * g.hd + lane + 32 * x] = __float2bfloat16(res[x]);
+  }
+  cluster_sync_all();                                                  // nobody's shared memory goes while another reads it
+}
 
 template <int HDP>
 __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ DecodeArgs a) {
@@ -68,14 +126,17 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
   unsigned u_begin, u_end;
   PagedItem first{};
   if (a.whole) {
-    first.b = blockIdx.x / g.Hkv;
-    first.h = blockIdx.x % g.Hkv;
+    const int item = blockIdx.x / a.whole, rank = blockIdx.x - item * a.whole;
+    first.b = item / g.Hkv;
+    first.h = item - first.b * g.Hkv;
     first.t = 0;
     first.s = paged_seq(g, first.b);
     first.tiles = paged_tiles(g, first.s);
     first.span = paged_span<DBLK>(g, first.s, 0);
-    first.u0 = u_begin = 0;
-    u_end = first.tiles ? first.span.n : 0;
+    first.u0 = 0;
+    const unsigned n = first.tiles ? first.span.n : 0;
+    u_begin = n * rank / a.whole;
+    u_end = n * (rank + 1) / a.whole;
     __syncthreads();
   } else {
     const PagedLine line = paged_line(smem + L::LINE, g.B, reinterpret_cast<unsigned*>(smem + L::TOT));
@@ -89,7 +150,7 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
     if (threadIdx.x == 0) paged_join_note(g, a.notes, first, shares, blockIdx.x, u_begin < u_end && u_begin > first.u0);
   }
   pdl_next();
-  if (u_begin >= u_end) return;
+  if (u_begin >= u_end && !(a.whole > 1 && first.tiles)) return;           // a cluster stays together
 
   // ---- the warp's own loads: unit u_begin + warp, then every fourth; the page of the next one is looked up a turn ahead
   PagedItem pi = first;
@@ -306,7 +367,17 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
     __syncthreads();
     if (warp == 0) {
       add(merge + DROWS * HDP);
-      if (u == it.u0 && ue == it.u0 + it.span.n) {
+      if (a.whole > 1) {                                               // for the cluster to read
+#pragma unroll
+        for (int d = 0; d < HDP / 8; ++d) {
+          *reinterpret_cast<float2*>(merge + gr * HDP + d * 8 + qd * 2) = make_float2(o[d][0], o[d][1]);
+          *reinterpret_cast<float2*>(merge + (gr + 8) * HDP + d * 8 + qd * 2) = make_float2(o[d][2], o[d][3]);
+        }
+        if (qd == 0) {
+          stat[gr] = make_float2(M[0], sum[0]);
+          stat[gr + 8] = make_float2(M[1], sum[1]);
+        }
+      } else if (u == it.u0 && ue == it.u0 + it.span.n) {
         unsigned bad = 0;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -355,6 +426,7 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
     u = ue;
     if (u < u_end) paged_next<DBLK>(g, it);
   }
+  if (a.whole > 1) join_cluster<HDP>(a, it, merge, stat, u_begin < u_end);
 }
 
 // Block c - 1 joins the item that CTA c has noted. Rows, and of few rows the parts too, go to groups of HDP / 4 threads with four columns each.
@@ -430,10 +502,16 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(const __grid_con
 constexpr int MIN_UNITS = 4;
 
 int decode_grid(int hd) { return 148 * (hd <= 64 ? 2 : 1); }
-// A CTA per item, no line and no join, where an item cannot be long. us, cut against whole: 1 sequence of 500, 16 heads of 64 10.6, 9.7; of 1000 10.6, 13.4; 4 of 500 11.4, 10.4;
-// 4 of 1000 14.8, 13.6; 16 of 500 17.1, 11.0; of 1000 21.4, 15.7; of 2000 34.5, 28.6, but then one long sequence among short ones would hold up the others.
-bool decode_whole(int B, int Hkv, int max_new, int rep, long long most_keys) {
-  return (long long)max_new * rep <= DROWS && (most_keys <= 512 || (most_keys <= 1024 && (long long)B * Hkv >= 64));
+// CTAs per item (a cluster) where items are alike or cannot be long, 0 for the line of units. us, line against clusters (their size), 16 heads of 64: 1 sequence of 500 10.6, 9.7 (1);
+// of 2000 12.8, 10.8 (8); of 8000 16.7, 16.9 (8); of 32000 34.5, 42.1 (8); 4 of 1000 13.8, 10.8 (4); of 2000 16.7, 13.2 (4); 8 of 2000 21.4, 17.5 (2); 16 of 500 17.1, 11.0 (1); of 1000
+// 21.4, 15.7 (1); of 2000 34.5, 28.6 (1), but then, as among 4 of 8000, one long sequence among short ones would hold up the others.
+int decode_whole(int B, int Hkv, int hd, int max_new, int rep, long long cache, int window, int sinks) {
+  if ((long long)max_new * rep > DROWS) return 0;
+  const long long items = (long long)B * Hkv, seen = (long long)window + max_new + sinks + 2 * DBLK, most = window && seen < cache ? seen : cache;
+  if (most <= 512) return 1;
+  for (int n = 8; n > 1; n /= 2)           // clusters that run at once: one CTA per SM (two of 64-wide heads), and clusters of eight leave some out
+    if (items * n <= (hd <= 64 ? 256 : 128) && most >= 256 * n && most <= 1280 * n && (window || B == 1 || most <= 2048)) return n;
+  return most <= 1024 && items >= 64;
 }
 
 template <int HDP>
@@ -443,8 +521,19 @@ int launch_decode(DecodeArgs& a, int page, cudaStream_t st) {
   if (rc != ELFA_OK) return rc;
   const int smem = DecodeSmem<HDP>::bytes(a.whole ? 0 : a.g.B);
   ELFA_CUDA(allow_shared<paged_decode_kernel<HDP>>(DecodeSmem<HDP>::bytes(PAGED_MAX_SEQS)));
-  const int grid = a.whole ? a.g.B * a.g.Hkv : decode_grid(a.g.hd);
-  paged_decode_kernel<HDP><<<grid, DWARPS * 32, smem, st>>>(tm, a);
+  const int grid = a.whole ? a.g.B * a.g.Hkv * a.whole : decode_grid(a.g.hd);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(DWARPS * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = a.whole;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = a.whole > 1 ? 1 : 0;
+  ELFA_CUDA(cudaLaunchKernelEx(&cfg, paged_decode_kernel<HDP>, tm, a));
   ELFA_CUDA(cudaGetLastError());
   ::elfa::count_launches(1);
   if (a.whole) return ELFA_OK;
@@ -508,10 +597,10 @@ static bool many_rows(int max_new, int rep, int hd) { return (long long)max_new 
 using namespace elfa;
 
 // Floats of scratch that elfa_paged_attention wants for a call of these sizes.
-ELFA_API int elfa_paged_attention_scratch(int B, int N, int page, int H, int Hkv, int hd, int max_new) {
+ELFA_API int elfa_paged_attention_scratch(int B, int N, int page, int H, int Hkv, int hd, int max_new, int window, int sinks) {
   if (B <= 0 || N <= 0 || page <= 0 || Hkv <= 0 || H % Hkv || max_new <= 0) return 0;
   if (many_rows(max_new, H / Hkv, hd)) return (int)paged_prefill_scratch(hd);
-  if (decode_whole(B, Hkv, max_new, H / Hkv, (long long)N * page)) return 0;
+  if (decode_whole(B, Hkv, hd, max_new, H / Hkv, (long long)N * page, window, sinks)) return 0;
   return decode_grid(hd) * (2 * DROWS * ((hd <= 64 ? 64 : 128) + 2) + 8);
 }
 
@@ -537,7 +626,7 @@ ELFA_API int elfa_paged_attention(const void* q, long long qs, const void* pages
   a.scale = scale;
   a.g.tile_rows = DROWS;
   a.g.by_tile = div_by(DROWS);
-  a.whole = decode_whole(B, Hkv, max_new, a.g.rep, (long long)N * page);
+  a.whole = decode_whole(B, Hkv, hd, max_new, a.g.rep, (long long)N * page, a.g.window, a.g.sinks);
   a.wide = ((long long)max_new * a.g.rep + DROWS - 1) / DROWS > 4;
   a.min_units = MIN_UNITS;
   ELFA_REQUIRE(paged_units_fit(a.g, DBLK), "paged_attention: too much work for one call (2^32 tiles of 16 rows by 32 keys)");

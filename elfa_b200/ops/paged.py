@@ -94,8 +94,9 @@ def _rows(t: torch.Tensor, hd: int) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=256)
-def _scratch_floats(B: int, N: int, page: int, H: int, Hkv: int, hd: int, max_new: int) -> int:
-    return lib.raw("elfa_paged_attention_scratch")(B, N, page, H, Hkv, hd, max_new)
+def _scratch_floats(B: int, *sizes: int) -> int:
+    parts = {B} if B <= _MAX_SEQS else {_MAX_SEQS, B % _MAX_SEQS or _MAX_SEQS}
+    return max(lib.raw("elfa_paged_attention_scratch")(b, *sizes) for b in parts)
 
 
 def paged_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
@@ -131,12 +132,13 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q
     q = _rows(q, hd)
     if not (table.is_contiguous() and q_start.is_contiguous() and kv_len.is_contiguous()):
         table, q_start, kv_len = table.contiguous(), q_start.contiguous(), kv_len.contiguous()
-    n = _scratch_floats(B if B <= _MAX_SEQS else 1, N, page, H, Hkv, hd, max_new)       # of a batch in parts the last one may be any size
+    window, sinks = min(window or 0, 1 << 30), min(sinks, 1 << 30)
+    n = _scratch_floats(B, N, page, H, Hkv, hd, max_new, window, sinks)
     scratch = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     pt, pq, pk = table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr()
     for b in range(0, B, _MAX_SEQS):           # q_start counts from the first row of the whole call in every part
         lib.call("elfa_paged_attention", q, q.stride(0), pages, pt + 4 * b * N, pq + 4 * b, pk + 4 * b, out, scratch, min(_MAX_SEQS, B - b), N, P, page, T, H,
-                 Hkv, hd, max_new, min(window or 0, 1 << 30), min(sinks, 1 << 30), scale if scale is not None else hd ** -0.5, stream_ptr(q))
+                 Hkv, hd, max_new, window, sinks, scale if scale is not None else hd ** -0.5, stream_ptr(q))
     return out
 
 

@@ -55,6 +55,49 @@ def test_attention(cuda_device, lens, H, Hkv, hd, page, window, sinks):
     assert close(_run(c, window=window, sinks=sinks), ref, mag)                                          # without a bound of the new tokens
 
 
+LONG_TABLES = [
+    # lens, H, Hkv, hd, page, pages that the table has room for, window, sinks: few rows, and items that several CTAs take together
+    ([(1, 4000)], 16, 2, 64, 16, 250, None, 0),
+    ([(2, 3999)], 16, 2, 128, 64, 63, None, 0),
+    ([(1, 3)], 16, 2, 64, 16, 300, None, 0),
+    ([(3, 40)], 5, 1, 128, 16, 300, None, 0),
+    ([(1, 225)], 4, 1, 8, 32, 200, None, 0),
+    ([(2, 2047), (0, 900), (1, 1), (16, 600)], 2, 2, 80, 128, 16, None, 0),
+    ([(0, 0), (4, 1030), (1, 33), (0, 0), (2, 2)], 4, 1, 64, 16, 100, None, 0),
+    ([(1, 5000), (1, 700), (1, 20), (1, 601)], 8, 2, 128, 16, 400, 600, 4),
+    ([(4, 5000), (3, 3)], 8, 2, 64, 16, 400, 2000, 40),
+    ([(1, 2500)], 6, 6, 96, 256, 10, 1000, 300),
+]
+
+
+@pytest.mark.parametrize("lens,H,Hkv,hd,page,room,window,sinks", LONG_TABLES)
+def test_attention_with_room_in_the_table(cuda_device, lens, H, Hkv, hd, page, room, window, sinks):
+    c = make(lens, H, Hkv, hd, page, seed=room)
+    table = torch.full((len(lens), room), -1, dtype=torch.int32, device=cuda_device)
+    table[:, :c["table"].shape[1]] = c["table"]
+    c["table"] = table
+    new = max(n for n, _ in lens)
+    ref, mag = attend64(c, window, sinks)
+    o = _run(c, max_new=new, window=window, sinks=sinks)
+    assert native.status() == 0 and close(o, ref, mag)
+    assert torch.equal(o, _run(c, max_new=new, window=window, sinks=sinks))
+    # a value that is not finite reaches the rows that see it, and a page that is gone takes its keys with it
+    kv = lens[0][1]
+    if kv > 2 * page:
+        at = kv // 2 if window is None else kv - min(window, kv) // 2 - new
+        bad = {**c, "pages": c["pages"].clone()}
+        bad["pages"][int(table[0, at // page]), 1, 0, at % page] = float("inf")
+        o = _run(bad, max_new=new, window=window, sinks=sinks).view(-1, H, hd)
+        sees = torch.zeros_like(o, dtype=torch.bool)
+        sees[:lens[0][0], :H // Hkv] = True
+        assert not torch.isfinite(o[sees]).any()
+        assert close(o.masked_fill(sees, 0).view(ref.shape), ref.view(o.shape).masked_fill(sees, 0).view(ref.shape), mag)
+        table[0, at // page] = -1
+        ref, mag = attend64(c, window, sinks)
+        assert close(_run(c, max_new=new, window=window, sinks=sinks), ref, mag)
+    assert native.status() == 0
+
+
 def test_scale_and_strides(cuda_device):
     c = make([(3, 400), (1, 90)], 8, 2, 64, 16)
     ref, mag = attend64(c, scale=0.3)
