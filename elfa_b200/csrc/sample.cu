@@ -179,6 +179,20 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     return (unsigned long long)__double_as_longlong(r.x);
   };
 
+  // the sum of u and, in one number, that of n over the CTAs and the largest f
+  auto race_total = [&](double u, int n, float f) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      u += __shfl_xor_sync(0xffffffffu, u, o);
+      f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, o));
+    }
+    return gather(make_double2(u, __hiloint2double(__float_as_int(f), warp == 0 ? n : 0)), [](double2 p, double2 q) {
+      const float top = fmaxf(__int_as_float(__double2hiint(p.y)), __int_as_float(__double2hiint(q.y)));
+      return make_double2(p.x + q.x, __hiloint2double(__float_as_int(top), __double2loint(p.y) + __double2loint(q.y)));
+    });
+  };
+  auto race_top = [](double2 all) { return __int_as_float(__double2hiint(all.y)); };
+
   const int kr = a.top_k ? a.top_k[b] : a.top_k_all, k = kr > 0 && kr < V ? kr : V;
   const float asked = a.temperature ? a.temperature[b] : a.temperature_all, temp = fminf(asked, 1e30f), p = a.top_p ? a.top_p[b] : a.top_p_all,
               min_p = a.min_p ? a.min_p[b] : a.min_p_all;
@@ -217,16 +231,17 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
   };
   auto kept = [&](float v, int i) { return v > last_value || (v == last_value && i <= last_index); };
 
-  // The race of the tokens for which in(value, index, depth) holds; out(value, index, depth, weight) is told of the others. A rough score of every token, the
-  // exact one (settle) of the best of each thread, or of all of its tokens where another one (or the line of min_p) was within 10^-4, more than the rough
-  // scores are off. The variates of a batch are asked for at once.
+  // The race of the tokens for which in(value, index, depth) holds; out(value, index, depth, weight) is told of the others. A rough score of every token; the
+  // exact one (settle) where a thread's best is within 10^-4 of the row's, more than the rough scores are off: of that token, or of all of the thread's where
+  // another one, or one at the line of min_p, is as near (few rows have such a thread). The variates of a batch are asked for at once.
   float bar = -1.f, second = -1.f;         // of this thread's rough scores
+  float maybe = -1.f;                      // the best of those that min_p may keep out
+  float top = -1.f;                        // the best of the row's (those aside)
   int bar_at = 0;
-  bool close = false, raced = false;
+  bool raced = false;
   const float least = fmaxf(min_p, 0.f) * (1.f - 1e-5f), sure = min_p * (1.f + 1e-5f);
   auto run_race = [&](auto&& in, auto&& out) {
-    bar = second = -1.f;
-    close = false;
+    bar = second = maybe = -1.f;
     float sum = 0.f;
     each_batch(std::integral_constant<int, RACE / PER>{}, [&](auto& v, auto& at, auto runs, auto len, int n) {
       if constexpr (len.value > 1) {       // the variates of the next batch on their way to the L2
@@ -261,25 +276,30 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         for (int q = 0; q < len.value; ++q) {
           float inv;
           asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(e[u][q]));
-          const float sc = w[u][q] * inv;  // -1 of what does not race
+          float sc = w[u][q] * inv;        // -1 of what does not race
+          if (min_p > 0.f && w[u][q] < sure) {
+            maybe = fmaxf(maybe, sc);
+            sc = -1.f;
+          }
           if (sc > bar) bar_at = at[u] + q;
           second = fmaxf(second, fminf(sc, bar));
           bar = fmaxf(bar, sc);
-          if (min_p > 0.f) close = close | (w[u][q] >= 0.f && w[u][q] < sure);
         }
     });
-    close = close || (bar >= 0.f && !(second < bar * (1.f - 1e-4f)));
     return sum;                            // the mass of those that raced, and of those that min_p keeps out
   };
   auto settle = [&](auto&& in) {
-    if (close) {
+    const bool plain = top > 1e-30f && top < CUDART_INF_F; // else some may have left the range in which they are that good
+    const float near = plain ? top * (1.f - 1e-4f) : top < 0.f ? 0.f : -2.f;
+    if (bar < near && maybe < near) return;
+    if (plain && maybe < near && second < near) {
+      race(weight(value(x[bar_at])), bar_at);
+    } else {
       each([&](float v, int i) {
         if (!in(v, i, depth(v))) return;
         const float w = weight(v);
         if (w >= min_p) race(w, i);
       });
-    } else if (bar >= 0.f) {
-      race(weight(value(x[bar_at])), bar_at);
     }
   };
 
@@ -343,12 +363,13 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
       u = iu - u + (warp ? wu : 0.0);
       v = iv - v + (warp ? wv : 0.0);
     };
-    // Of tokens (exact) and mass (fp32, its error far below the windows' margins): what lies before this thread and what up to its end, which is where the next one starts.
+    // Of tokens (exact) and mass (fp32, its error far below the windows' margins): what lies before this thread and what up to its end, which is where the next one
+    // starts; and all of sq.
     struct Span {
       unsigned before, upto;
-      float front, back;
+      float front, back, sq;
     };
-    auto spans = [&](unsigned n, float mass) {
+    auto spans = [&](unsigned n, float mass, float sq) {
       auto scan = [&](auto v) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -359,30 +380,36 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
       };
       const unsigned in = scan(n);
       const float im = scan(mass);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
       __syncthreads();
-      if (lane == 31) s.scan[warp] = make_double2(in, im);
+      if (lane == 31) s.scan[warp] = make_double2(__hiloint2double(__float_as_int(im), (int)in), sq);
       __syncthreads();
       const double2 all = lane < SW ? s.scan[lane] : make_double2(0.0, 0.0);
-      const unsigned wn = scan((unsigned)all.x);
-      const float wm = scan((float)all.y);
+      const unsigned wn = scan((unsigned)__double2loint(all.x));
+      const float wm = scan(__int_as_float(__double2hiint(all.x)));
+      sq = (float)all.y;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
       const unsigned n0 = __shfl_sync(0xffffffffu, wn, warp ? warp - 1 : 0), n1 = __shfl_sync(0xffffffffu, wn, warp);
       const float m0 = __shfl_sync(0xffffffffu, wm, warp ? warp - 1 : 0), m1 = __shfl_sync(0xffffffffu, wm, warp);
       const unsigned bn = warp ? n0 : 0u;
       const float bm = warp ? m0 : 0.f;
       const unsigned pn = __shfl_up_sync(0xffffffffu, in, 1);
       const float pm = __shfl_up_sync(0xffffffffu, im, 1);
-      return Span{lane ? bn + pn : bn, lane == 31 ? n1 : bn + in, lane ? bm + pm : bm, lane == 31 ? m1 : bm + im};
+      return Span{lane ? bn + pn : bn, lane == 31 ? n1 : bn + in, lane ? bm + pm : bm, lane == 31 ? m1 : bm + im, sq};
     };
     const int bin0 = tid * OWN;
     // The window (first CTA): where the number of tokens reaches `want`, or the mass may. A bin's tokens weigh between exp(-(bin + 1) / 256) and
     // exp(-bin / 256); those of bin `last`, of which not all may count, between nothing and that. `wide` takes the bounds; else the middle of the bin stands for
-    // them, with 2^-11 to either side, which holds nearly always and leaves an eighth of the tokens to sort; what the list then holds shows whether it did.
+    // them (the largest token's weight is known). Places within a bin are as good as even, so the whole is off by 1 / (256 sqrt 12) of sqrt(sum w^2): four times
+    // that to either side hold nearly always and leave a twentieth of the tokens to sort; what the list then holds shows whether they did.
     auto window_of_count = [&](unsigned want) {
       unsigned int cnt[OWN], n = 0;
       load_counts(cnt);
 #pragma unroll
       for (int j = 0; j < OWN; ++j) n += cnt[j];
-      unsigned at = spans(n, 0.f).before;
+      unsigned at = spans(n, 0.f, 0.f).before;
 #pragma unroll
       for (int j = 0; j < OWN; ++j) {
         if (at < want && at + cnt[j] >= want) {
@@ -399,14 +426,16 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
       load_counts(cnt);
       constexpr float RATIO = 0.99610137f;                 // exp(-1 / 256)
       const float edge = expf(-bin0 / BINS_PER) * (wide ? 1.f : 0.99804878f);          // exp(-1 / 512)
-      const float shrink = wide ? RATIO : 1.f, gap = wide ? 2e-5f : 0x1p-11f, want = (float)target;       // 2e-5: more than the sums' and the weights' rounding
-      float w = edge, sum = 0.f;
+      const float shrink = wide ? RATIO : 1.f, want = (float)target;
+      const float largest = wide || tid ? 0.f : 1.f - edge;
+      float w = edge, sum = largest, sq = largest > 0.f ? -edge * edge : 0.f;
       unsigned int n = 0;
 #pragma unroll
       for (int j = 0; j < OWN; ++j) {
         if (bin0 + j <= last) {
           n += cnt[j];
           sum += cnt[j] * w;
+          sq += cnt[j] * w * w;
         }
         w *= RATIO;
       }
@@ -415,7 +444,9 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         s.before = 0;
         s.upto = 1LL << 40;
       }
-      const Span at = spans(n, sum);                       // (with a barrier)
+      const Span at = spans(n, sum, sq);                   // (with a barrier)
+      // 2e-5: more than the sums' and the weights' rounding
+      const float gap = 2e-5f + (wide ? 0.f : fminf(4.f / (256.f * 3.4641f) * sqrtf(fmaxf(at.sq, 0.f)) / want, 0x1p-9f));
       const float up = want * (1.f - gap), down = want * (1.f + gap);
       const bool ends_here = bin0 <= last && bin0 + OWN > last;
       if ((at.front < up && at.back >= up) || (at.front * shrink < down && at.back * shrink >= down) || ends_here) {
@@ -426,7 +457,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         for (int j = 0; j < OWN; ++j) {
           const int bin = bin0 + j;
           if (bin > last) continue;
-          const float next = j == OWN - 1 || bin == last ? fmaxf(high, at.back) : high + cnt[j] * w;
+          const float next = j == OWN - 1 || bin == last ? fmaxf(high, at.back) : high + cnt[j] * w + (j == 0 ? largest : 0.f);
           if (high < up && (next >= up || bin == last)) {
             s.b1 = bin;
             s.before = count;
@@ -474,10 +505,11 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
       }
       __syncthreads();
       const int fill = min(s.fill, LIST);
-      const double2 all = total(sum, tid == 0 ? fill : 0);
+      const double2 all = race_total(sum, fill, bar);
+      top = race_top(all);
       if (C > 1) {                                         // behind those of the CTAs before, in the first one
         int at = 0;
-        for (int r = 0; r < rank; ++r) at += (int)s.mail[turn ^ 1][r].y;
+        for (int r = 0; r < rank; ++r) at += __double2loint(s.mail[turn ^ 1][r].y);
         unsigned long long* to0 = peer(s.swap, 0);
         for (int i = tid; i < fill && at + i < LIST; i += ST) to0[at + i] = s.list[i];
         cluster_sync_all();
@@ -485,7 +517,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         for (int i = tid; i < fill; i += ST) s.swap[i] = s.list[i];
         __syncthreads();
       }
-      return make_double2(all.x, fmin(all.y, LIST));
+      return make_double2(all.x, min(__double2loint(all.y), LIST));
     };
     // first CTA: all lists to one, in order: a bitonic network, E neighbouring entries per thread in registers, exchanges between warps through shared memory
     auto order = [&](auto per_thread, int m) {
@@ -698,6 +730,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     auto all = [&](float v, int i, float) { return kept(v, i); };
     auto ignore = [](float, int, float, float) {};
     run_race(all, ignore);
+    top = race_top(race_total(0.0, 0, bar));
     settle(all);
   }
   win = most(win);
