@@ -7,7 +7,7 @@
 //
 // Sums are of fp32 weights, joined in fp32 or fp64; what decides between two tokens is fp32. Counts and places are integers, so a result does not depend on the order in
 // which threads come. Bound by latency where rows are few (a dozen meetings of a row's CTAs: one row of 32000, all filters, 20 us) and by the passes' instructions
-// where they are many: 96 rows of 131072, top-p, 104 to 110 us, 45 of them per row and wave: maximum 3, counting 8, window 5, race 13, sort 6, meetings 8.
+// where they are many: 96 rows of 131072, top-p, 75 us, of a CTA's row maximum 13, counting 19, window 8, race 30, sort 5.
 #include <math_constants.h>
 
 #include <type_traits>
@@ -40,7 +40,7 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 constexpr int ST = 512, SW = ST / 32;      // threads of a CTA
 constexpr int BINS = 8192, LIST = 4096;    // bins of width T / 256 below the maximum; tokens that are sorted
 constexpr float BINS_PER = 256.f;
-// Vectors of 16 bytes that a thread asks for at once, tokens of it whose variates it does: what 64 registers hold (twice as many of either cost 7 to 20 %).
+// Vectors of 16 bytes that a thread asks for at once, tokens of the race's batches: what 64 registers hold (twice as many of either cost 7 to 25 %).
 constexpr int EACH = 2, RACE = 8;
 
 // (key, index) as one number: larger is earlier in the order of falling logits, equal ones by index. Never 0.
@@ -69,6 +69,186 @@ struct SampleShared {
 };
 enum { SORT_ALL, SORT_WINDOW, SEARCH };
 
+// A CTA's part of a row: single elements up to a 16-byte boundary (the first CTA's), vectors of 16 bytes, single ones behind the last vector (the last CTA's).
+template <typename T>
+struct Part {
+  static constexpr int PER = 16 / sizeof(T);
+  const T* x;
+  int V, head, vecs, v0, v1;
+  bool front, back;
+
+  __device__ __forceinline__ static float value(T v) {     // of a NaN and -inf the latter
+    if constexpr (std::is_same<T, float>::value) return fmaxf(v, -CUDART_INF_F);
+    else return fmaxf(__bfloat162float(v), -CUDART_INF_F);
+  }
+  __device__ __forceinline__ const uint4* vectors() const { return reinterpret_cast<const uint4*>(x + head); }
+  // f(index) of the single ones
+  template <typename F>
+  __device__ __forceinline__ void singles(F&& f) const {
+    if (front && threadIdx.x < head) f((int)threadIdx.x);
+    const int tail = head + vecs * PER + threadIdx.x;
+    if (back && tail < V) f(tail);
+  }
+  // f(value, index), U vectors asked for at once and a batch ahead
+  template <int U, typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    singles([&](int i) { f(value(x[i]), i); });
+    const uint4* xv = vectors();
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v0 + (int)threadIdx.x + u * ST < v1) w[u] = __ldg(xv + v0 + threadIdx.x + u * ST);
+    for (int v = v0 + threadIdx.x; v < v1; v += U * ST) {
+      uint4 now[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) now[u] = w[u];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (v + (U + u) * ST < v1) w[u] = __ldg(xv + v + (U + u) * ST);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (v + u * ST >= v1) break;
+        const T* e = reinterpret_cast<const T*>(&now[u]);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) f(value(e[k]), head + (v + u * ST) * PER + k);
+      }
+    }
+  }
+};
+
+struct Weights {
+  float mx, temp, per;
+  __device__ __forceinline__ float exact(float v) const { return v == mx ? 1.f : expf((v - mx) / temp); }
+  // y = 256 (mx - v) / T, 0 for the largest whatever it is (inf - inf is a NaN), never falling as v falls; exp(-y / 256) for the sums: 2^-22 of each
+  __device__ __forceinline__ float depth(float v) const { return fmaxf(mx - v, 0.f) * per; }
+  __device__ __forceinline__ static float rough(float y) { return fast_exp2(y * (-1.4426950408889634f / BINS_PER)); }
+};
+
+__device__ __forceinline__ void enter_race(unsigned long long& win, float w, float e, int i) {
+  const float sc = w / e;
+  if (sc >= 0.f) win = max(win, (unsigned long long)__float_as_uint(sc) << 32 | (uint32_t)~i);
+}
+
+// The passes over a row are functions of their own, with all registers for a loop each.
+template <typename T>
+__device__ __noinline__ float part_max(Part<T> p) {
+  float mx = -CUDART_INF_F;
+  p.template each<6>([&](float v, int) { mx = fmaxf(mx, v); });
+  return mx;
+}
+
+// Tokens per bin; -> the mass.
+template <typename T>
+__device__ __noinline__ float part_count(Part<T> p, Weights w, unsigned int* hist) {
+  float sum = 0.f;
+  unsigned int rest = 0;                   // what weighs less than 2^-46, often most of the row, would meet in one word
+  p.template each<EACH>([&](float v, int) {
+    const float y = w.depth(v);
+    if (y >= BINS - 1.f) ++rest;
+    else atomicAdd(&hist[__float_as_uint(__fadd_rd(y, 8388608.f)) - 0x4b000000u], 1u);               // its whole part
+    sum += Weights::rough(y);
+  });
+  if (rest) atomicAdd(&hist[BINS - 1], rest);
+  return sum;
+}
+
+// What a thread has found of the race: the mass of its tokens, the best rough score, that token, the next best; and of the exact ones the best.
+struct Raced {
+  float sum, bar, second;
+  int bar_at;
+  unsigned long long win;
+};
+struct RaceRules {
+  float min_p, from, to;                   // bins in front of which tokens race, and in front of which they are collected
+  float last_value;                        // the last token that is kept so far
+  int last_index;
+  __device__ __forceinline__ bool kept(float v, int i) const { return v > last_value || (v == last_value && i <= last_index); }
+};
+enum { FRONT, KEPT, EVERY };
+// The race of the tokens in front of bin `from`, of those that are kept or of every one: a rough score of each. Tokens at the line of min_p are few: their exact scores are
+// taken at once. Those in the bins behind, few as well, go to the list.
+template <typename T, int WHO>
+__device__ __noinline__ Raced part_race(Part<T> p, Weights ws, const float* noise, RaceRules rules, SampleShared* s) {
+  constexpr int PER = Part<T>::PER, RUNS = RACE / PER;
+  Raced out{0.f, -1.f, -1.f, 0, 0};
+  const float floor_p = fmaxf(rules.min_p, 0.f), least = floor_p * (1.f - 1e-5f), sure = floor_p * (1.f + 1e-5f);
+  const bool rest = rules.to == CUDART_INF_F;
+  auto in = [&](float v, int i, float y) { return WHO == EVERY || (WHO == KEPT ? rules.kept(v, i) : y < rules.from); };
+  auto rare = [&](int i) {
+    const float v = p.value(p.x[i]);
+    if (in(v, i, ws.depth(v))) {
+      const float w = ws.exact(v);
+      if (w >= rules.min_p) enter_race(out.win, w, noise[i], i);
+    } else if (rules.kept(v, i)) {
+      const int at = atomicAdd(&s->fill, 1);               // the window's count fits
+      if (at < LIST) s->list[at] = place(v, i);
+    }
+  };
+  // -> whether it is one of the few
+  auto take = [&](float v, int i, float e) {
+    const float y = ws.depth(v), r = Weights::rough(y);
+    const bool now = in(v, i, y);
+    out.sum += now ? r : 0.f;
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(e));
+    const float sc = now && r >= sure ? r * inv : -1.f;
+    if (sc > out.bar) out.bar_at = i;
+    out.second = fmaxf(out.second, fminf(sc, out.bar));
+    out.bar = fmaxf(out.bar, sc);
+    return now ? r >= least && r < sure : WHO == FRONT && (y < rules.to || rest);
+  };
+  p.singles([&](int i) {
+    if (take(p.value(p.x[i]), i, noise[i])) rare(i);
+  });
+  const uint4* xv = p.vectors();
+  const float* ev = noise + p.head;
+  const bool even = (reinterpret_cast<uintptr_t>(ev) & 15) == 0;
+  uint4 w[RUNS];                           // asked for a batch ahead, with their variates
+  float4 e[RUNS][PER / 4];
+  auto ask = [&](int v) {
+#pragma unroll
+    for (int u = 0; u < RUNS; ++u) {
+      const int at = v + u * ST;
+      if (at >= p.v1) continue;
+      w[u] = __ldg(xv + at);
+#pragma unroll
+      for (int h = 0; h < PER / 4; ++h) {
+        const float* from = ev + (long long)at * PER + 4 * h;
+        e[u][h] = even ? __ldg(reinterpret_cast<const float4*>(from)) : make_float4(__ldg(from), __ldg(from + 1), __ldg(from + 2), __ldg(from + 3));
+      }
+    }
+  };
+  const int start = p.v0 + threadIdx.x;
+  ask(start);
+  for (int v = start; v < p.v1; v += RUNS * ST) {
+    uint4 now[RUNS];
+    float4 en[RUNS][PER / 4];
+#pragma unroll
+    for (int u = 0; u < RUNS; ++u) {
+      now[u] = w[u];
+#pragma unroll
+      for (int h = 0; h < PER / 4; ++h) en[u][h] = e[u][h];
+    }
+    ask(v + RUNS * ST);
+    unsigned few = 0;
+#pragma unroll
+    for (int u = 0; u < RUNS; ++u) {
+      if (v + u * ST >= p.v1) break;
+      const T* el = reinterpret_cast<const T*>(&now[u]);
+      const float* ee = reinterpret_cast<const float*>(en[u]);
+#pragma unroll
+      for (int q = 0; q < PER; ++q)
+        if (take(p.value(el[q]), p.head + (v + u * ST) * PER + q, ee[q])) few |= 1u << (u * PER + q);
+    }
+    while (few) {
+      const int q = __ffs(few) - 1;
+      few &= few - 1;
+      rare(p.head + (v + q / PER * ST) * PER + q % PER);
+    }
+  }
+  return out;
+}
+
 // A row belongs to a cluster of C CTAs: CTA r reads the r-th part of it, in every pass. Passes: the maximum; tokens per bin (and the whole mass); the race over
 // the tokens in front of the few bins that a filter's line runs through, whose tokens the first CTA sorts to find out which of them race too. Where the sorted list
 // holds all that can be kept, it races alone. The row is read again from the L2 in each pass (a row of 131072 fp32 logits is 512 KB). What does not fit the
@@ -91,59 +271,16 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     else __syncthreads();
   };
 
-  // ---- every element of this CTA's part: single ones up to a 16-byte boundary, then vectors
-  constexpr int PER = 16 / sizeof(T);
-  const int head = min(V, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)));
-  const int vecs = (V - head) / PER, v0 = (int)((long long)vecs * rank / C), v1 = (int)((long long)vecs * (rank + 1) / C);
-  auto value = [](T v) {
-    float y;
-    if constexpr (std::is_same<T, float>::value) y = v;
-    else y = __bfloat162float(v);
-    return fmaxf(y, -CUDART_INF_F);        // of a NaN and -inf the latter
-  };
-  // f(values, first indices, std::integral_constants of the number of runs and of a run's length): up to four vectors of 16 bytes at once
-  auto each_batch = [&](auto runs, auto&& f) {
-    constexpr int U = runs.value;
-    auto single = [&](int i) {
-      const float v[1][1] = {{value(x[i])}};
-      const int at[1] = {i};
-      f(v, at, std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}, 1);
-    };
-    if (rank == 0 && tid < head) single(tid);
-    const uint4* xv = reinterpret_cast<const uint4*>(x + head);
-    uint4 w[U];                            // asked for a batch ahead
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v0 + tid + u * ST < v1) w[u] = __ldg(xv + v0 + tid + u * ST);
-    for (int v = v0 + tid; v < v1; v += U * ST) {
-      float y[U][PER];
-      int at[U];
-      const int n = min(U, (v1 - v + ST - 1) / ST);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const T* e = reinterpret_cast<const T*>(&w[u]);
-        at[u] = head + (v + u * ST) * PER;
-#pragma unroll
-        for (int k = 0; k < PER; ++k) y[u][k] = value(e[k]);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (v + (U + u) * ST < v1) w[u] = __ldg(xv + v + (U + u) * ST);
-      f(y, at, std::integral_constant<int, U>{}, std::integral_constant<int, PER>{}, n);
-    }
-    const int tail = head + vecs * PER;
-    if (rank == C - 1 && tail + tid < V) single(tail + tid);
-  };
-  auto each = [&](auto&& f) {
-    each_batch(std::integral_constant<int, EACH>{}, [&](auto& v, auto& at, auto runs, auto len, int n) {
-#pragma unroll
-      for (int u = 0; u < runs.value; ++u) {
-        if (u >= n) break;
-#pragma unroll
-        for (int k = 0; k < len.value; ++k) f(v[u][k], at[u] + k);
-      }
-    });
-  };
+  Part<T> part;
+  part.x = x;
+  part.V = V;
+  part.head = min(V, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)));
+  part.vecs = (V - part.head) / Part<T>::PER;
+  part.v0 = (int)((long long)part.vecs * rank / C);
+  part.v1 = (int)((long long)part.vecs * (rank + 1) / C);
+  part.front = rank == 0;
+  part.back = rank == C - 1;
+  auto each = [&](auto&& f) { part.template each<EACH>(f); };
   // ---- sums and maxima over the row, the same in every thread of the cluster
   int turn = 0;
   auto gather = [&](double2 mine, auto&& join) {
@@ -197,9 +334,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
   const float asked = a.temperature ? a.temperature[b] : a.temperature_all, temp = fminf(asked, 1e30f), p = a.top_p ? a.top_p[b] : a.top_p_all,
               min_p = a.min_p ? a.min_p[b] : a.min_p_all;
   if (C > 1) cluster_sync_all();           // every CTA of the row has started
-  float mx = -CUDART_INF_F;
-  each([&](float v, int) { mx = fmaxf(mx, v); });
-  mx = value_of(most(place(mx, 0)));
+  const float mx = value_of(most(place(part_max<T>(part), 0)));
   if (mx == -CUDART_INF_F || !(asked > 0.f)) {
     unsigned long long first = 0;          // of the largest, the one with the lowest index
     if (mx != -CUDART_INF_F)
@@ -210,96 +345,40 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     if (rank == 0 && tid == 0) a.out[b] = index_of(first);             // -1 of 0
     return;
   }
-  auto weight = [&](float v) { return v == mx ? 1.f : expf((v - mx) / temp); };
-  // y = 256 (mx - v) / T, 0 for the largest whatever it is (inf - inf is a NaN), never falling as v falls; exp(-y / 256) for the sums: 2^-22 of each
-  const float per = fminf(BINS_PER / temp, 1e30f);
-  auto depth = [&](float v) { return fmaxf(mx - v, 0.f) * per; };
-  auto rough = [&](float y) { return fast_exp2(y * (-1.4426950408889634f / BINS_PER)); };
+  const Weights ws{mx, temp, fminf(BINS_PER / temp, 1e30f)};
+  auto weight = [&](float v) { return ws.exact(v); };
+  auto depth = [&](float v) { return ws.depth(v); };
+  auto rough = [&](float y) { return Weights::rough(y); };
   unsigned long long win = 0;
-  auto race = [&](float w, int i) {
-    const float sc = w / noise[i];
-    if (sc >= 0.f) win = max(win, (unsigned long long)__float_as_uint(sc) << 32 | (uint32_t)~i);
-  };
+  auto race = [&](float w, int i) { enter_race(win, w, noise[i], i); };
   // what is kept: cut and all before it in the order
   unsigned long long cut = 0;
-  float last_value = -CUDART_INF_F;
-  int last_index = V;
+  RaceRules rules{min_p, 0.f, 0.f, -CUDART_INF_F, V};
   auto keep_to = [&](unsigned long long c) {
     if (c == 0) return;
-    last_value = value_of(c);
-    last_index = index_of(c);
+    rules.last_value = value_of(c);
+    rules.last_index = index_of(c);
   };
-  auto kept = [&](float v, int i) { return v > last_value || (v == last_value && i <= last_index); };
+  auto kept = [&](float v, int i) { return rules.kept(v, i); };
 
-  // The race of the tokens for which in(value, index, depth) holds; out(value, index, depth, weight) is told of the others. A rough score of every token; the
-  // exact one (settle) where a thread's best is within 10^-4 of the row's, more than the rough scores are off: of that token, or of all of the thread's where
-  // another one, or one at the line of min_p, is as near (few rows have such a thread). The variates of a batch are asked for at once.
-  float bar = -1.f, second = -1.f;         // of this thread's rough scores
-  float maybe = -1.f;                      // the best of those that min_p may keep out
-  float top = -1.f;                        // the best of the row's (those aside)
-  int bar_at = 0;
+  // The exact score where a thread's best is within 10^-4 of the row's, more than the rough scores are off: of that token, or of all of the CTA's where a thread
+  // has another one as near (few rows do).
+  Raced found_by_me{0.f, -1.f, -1.f, 0, 0};
+  float top = -1.f;                        // the best of the row's
   bool raced = false;
-  const float least = fmaxf(min_p, 0.f) * (1.f - 1e-5f), sure = min_p * (1.f + 1e-5f);
-  auto run_race = [&](auto&& in, auto&& out) {
-    bar = second = maybe = -1.f;
-    float sum = 0.f;
-    each_batch(std::integral_constant<int, RACE / PER>{}, [&](auto& v, auto& at, auto runs, auto len, int n) {
-      if constexpr (len.value > 1) {       // the variates of the next batch on their way to the L2
-#pragma unroll
-        for (int u = 0; u < runs.value; ++u) {
-          const int next = at[u] + RACE * ST;
-          if (lane % (32 / PER) == 0 && next < V) asm volatile("prefetch.global.L2 [%0];" ::"l"(noise + next));
-        }
-      }
-      float w[runs.value][len.value], e[runs.value][len.value];
-#pragma unroll
-      for (int u = 0; u < runs.value; ++u)
-#pragma unroll
-        for (int q = 0; q < len.value; ++q) {
-          w[u][q] = -1.f;
-          e[u][q] = 1.f;
-          if (u >= n) continue;
-          const float y = depth(v[u][q]), r = rough(y);
-          if (in(v[u][q], at[u] + q, y)) {
-            sum += r;
-            if (r >= least) {
-              w[u][q] = r;
-              e[u][q] = __ldg(noise + at[u] + q);
-            }
-          } else {
-            out(v[u][q], at[u] + q, y, r);
-          }
-        }
-#pragma unroll
-      for (int u = 0; u < runs.value; ++u)
-#pragma unroll
-        for (int q = 0; q < len.value; ++q) {
-          float inv;
-          asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(e[u][q]));
-          float sc = w[u][q] * inv;        // -1 of what does not race
-          if (min_p > 0.f && w[u][q] < sure) {
-            maybe = fmaxf(maybe, sc);
-            sc = -1.f;
-          }
-          if (sc > bar) bar_at = at[u] + q;
-          second = fmaxf(second, fminf(sc, bar));
-          bar = fmaxf(bar, sc);
-        }
-    });
-    return sum;                            // the mass of those that raced, and of those that min_p keeps out
-  };
-  auto settle = [&](auto&& in) {
+  auto settle = [&](auto&& in) {           // by all threads of a CTA
+    win = max(win, found_by_me.win);
     const bool plain = top > 1e-30f && top < CUDART_INF_F; // else some may have left the range in which they are that good
     const float near = plain ? top * (1.f - 1e-4f) : top < 0.f ? 0.f : -2.f;
-    if (bar < near && maybe < near) return;
-    if (plain && maybe < near && second < near) {
-      race(weight(value(x[bar_at])), bar_at);
-    } else {
+    const bool mine = found_by_me.bar >= near;
+    if (__syncthreads_or(mine && (!plain || found_by_me.second >= near))) {
       each([&](float v, int i) {
         if (!in(v, i, depth(v))) return;
         const float w = weight(v);
         if (w >= min_p) race(w, i);
       });
+    } else if (mine) {
+      race(weight(part.value(x[found_by_me.bar_at])), found_by_me.bar_at);
     }
   };
 
@@ -308,15 +387,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     if (tid == 0) s.fill = 0;
     __syncthreads();
     const bool want_all = p < 1.f && k == V;
-    float sum = 0.f;
-    unsigned int rest = 0;                                 // what weighs less than 2^-46, often most of the row, would meet in one word
-    each([&](float v, int) {
-      const float y = depth(v);
-      if (y >= BINS - 1.f) ++rest;
-      else atomicAdd(&s.hist[__float_as_uint(__fadd_rd(y, 8388608.f)) - 0x4b000000u], 1u);           // its whole part
-      if (want_all) sum += rough(y);
-    });
-    if (rest) atomicAdd(&s.hist[BINS - 1], rest);
+    const float sum = part_count<T>(part, ws, s.hist);
     double mass = 0.0;                                     // of what top-k keeps
     if (want_all) mass = total(sum, 0.0).x;
     else meet();
@@ -364,10 +435,10 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
       v = iv - v + (warp ? wv : 0.0);
     };
     // Of tokens (exact) and mass (fp32, its error far below the windows' margins): what lies before this thread and what up to its end, which is where the next one
-    // starts; and all of sq.
+    // starts; and all of the mass and of sq.
     struct Span {
       unsigned before, upto;
-      float front, back, sq;
+      float front, back, all, sq;
     };
     auto spans = [&](unsigned n, float mass, float sq) {
       auto scan = [&](auto v) {
@@ -397,13 +468,14 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
       const float bm = warp ? m0 : 0.f;
       const unsigned pn = __shfl_up_sync(0xffffffffu, in, 1);
       const float pm = __shfl_up_sync(0xffffffffu, im, 1);
-      return Span{lane ? bn + pn : bn, lane == 31 ? n1 : bn + in, lane ? bm + pm : bm, lane == 31 ? m1 : bm + im, sq};
+      return Span{lane ? bn + pn : bn, lane == 31 ? n1 : bn + in, lane ? bm + pm : bm, lane == 31 ? m1 : bm + im, __shfl_sync(0xffffffffu, wm, SW - 1), sq};
     };
     const int bin0 = tid * OWN;
     // The window (first CTA): where the number of tokens reaches `want`, or the mass may. A bin's tokens weigh between exp(-(bin + 1) / 256) and
     // exp(-bin / 256); those of bin `last`, of which not all may count, between nothing and that. `wide` takes the bounds; else the middle of the bin stands for
-    // them (the largest token's weight is known). Places within a bin are as good as even, so the whole is off by 1 / (256 sqrt 12) of sqrt(sum w^2): four times
-    // that to either side hold nearly always and leave a twentieth of the tokens to sort; what the list then holds shows whether they did.
+    // them (the largest token's weight is known), as shares of their sum where that is the whole. Places within a bin are as good as even, so a sum is off by
+    // 1 / (256 sqrt 12) of sqrt(sum w^2), of bf16 logits, where a bin holds one or two values, of sqrt(sum (n w)^2): four times that to either side hold nearly always
+    // and leave 10 to 500 tokens to sort; what the list then holds shows whether they did.
     auto window_of_count = [&](unsigned want) {
       unsigned int cnt[OWN], n = 0;
       load_counts(cnt);
@@ -426,16 +498,17 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
       load_counts(cnt);
       constexpr float RATIO = 0.99610137f;                 // exp(-1 / 256)
       const float edge = expf(-bin0 / BINS_PER) * (wide ? 1.f : 0.99804878f);          // exp(-1 / 512)
-      const float shrink = wide ? RATIO : 1.f, want = (float)target;
+      constexpr bool FINE = std::is_same<T, float>::value;
+      const float shrink = wide ? RATIO : 1.f;
       const float largest = wide || tid ? 0.f : 1.f - edge;
-      float w = edge, sum = largest, sq = largest > 0.f ? -edge * edge : 0.f;
+      float w = edge, sum = largest, sq = FINE && largest > 0.f ? -edge * edge : 0.f;
       unsigned int n = 0;
 #pragma unroll
       for (int j = 0; j < OWN; ++j) {
         if (bin0 + j <= last) {
           n += cnt[j];
           sum += cnt[j] * w;
-          sq += cnt[j] * w * w;
+          sq += cnt[j] * w * (FINE ? w : cnt[j] * w);
         }
         w *= RATIO;
       }
@@ -445,6 +518,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         s.upto = 1LL << 40;
       }
       const Span at = spans(n, sum, sq);                   // (with a barrier)
+      const float want = !wide && k == V ? p * at.all : (float)target;
       // 2e-5: more than the sums' and the weights' rounding
       const float gap = 2e-5f + (wide ? 0.f : fminf(4.f / (256.f * 3.4641f) * sqrtf(fmaxf(at.sq, 0.f)) / want, 0x1p-9f));
       const float up = want * (1.f - gap), down = want * (1.f + gap);
@@ -485,27 +559,26 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     // The window's tokens (those that are kept so far) to the list; the mass of the ones before it, which race here if this filter is the last one.
     auto before_window = [&](float, int, float y) { return y < s.b1; };
     auto collect = [&](bool last) {
-      const float from = (float)s.b1, to = s.b2 == BINS - 1 ? CUDART_INF_F : (float)(s.b2 + 1);
-      auto in = [&](float, int, float y) { return y < from; };
-      auto list = [&](float v, int i, float y, float) {
-        if ((y < to || to == CUDART_INF_F) && kept(v, i)) {
-          const int at = atomicAdd(&s.fill, 1);            // the window's count fits
-          if (at < LIST) s.list[at] = place(v, i);
-        }
-      };
+      rules.from = (float)s.b1;
+      rules.to = s.b2 == BINS - 1 ? CUDART_INF_F : (float)(s.b2 + 1);
       float sum = 0.f;
       if (last) {
-        sum = run_race(in, list);
+        found_by_me = part_race<T, FRONT>(part, ws, noise, rules, &s);
+        sum = found_by_me.sum;
       } else {
         each([&](float v, int i) {
           const float y = depth(v);
-          if (in(v, i, y)) sum += rough(y);
-          else list(v, i, y, 0.f);
+          if (y < rules.from) {
+            sum += rough(y);
+          } else if ((y < rules.to || rules.to == CUDART_INF_F) && kept(v, i)) {
+            const int at = atomicAdd(&s.fill, 1);          // the window's count fits
+            if (at < LIST) s.list[at] = place(v, i);
+          }
         });
       }
       __syncthreads();
       const int fill = min(s.fill, LIST);
-      const double2 all = race_total(sum, fill, bar);
+      const double2 all = race_total(sum, fill, found_by_me.bar);
       top = race_top(all);
       if (C > 1) {                                         // behind those of the CTAs before, in the first one
         int at = 0;
@@ -693,8 +766,8 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         __syncthreads();
       }
       bool found = false;
-      // bf16 logits of one bin are one or two numbers: its middle says too little of them
-      for (int wide = std::is_same<T, float>::value ? 0 : 1; wide < 2 && !found; ++wide) {
+      // bf16 logits of one bin are one or two numbers: its middle says too little of them, but as shares
+      for (int wide = std::is_same<T, float>::value || k == V ? 0 : 1; wide < 2 && !found; ++wide) {
         if (rank == 0) {
           window_of_mass(want, last, wide);
           if (tid == 0) tell(s.upto - s.before <= LIST ? SORT_WINDOW : SEARCH);
@@ -728,9 +801,8 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
   if (!raced) {
     keep_to(cut);
     auto all = [&](float v, int i, float) { return kept(v, i); };
-    auto ignore = [](float, int, float, float) {};
-    run_race(all, ignore);
-    top = race_top(race_total(0.0, 0, bar));
+    found_by_me = cut ? part_race<T, KEPT>(part, ws, noise, rules, &s) : part_race<T, EVERY>(part, ws, noise, rules, &s);
+    top = race_top(race_total(0.0, 0, found_by_me.bar));
     settle(all);
   }
   win = most(win);
@@ -739,11 +811,10 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
 
 template <typename T>
 int launch_sample(const SampleArgs& a, int B, cudaStream_t st) {
-  // CTAs per row: while all rows' run at once (two per SM) and keep 8192 logits each, twice as many, and of long parts half a wave more. Measured, us on 1, 2, 4, 8
-  // (top-p, but for the 8192): 1 row of 131072: 87, 70, 50, 39; 64 of 32000 bf16: 38, 36, 38, 67; 150 of 50000: 75, 86, 106, 166; 96 of 131072: 168, 131, 108, 149;
-  // 32 of 8192: 15, 19, 19, 25.
+  // CTAs per row: while each has an SM of its own and 8192 logits, twice as many. Measured, us on 1, 2, 4, 8 (top-p, but for the 8192): 1 row of 131072: 65, 49, 38, 32;
+  // 40: 71, 53, 54, 72; 96: 74, 76, 89, 127; 120: 91, 80, 109, 163; 64 of 32000 bf16: 33, 32, 37, 66; 150 of 50000: 58, 73, 94, 153; 32 of 8192: 17, 19, 19, 23.
   int C = 1;
-  while (C < 8 && a.V > 8192LL * C && ((long long)B * C * 2 <= 256 || (a.V > 60000LL * C && (long long)B * C * 2 <= 444))) C *= 2;
+  while (C < 8 && a.V > 8192LL * C && (long long)B * C * 2 <= 148) C *= 2;
   ELFA_CUDA(allow_shared<sample_kernel<T>>((int)sizeof(SampleShared)));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)B * C);

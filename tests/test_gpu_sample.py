@@ -152,3 +152,38 @@ def test_refusals(cuda_device):
         with pytest.raises(ValueError, match="sample"):
             bad()
     assert native.status() == 0
+
+
+@pytest.mark.parametrize("V,dtype", [(1000, torch.float32), (32000, torch.bfloat16), (131072, torch.float32)])
+@pytest.mark.parametrize("p,m", [(1.0, 0.0), (0.9, 0.0), (1.0, 0.02), (0.9, 0.02)])
+def test_scores_that_are_nearly_alike(cuda_device, V, dtype, p, m):
+    """All kept tokens' scores lie within 5e-5 of each other, the winner's 2e-5 in front: more than fp32 is off (exponents up to 12 are off by 2^-20, weights and quotients by
+    2^-22). What the filters leave out has far better ones; tokens about a filter's line are out of the race."""
+    B = 12
+    x, u = _draws(B, V, V, dtype, std=1.2)
+    w = torch.exp(x.double() - x.double().amax(1, keepdim=True))
+    order = torch.sort(w, dim=1, descending=True, stable=True)
+    mass = torch.zeros_like(w).scatter_(1, order.indices, (order.values.cumsum(1) - order.values) / w.sum(1, keepdim=True))       # in front of a token
+    inside, outside = (mass < p - 0.02) & (w >= m * 1.02), (mass > p + 0.02) | (w < m * 0.98)
+    if p == 1.0:
+        inside, outside = w >= m * 1.02, w < m * 0.98
+    score = 1 - 5e-5 * (1 - torch.exp(-u.double()))
+    score[~inside] = 0.5
+    score[outside] = 3.0
+    best = torch.where(inside, torch.rand(B, V, device=cuda_device), -1.0).argmax(1)
+    score[torch.arange(B, device=cuda_device), best] = 1 + 2e-5
+    assert torch.equal(ops.sample(x, (w / score).float(), 1.0, 0, p, m), best)
+    assert native.status() == 0
+
+
+def test_variates_out_of_range(cuda_device):
+    """Scores beyond fp32's largest, below its smallest, and of denormal variates."""
+    x, noise = _draws(4, 40000, 5)
+    for at, e in ((17, 1e-39), (30000, 0.0)):
+        n = noise.clone()
+        n[:, at] = e
+        assert (ops.sample(x, n) == at).all()
+    n = torch.full_like(noise, 3e38)
+    n[:, 123] = 2e38
+    x[:, 123] = x.amax(1)
+    assert (ops.sample(x, n) == 123).all()
