@@ -9,7 +9,7 @@
 // The exponent's reference may lag behind the row's maximum by up to 2^8 before sums are scaled again.
 // Probabilities are rounded to bf16 for the second product (relative 2^-8 at most, as the result will be); their sum is taken before that.
 // 48 sequences of up to 8191 tokens, 32 heads on 8 of 128: 867 MB in 165 us, 5.2 TB/s (about 145 us of it at 6 TB/s; the first keys arrive after 4.5 us, the join takes 5).
-// 16 sequences, a window of 4096: 65 MB in 20.5 us (in clusters of four; as a line of units 24). One sequence of 129 tokens: a 4 us kernel in a call that the host takes 15 us to issue.
+// 16 sequences, a window of 4096: 65 MB in 20.5 us (in clusters of four; as a line of units 24). One sequence of 129 tokens: a 4 us kernel in a call that the host takes 13 us to issue.
 #include "elfa_native.h"
 #include "mma_sync.cuh"
 #include "paged.cuh"

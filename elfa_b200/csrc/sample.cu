@@ -7,7 +7,7 @@
 //
 // Sums are of fp32 weights, joined in fp32 or fp64; what decides between two tokens is fp32. Counts and places are integers, so a result does not depend on the order in
 // which threads come. Bound by latency where rows are few (a dozen meetings of a row's CTAs: one row of 32000, all filters, 20 us) and by the passes' instructions
-// where they are many: 96 rows of 131072, top-p, 75 us, of a CTA's row maximum 13, counting 19, window 8, race 30, sort 5.
+// where they are many: 96 rows of 131072, top-p, 75 us out of the L2 and 84 from memory, of a CTA's row maximum 12, counting 19, window 8, race 30, sort 5.
 #include <math_constants.h>
 
 #include <type_traits>

@@ -121,7 +121,7 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q
     T, H = qs[0], qs[1]
     if dev < 0:
         return paged_attention_ref(q, pages, table, q_start, kv_len, window, sinks, scale)
-    out = torch.empty((T, H * hd), dtype=torch.bfloat16, device=q.device)
+    out = q.new_empty((T, H * hd))
     if T == 0:
         return out
     if B == 0 or N == 0:
@@ -134,11 +134,11 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q
         table, q_start, kv_len = table.contiguous(), q_start.contiguous(), kv_len.contiguous()
     window, sinks = min(window or 0, 1 << 30), min(sinks, 1 << 30)
     n = _scratch_floats(B, N, page, H, Hkv, hd, max_new, window, sinks)
-    scratch = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
-    pt, pq, pk = table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr()
+    scratch = q.new_empty(n, dtype=torch.float32) if n else None
+    pt, pq, pk, ps = table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), scratch.data_ptr() if n else None
     for b in range(0, B, _MAX_SEQS):           # q_start counts from the first row of the whole call in every part
-        lib.call("elfa_paged_attention", q, q.stride(0), pages, pt + 4 * b * N, pq + 4 * b, pk + 4 * b, out, scratch, min(_MAX_SEQS, B - b), N, P, page, T, H,
-                 Hkv, hd, max_new, window, sinks, scale if scale is not None else hd ** -0.5, stream_ptr(q))
+        lib.call_plain("elfa_paged_attention", q.data_ptr(), q.stride(0), pages.data_ptr(), pt + 4 * b * N, pq + 4 * b, pk + 4 * b, out.data_ptr(), ps,
+                       min(_MAX_SEQS, B - b), N, P, page, T, H, Hkv, hd, max_new, window, sinks, scale if scale is not None else hd ** -0.5, stream_ptr(q))
     return out
 
 
@@ -171,7 +171,8 @@ def paged_write(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, table: to
     k, v = _rows(k, hd), _rows(v, hd)
     if not (table.is_contiguous() and q_start.is_contiguous() and kv_len.is_contiguous()):
         table, q_start, kv_len = table.contiguous(), q_start.contiguous(), kv_len.contiguous()
-    lib.call("elfa_paged_write", k, k.stride(0), v, v.stride(0), pages, table, q_start, kv_len, B, N, P, page, T, Hkv, hd, stream_ptr(k))
+    lib.call_plain("elfa_paged_write", k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), pages.data_ptr(), table.data_ptr(), q_start.data_ptr(),
+                   kv_len.data_ptr(), B, N, P, page, T, Hkv, hd, stream_ptr(k))
 
 
 def copy_pages(pages: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> None:
@@ -202,4 +203,4 @@ def copy_pages(pages: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> N
         return
     size = pages.stride(-5) * pages.element_size()
     a, b = array.array("i", src), array.array("i", dst)
-    lib.call("elfa_copy_pages", pages, P * size, size, L, P, a.buffer_info()[0], b.buffer_info()[0], n, stream_ptr(pages))
+    lib.call_plain("elfa_copy_pages", pages.data_ptr(), P * size, size, L, P, a.buffer_info()[0], b.buffer_info()[0], n, stream_ptr(pages))

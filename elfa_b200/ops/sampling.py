@@ -43,12 +43,12 @@ def sample_ref(logits: torch.Tensor, noise: Optional[torch.Tensor], temperature:
     return torch.where(empty, torch.full_like(ids, -1), torch.where((top.squeeze(1) < 0) | greedy.squeeze(1), order[:, 0], ids))
 
 
-def _setting(value: _Setting, name: str, dtype: torch.dtype, logits: torch.Tensor):
+def _setting(value: _Setting, name: str, dtype: torch.dtype, rows: torch.Size, dev: int):
     """(tensor or None, number) of a setting that is one number for all rows or a tensor with one per row."""
     if not isinstance(value, torch.Tensor):
         return None, value
-    if value.shape != logits.shape[:1] or value.get_device() != logits.get_device():
-        raise ValueError(f"sample: {name} must be a number or one per row, [{logits.shape[0]}] on {logits.device}")
+    if value.shape != rows or value.get_device() != dev:
+        raise ValueError(f"sample: {name} must be a number or one per row, {list(rows)} on device {dev} (-1: host)")
     if value.dtype is not dtype or not value.is_contiguous():
         value = value.to(dtype).contiguous()
     return value, 0
@@ -66,29 +66,30 @@ def sample(logits: torch.Tensor, noise: Optional[torch.Tensor], temperature: _Se
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"sample: logits must be [B, V], got {tuple(logits.shape)}")
     B, V = logits.shape
-    dev = logits.get_device()
+    rows, dev = logits.shape[:1], logits.get_device()
     if noise is None:
         if isinstance(temperature, torch.Tensor) or temperature > 0:
             raise ValueError("sample: noise may be left out where temperature is 0 for all rows")
     elif noise.shape != logits.shape or noise.dtype is not torch.float32 or noise.get_device() != dev:
         raise ValueError(f"sample: noise must be fp32 {tuple(logits.shape)} on {logits.device}")
-    t, tn = _setting(temperature, "temperature", torch.float32, logits)
-    k, kn = _setting(top_k, "top_k", torch.int32, logits)
-    p, pn = _setting(top_p, "top_p", torch.float32, logits)
-    m, mn = _setting(min_p, "min_p", torch.float32, logits)
+    t, tn = _setting(temperature, "temperature", torch.float32, rows, dev)
+    k, kn = _setting(top_k, "top_k", torch.int32, rows, dev)
+    p, pn = _setting(top_p, "top_p", torch.float32, rows, dev)
+    m, mn = _setting(min_p, "min_p", torch.float32, rows, dev)
     if B == 0:
         return torch.empty(0, dtype=torch.int64, device=logits.device)
     if dev < 0:
-        rows = [s if s is not None else torch.full((B,), n, dtype=d)
+        each = [s if s is not None else torch.full((B,), n, dtype=d)
                 for s, n, d in ((t, tn, torch.float32), (k, kn, torch.int32), (p, pn, torch.float32), (m, mn, torch.float32))]
-        return sample_ref(logits, noise, *rows)
+        return sample_ref(logits, noise, *each)
     if logits.dtype is not torch.bfloat16 and logits.dtype is not torch.float32:
         logits = logits.float()
     if logits.stride(1) != 1:
         logits = logits.contiguous()
     if noise is not None and noise.stride(1) != 1:
         noise = noise.contiguous()
-    out = torch.empty(B, dtype=torch.int64, device=logits.device)
-    lib.call("elfa_sample", logits, int(logits.dtype == torch.float32), logits.stride(0), noise, noise.stride(0) if noise is not None else 0, t, k, p, m, tn,
-             max(0, min(int(kn), V)), pn, mn, out, B, V, stream_ptr(logits))
+    out = logits.new_empty(B, dtype=torch.int64)
+    pt, pk, pp, pm, pe = (s.data_ptr() if s is not None else None for s in (t, k, p, m, noise))
+    lib.call_plain("elfa_sample", logits.data_ptr(), int(logits.dtype is torch.float32), logits.stride(0), pe, noise.stride(0) if pe else 0, pt, pk, pp, pm, tn,
+                   max(0, min(int(kn), V)), pn, mn, out.data_ptr(), B, V, stream_ptr(logits))
     return out
