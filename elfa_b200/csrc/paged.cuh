@@ -55,9 +55,15 @@ __device__ __forceinline__ int paged_tiles(const PagedGeom& g, const PagedSeq& s
   return g.by_tile(s.n * g.rep + g.tile_rows - 1);
 }
 
+// An item's end (partial results meet, the result is written) takes as long as some blocks: with 16-row tiles it stands in the line as that many empty units in
+// front of the item, or a CTA whose share is many short items would be the last by far. us with 0, 3, 5, 7, 10, 14 of them: 48 sequences to 8191, 32 heads on 8 of
+// 128: 165, 157, 150, 147, 147, 150; 64 to 1500: 91, 69, 58, 56, 52, 52; 16 to 1500, 16 heads of 64: 47, 28, 23, 23, 23, 24.
+template <int BLK>
+constexpr int paged_front = BLK == 32 ? 10 : 0;
+
 // key blocks that the rows of a tile see: i < ns is block i (sinks), later ones are w0 + i - ns. A tile that sees nothing still has one block.
 struct PagedSpan {
-  int ns, w0, n;
+  int ns, w0, n;                           // n: units, with the empty ones in front
   __device__ __forceinline__ int block(int i) const { return i < ns ? i : w0 + i - ns; }
 };
 template <int BLK>
@@ -68,7 +74,7 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedGeom& g, const PagedS
   PagedSpan p;
   p.w0 = lo / BLK;
   p.ns = g.window ? min((min(g.sinks, hi) + BLK - 1) / BLK, p.w0) : 0;
-  p.n = max(p.ns + (hi + BLK - 1) / BLK - p.w0, 1);
+  p.n = max(p.ns + (hi + BLK - 1) / BLK - p.w0, 1) + paged_front<BLK>;
   return p;
 }
 

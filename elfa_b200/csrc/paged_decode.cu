@@ -8,7 +8,7 @@
 // alike, a cluster of up to eight CTAs takes each instead and joins its parts through distributed shared memory: no line to count, no second launch.
 // The exponent's reference may lag behind the row's maximum by up to 2^8 before sums are scaled again.
 // Probabilities are rounded to bf16 for the second product (relative 2^-8 at most, as the result will be); their sum is taken before that.
-// 48 sequences of up to 8191 tokens, 32 heads on 8 of 128: 867 MB in 165 us, 5.2 TB/s (about 145 us of it at 6 TB/s; the first keys arrive after 4.5 us, the join takes 5).
+// 48 sequences of up to 8191 tokens, 32 heads on 8 of 128: 867 MB in 144 to 148 us, 6 TB/s (the first keys arrive after 4.5 us, the join takes 5).
 // 16 sequences, a window of 4096: 65 MB in 20.5 us (in clusters of four; as a line of units 24). One sequence of 129 tokens: a 4 us kernel in a call that the host takes 13 us to issue.
 #include "elfa_native.h"
 #include "mma_sync.cuh"
@@ -108,6 +108,7 @@ template <int HDP>
 __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ DecodeArgs a) {
   using L = DecodeSmem<HDP>;
   constexpr int NSUB = L::NSUB;
+  constexpr unsigned FRONT = paged_front<DBLK>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* merge = reinterpret_cast<float*>(smem + L::MERGE);
@@ -133,8 +134,8 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
     first.s = paged_seq(g, first.b);
     first.tiles = paged_tiles(g, first.s);
     first.span = paged_span<DBLK>(g, first.s, 0);
-    first.u0 = 0;
-    const unsigned n = first.tiles ? first.span.n : 0;
+    first.u0 = 0u - FRONT;                               // no empty units
+    const unsigned n = first.tiles ? first.span.n - FRONT : 0;
     u_begin = n * rank / a.whole;
     u_end = n * (rank + 1) / a.whole;
     __syncthreads();
@@ -160,20 +161,25 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
   uint32_t there = 0;                                    // two bits per ring slot: which half's page is there
   struct Ahead {
     int id, row, h;
+    bool any;
   };
   auto look = [&]() {
-    Ahead n{-1, 0, 0};
-    if (pu < u_end) {
-      while (pu >= pi.u0 + pi.span.n) paged_next<DBLK>(g, pi);
-      const int key = pi.span.block((int)(pu - pi.u0)) * DBLK + box * rows_per_box;
+    Ahead n{-1, 0, 0, false};
+    for (; pu < u_end; pu += DWARPS) {
+      while (pu - pi.u0 >= (unsigned)pi.span.n) paged_next<DBLK>(g, pi);
+      if (pu - pi.u0 < FRONT) continue;
+      const int key = pi.span.block((int)(pu - pi.u0 - FRONT)) * DBLK + box * rows_per_box;
       n.row = key & ((1 << g.page_shift) - 1);
       n.h = pi.h;
+      n.any = true;
       if (box < boxes && key < pi.s.kv) n.id = __ldg(g.table + (long long)pi.b * g.N + (key >> g.page_shift));
+      pu += DWARPS;
+      break;
     }
     return n;
   };
   auto issue = [&](int slot, const Ahead& n) {
-    if (pu >= u_end) return;
+    if (!n.any) return;
     const uint32_t bar = bars + 8 * slot, dst = ring + slot * L::UNIT;
     if (lane == 0) mbar_expect_tx(bar, L::UNIT);
     const bool ok = n.id >= 0 && n.id < g.P;
@@ -185,7 +191,6 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
     const unsigned who = __ballot_sync(0xffffffffu, ok);
     const uint32_t two = (who & 1u) | ((boxes > 1 ? who >> (2 * NSUB) & 1u : who & 1u) << 1);
     there = (there & ~(3u << (2 * slot))) | two << (2 * slot);
-    pu += DWARPS;
   };
   Ahead ahead;
   {
@@ -193,10 +198,8 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
 #pragma unroll
     for (int s = 0; s < DST; ++s) {
       n[s] = look();
-      pu += DWARPS;
     }
     ahead = look();
-    pu -= DST * DWARPS;
 #pragma unroll
     for (int s = 0; s < DST; ++s) issue(s, n[s]);
   }
@@ -209,6 +212,13 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
   for (unsigned u = u_begin; u < u_end;) {
     const unsigned ue = min(u_end, it.u0 + it.span.n);
     const int r0 = it.t * DROWS, rows = min(DROWS, it.s.n * g.rep - r0), pos0 = it.s.kv - it.s.n;
+    if (!a.whole && ue - it.u0 <= FRONT) {                 // a share that ends before the item's first block: a part of nothing, for the join
+      const long long ps = 2LL * blockIdx.x + (u == it.u0);
+      for (int i = threadIdx.x; i < rows * HDP; i += DWARPS * 32) a.part[ps * DROWS * HDP + i] = 0.f;
+      if ((int)threadIdx.x < rows) reinterpret_cast<float2*>(a.stat)[ps * DROWS + threadIdx.x] = make_float2(-INFINITY, 0.f);
+      u = ue;
+      continue;
+    }
     // rows behind the last one repeat it
     const int ra = r0 + min(gr, rows - 1), rb = r0 + min(gr + 8, rows - 1), ta = g.by_rep(ra), tb = g.by_rep(rb);
     const int pa = pos0 + ta, pb = pos0 + tb, pos_min = pos0 + g.by_rep(r0), pos_max = pos0 + g.by_rep(r0 + rows - 1);
@@ -232,7 +242,8 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
 
     const unsigned lead = (warp - (u - u_begin)) & (DWARPS - 1);       // this warp's first unit of the item
     for (unsigned x = u + lead; x < ue; x += DWARPS) {
-      const int key0 = it.span.block((int)(x - it.u0)) * DBLK;
+      if (x - it.u0 < FRONT) continue;
+      const int key0 = it.span.block((int)(x - it.u0 - FRONT)) * DBLK;
       ok = ok && __all_sync(0xffffffffu, mbar_wait(bars + 8 * slot, phase, abort_flag, g.status));
       if (!ok) break;
       const uint32_t kbase = ring + slot * L::UNIT, vbase = kbase + L::HALF;
@@ -377,7 +388,7 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
           stat[gr] = make_float2(M[0], sum[0]);
           stat[gr + 8] = make_float2(M[1], sum[1]);
         }
-      } else if (u == it.u0 && ue == it.u0 + it.span.n) {
+      } else if (a.whole || (u == it.u0 && ue == it.u0 + it.span.n)) {
         unsigned bad = 0;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -499,12 +510,13 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(const __grid_con
   }
 }
 
-constexpr int MIN_UNITS = 4;
+constexpr int MIN_UNITS = 4 + paged_front<DBLK>;                       // no share lies within the empty ones
 
 int decode_grid(int hd) { return 148 * (hd <= 64 ? 2 : 1); }
-// CTAs per item (a cluster) where items are alike or cannot be long, 0 for the line of units. us, line against clusters (their size), 16 heads of 64: 1 sequence of 500 10.6, 9.7 (1);
-// of 2000 12.8, 10.8 (8); of 8000 16.7, 16.9 (8); of 32000 34.5, 42.1 (8); 4 of 1000 13.8, 10.8 (4); of 2000 16.7, 13.2 (4); 8 of 2000 21.4, 17.5 (2); 16 of 500 17.1, 11.0 (1); of 1000
-// 21.4, 15.7 (1); of 2000 34.5, 28.6 (1), but then, as among 4 of 8000, one long sequence among short ones would hold up the others.
+// CTAs per item (a cluster) where items are alike or cannot be long, 0 for the line of units. us, line against clusters (their size), 16 heads of 64: 1 sequence of 500 12.6, 10.6 (1);
+// of 2000 13.6, 10.8 (8); of 8000 15.7, 16.9 (8; the line's two launches and scratch cost the host 7 us more); of 32000 34, 42 (8); 4 of 1000 14.9, 10.8 (4); of 2000 15.3, 13.8 (4);
+// 8 of 2000 21, 18 (2); 16 of 500 17.1, 11.4 (1); of 1000 21.6, 17.1 (1); of 2000 35, 29 (1), but then, as among 4 of 8000, one long sequence among short ones would hold up
+// the others.
 int decode_whole(int B, int Hkv, int hd, int max_new, int rep, long long cache, int window, int sinks) {
   if ((long long)max_new * rep > DROWS) return 0;
   const long long items = (long long)B * Hkv, seen = (long long)window + max_new + sinks + 2 * DBLK, most = window && seen < cache ? seen : cache;
@@ -583,7 +595,7 @@ int paged_prefill(PagedGeom g, const void* q, long long qs, const void* pages, v
 
 // Units are counted in 32 bits.
 bool paged_units_fit(const PagedGeom& g, int block) {
-  const double tiles = (double)g.T * g.rep / g.tile_rows + g.B, blocks = ((double)g.N * (1 << g.page_shift)) / block + 2;
+  const double tiles = (double)g.T * g.rep / g.tile_rows + g.B, blocks = ((double)g.N * (1 << g.page_shift)) / block + 2 + paged_front<32>;
   return tiles * blocks * g.Hkv < 4.0e9;
 }
 
