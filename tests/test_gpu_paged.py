@@ -98,6 +98,19 @@ def test_attention_with_room_in_the_table(cuda_device, lens, H, Hkv, hd, page, r
     assert native.status() == 0
 
 
+@pytest.mark.parametrize("hd,Hkv", [(64, 3), (128, 2)])
+@pytest.mark.parametrize("B", [3, 17, 33, 70])
+def test_shares_that_end_anywhere(cuda_device, B, hd, Hkv):
+    """Few long sequences among many short ones: the work is cut into equal shares wherever that falls."""
+    for step in range(5):
+        lens = [(1 + (b + step) % 2, 2 + (b * 37 + step * 11) % 70 if b % 9 else 700 + 331 * step + 17 * b) for b in range(B)]
+        c = make(lens, 2 * Hkv, Hkv, hd, 16, seed=B + step)
+        ref, mag = attend64(c)
+        o = _run(c, max_new=2)
+        assert close(o, ref, mag) and torch.equal(o, _run(c, max_new=2))
+    assert native.status() == 0
+
+
 def test_scale_and_strides(cuda_device):
     c = make([(3, 400), (1, 90)], 8, 2, 64, 16)
     ref, mag = attend64(c, scale=0.3)
