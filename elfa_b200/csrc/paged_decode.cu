@@ -600,8 +600,9 @@ bool paged_units_fit(const PagedGeom& g, int block) {
 }
 
 // Which calls go to the tiles of 2 x 128 rows, by the rows of a key head. 16-row tiles read the keys again for every 16 rows, 128-row tiles take as long for one row as for
-// all. us, 16-row tiles against 128-row tiles: 8 sequences of 3000, 16 heads of 128: 16 rows 48, 60; 24 rows 69, 60; 48 rows 94, 61. Heads of 64: 32 rows 40, 51; 48 rows 53, 52.
-// 32 of 2000, 32 heads on 8 of 128: 16 rows 60, 76; 24 rows 99, 77. One of 100000: 16 rows 89, 99; 24 rows 114, 101.
+// all. us, 16-row tiles against 128-row tiles: 8 sequences of 3000, 16 heads of 128: 16 rows 49, 60; 24 rows 73, 60; 48 rows 97, 61. Heads of 64: 32 rows 45, 51; 48 rows 55, 51.
+// 32 of 2000, 32 heads on 8 of 128: 16 rows 59, 76; 24 rows 97, 78. One of 30000: 16 rows 42, 49; 24 rows 50, 50; 48 rows 67, 51. Where the bound is far above what most
+// sequences have (up to 32 rows, half of that on average) 16-row tiles would be the faster ones, 50 against 57 us; the host knows the bound only.
 static bool many_rows(int max_new, int rep, int hd) { return (long long)max_new * rep > (hd > 64 ? 16 : 48) && rep <= 128; }
 
 }  // namespace elfa
