@@ -376,6 +376,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
             if (c == 0 && !landed) {                       // P is still the operand of the product before
               ok = __all_sync(0xffffffffu, mbar_wait(bar(PB_OFULL + t), (oc - 1) & 1, abort_flag, g.status));
               landed = true;
+              tc_fence_after();
             }
             if (ok) tmem_st16(TM_P[t] + lane_addr + c * 16, w);
           }
