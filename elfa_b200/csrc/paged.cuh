@@ -41,7 +41,8 @@ struct PagedSeq {
   int q0, n, kv;                           // first new token, new tokens, tokens with them
 };
 
-__device__ __forceinline__ PagedSeq paged_seq(const PagedGeom& g, int b) {
+// in_order: whether the sequence's rows are a piece of the call's. Where those of all sequences are, no row has two sequences (each starts where the one before ends).
+__device__ __forceinline__ PagedSeq paged_seq(const PagedGeom& g, int b, bool* in_order = nullptr) {
   const int a = g.q_start[b], e = g.q_start[b + 1], kv = g.kv_len[b];
   const long long most = (long long)g.N << g.page_shift;
   PagedSeq s;
@@ -49,6 +50,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedGeom& g, int b) {
   s.n = min(max(e, s.q0), g.T) - s.q0;
   s.kv = (int)min((long long)max(kv, 0), min(most, 0x7fffff00LL));
   if (s.q0 != a || s.q0 + s.n != e || s.kv != kv || s.n > s.kv || s.n > g.max_new) atomicOr(g.status, (unsigned)ELFA_ST_BAD_PAGE);
+  if (in_order) *in_order = s.q0 == a && s.q0 + s.n == e;
   return s;
 }
 __device__ __forceinline__ int paged_tiles(const PagedGeom& g, const PagedSeq& s) {
@@ -98,14 +100,18 @@ __device__ __forceinline__ PagedLine paged_line(void* at, int B, unsigned* warp_
   unsigned* p = static_cast<unsigned*>(at);
   return {p, reinterpret_cast<PagedSeq*>(p + B + 1), warp_tot};
 }
-// By all threads of the block (ends with a barrier). wide: a warp per sequence (many tiles each).
+// By all threads of the block (ends with a barrier); returns W. Rows that several sequences claim would make more units than the host has allowed for (more than 32
+// bits hold): such a call has no units, and the status word says why. wide: a warp per sequence (many tiles each).
 template <int BLK, int THREADS>
-__device__ __forceinline__ void paged_prefix(const PagedGeom& g, const PagedLine& line, bool wide) {
+__device__ __forceinline__ unsigned paged_prefix(const PagedGeom& g, const PagedLine& line, bool wide) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int WARPS = THREADS / 32;
+  bool in_order = true;
   if (wide) {
     for (int b = warp; b < g.B; b += WARPS) {
-      const PagedSeq s = paged_seq(g, b);
+      bool here;
+      const PagedSeq s = paged_seq(g, b, &here);
+      in_order = in_order && here;
       const unsigned u = __reduce_add_sync(0xffffffffu, paged_units<BLK>(g, s, lane, 32));
       if (lane == 0) {
         line.prefix[b + 1] = u;
@@ -122,7 +128,9 @@ __device__ __forceinline__ void paged_prefix(const PagedGeom& g, const PagedLine
       if (wide) {
         u = line.prefix[b + 1];
       } else {
-        const PagedSeq s = paged_seq(g, b);
+        bool here;
+        const PagedSeq s = paged_seq(g, b, &here);
+        in_order = in_order && here;
         line.seqs[b] = s;
         u = paged_units<BLK>(g, s, 0, 1);
       }
@@ -147,7 +155,7 @@ __device__ __forceinline__ void paged_prefix(const PagedGeom& g, const PagedLine
     if (b < g.B) line.prefix[b + 1] = u;
   }
   if (threadIdx.x == 0) line.prefix[0] = 0;
-  __syncthreads();
+  return __syncthreads_and(in_order) ? line.prefix[g.B] : 0;
 }
 
 struct PagedItem {

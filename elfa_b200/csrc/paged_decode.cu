@@ -141,8 +141,7 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
     __syncthreads();
   } else {
     const PagedLine line = paged_line(smem + L::LINE, g.B, reinterpret_cast<unsigned*>(smem + L::TOT));
-    paged_prefix<DBLK, DWARPS * 32>(g, line, a.wide);
-    const unsigned W = line.prefix[g.B];
+    const unsigned W = paged_prefix<DBLK, DWARPS * 32>(g, line, a.wide);
     const int G = decode_ctas(W, gridDim.x, a.min_units);
     const PagedShares shares(W, G);
     u_begin = (int)blockIdx.x < G ? shares.first(blockIdx.x) : 0;

@@ -108,8 +108,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
       asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sbase + L::Q + s * PSUB + i * 16), "r"(0) : "memory");
   fence_proxy_async();
   const PagedLine line = paged_line(smem + L::OUT, g.B, tmem_holder + 4);
-  paged_prefix<PBLK, PTHREADS>(g, line, true);
-  const unsigned W = line.prefix[g.B];
+  const unsigned W = paged_prefix<PBLK, PTHREADS>(g, line, true);
   const int G = (int)min(W, gridDim.x);
   const PagedShares shares(W, G);
   const unsigned u_begin = (int)blockIdx.x < G ? shares.first(blockIdx.x) : 0, u_end = (int)blockIdx.x < G ? shares.first(blockIdx.x + 1) : 0;

@@ -27,3 +27,36 @@ def test_blocks_that_follow_each_other(cuda_device, hd, step):
     outs = [_run(c, max_new=140) for _ in range(8)]
     assert close(outs[0], ref, mag) and all(torch.equal(o, outs[0]) for o in outs)
     assert native.status() == 0
+
+
+@pytest.mark.parametrize("starts", [[0, 3, 0, 3], [0, 6, 2, 8], [0, 9, 3, 8], [-4, 2, 3, 8], [5, 2, 3, 8]])
+@pytest.mark.parametrize("new,H", [(3, 2), (3, 64), (70, 8)])
+def test_rows_that_several_sequences_claim(cuda_device, starts, new, H):
+    """Few rows per sequence and many: recorded, and nothing outside is touched."""
+    c = make([(new, 300), (new, 90), (new, 200)], H, 2, 64, 16)
+    scale = c["q"].shape[0] // 8
+    c["q_start"] = torch.tensor([x * scale for x in starts], dtype=torch.int32, device=cuda_device)
+    before = c["pages"].clone()
+    for _ in range(2):
+        _run(c)
+        assert native.status() == native.ST_BAD_PAGE
+    assert torch.equal(c["pages"].view(torch.int16), before.view(torch.int16))
+
+
+def test_more_claimed_rows_than_32_bits_of_units(cuda_device):
+    """Every second of 1024 sequences claims all rows. Their units are 3 x 2^32 and 512 (256-row tiles, blocks of 128 keys): counted in 32 bits they would stand in a line
+    that ends inside the first item, whose parts would be looked for behind the scratch."""
+    T, H, Hkv, kv, other = 8192, 32, 8, 3149888, 3084416
+
+    def units(n):
+        return Hkv * sum(-(-(n - T + (t + 1) * 64) // 128) for t in range(T // 64))
+    assert 511 * units(kv) + units(other) == 3 * 2 ** 32 + 512
+    q = torch.zeros(T, H, 64, dtype=torch.bfloat16, device=cuda_device)
+    pages = torch.zeros(1, 2, Hkv, 256, 64, dtype=torch.bfloat16, device=cuda_device)
+    table = torch.zeros(1024, -(-kv // 256), dtype=torch.int32, device=cuda_device)
+    start = torch.zeros(1025, dtype=torch.int32, device=cuda_device)
+    start[1::2] = T
+    lens = torch.full((1024,), kv, dtype=torch.int32, device=cuda_device)
+    lens[0] = other
+    assert ops.paged_attention(q, pages, table, start, lens).shape == (T, H * 64)
+    assert native.status() == native.ST_BAD_PAGE
