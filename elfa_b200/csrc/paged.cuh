@@ -13,7 +13,7 @@
 
 namespace elfa {
 
-constexpr int PAGED_MAX_SEQS = 1024;       // per launch; the Python side cuts larger batches
+constexpr int PAGED_MAX_SEQS = 1024;       // of a launch of the attention, whose CTAs keep all sequences in shared memory; the Python side cuts larger batches
 
 // x / d for 0 <= x < 2^31 and a d that the host knows: with 2^s the power of two from d on and m = floor(2^32 (2^s - d) / d) + 1, (mulhi(x, m) + x) >> s
 // (the round-up method for invariant divisors). A division costs some 40 instructions, and the walk over items is made of them.

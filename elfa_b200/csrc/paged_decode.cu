@@ -565,11 +565,11 @@ int make_paged_tmap(CUtensorMap* tm, const void* pages, long long P, int Hkv, in
   return make_tmap_nd_bf16(tm, pages, 3, dims, strides, box);
 }
 
-// Checks that both forms of the attention share, and the geometry.
+// Checks that both forms of the attention and the write share, and the geometry.
 int paged_geom(PagedGeom* g, const void* pages, const int* table, const int* q_start, const int* kv_len, int B, int N, int P, int page, int T, int H,
                int Hkv, int hd, int max_new, int window, int sinks) {
   ELFA_REQUIRE(pages && table && q_start && kv_len, "paged: null pointer");
-  ELFA_REQUIRE(B > 0 && B <= PAGED_MAX_SEQS && N > 0 && P > 0 && T > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && max_new > 0, "paged: bad sizes");
+  ELFA_REQUIRE(B > 0 && N > 0 && P > 0 && T > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && max_new > 0, "paged: bad sizes");
   ELFA_REQUIRE(page >= 16 && page <= 256 && (page & (page - 1)) == 0, "paged: tokens per page must be 16, 32, 64, 128 or 256");
   ELFA_REQUIRE(hd >= 8 && hd <= 128 && hd % 8 == 0, "paged: head dimension must be a multiple of 8 up to 128");
   ELFA_REQUIRE((long long)P * 2 * Hkv < 0x7fffffffLL && (long long)N * page < 0x7fffff00LL, "paged: too many pages");
@@ -624,6 +624,7 @@ ELFA_API int elfa_paged_attention(const void* q, long long qs, const void* pages
   const int rc = paged_geom(&a.g, pages, table, q_start, kv_len, B, N, P, page, T, H, Hkv, hd, max_new, window, sinks);
   if (rc != ELFA_OK) return rc;
   ELFA_REQUIRE(q && out, "paged_attention: null pointer");
+  ELFA_REQUIRE(B <= PAGED_MAX_SEQS, "paged_attention: too many sequences for one launch");
   ELFA_REQUIRE(qs % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
                "paged_attention: query rows must lie on 16-byte boundaries");
   cudaStream_t st = static_cast<cudaStream_t>(stream);

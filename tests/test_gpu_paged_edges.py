@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from elfa_b200 import native, ops
+from elfa_b200.runtime.paged_cache import PagedCache
 
 from paged_cases import attend64, close, make
 
@@ -60,3 +61,34 @@ def test_more_claimed_rows_than_32_bits_of_units(cuda_device):
     lens[0] = other
     assert ops.paged_attention(q, pages, table, start, lens).shape == (T, H * 64)
     assert native.status() == native.ST_BAD_PAGE
+
+
+def test_writing_for_more_sequences_than_a_launch_of_the_attention_takes(cuda_device):
+    lens = [(1 + i % 3 if i % 7 else 0, 3 + i % 50) for i in range(2500)]
+    c = make(lens, 4, 2, 32, 16)
+    want = c["pages"].clone()
+    seq = torch.tensor([b for b, (n, _) in enumerate(lens) for _ in range(n)], device=cuda_device)
+    pos = torch.tensor([p for n, kv in lens for p in range(kv - n, kv)], device=cuda_device)
+    ids = c["table"][seq, pos // 16].long()
+    want[ids, 0, :, pos % 16], want[ids, 1, :, pos % 16] = c["k"], c["v"]
+    ops.paged_write(c["k"], c["v"], c["pages"], c["table"], c["q_start"], c["kv_len"])
+    assert native.status() == 0 and torch.equal(c["pages"].view(torch.int16), want.view(torch.int16))
+
+
+def test_a_step_of_many_sequences(cuda_device):
+    """A prompt, 1100 forks of it, and a step of all of them: copied pages, written tokens and attention."""
+    cache = PagedCache(1, 1300, 16, 1, 64, device=cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(0)
+    root, q, k, v = cache.add(), *(torch.randn(20 + 1100, h, 64, generator=g, device=cuda_device).bfloat16() for h in (2, 1, 1))
+    batch = cache.append([root], [20])
+    cache.write(0, k[:20], v[:20], batch)
+    seqs = [root] + cache.fork(root, 1099)
+    batch = cache.append(seqs, [1] * 1100)
+    cache.write(0, k[20:], v[20:], batch)
+    o = cache.attend(0, q[20:], batch).view(1100, 2, 64).double()
+    s = torch.cat([torch.einsum("nhd,kd->nhk", q[20:].double(), k[:20, 0].double()), torch.einsum("nhd,nd->nh", q[20:].double(), k[20:, 0].double())[..., None]], 2) / 8
+    p = torch.softmax(s, -1)
+
+    def mix(vals):
+        return torch.einsum("nhk,kd->nhd", p[..., :20], vals[:20, 0]) + p[..., 20:] * vals[20:, 0][:, None]
+    assert native.status() == 0 and close(o, mix(v.double()), mix(v.double().abs()))
