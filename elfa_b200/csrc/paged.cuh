@@ -13,7 +13,7 @@
 
 namespace elfa {
 
-constexpr int PAGED_MAX_SEQS = 1024;       // of a launch of the attention, whose CTAs keep all sequences in shared memory; the Python side cuts larger batches
+constexpr int PAGED_MAX_SEQS = 1024;       // of a launch of the attention, whose CTAs keep all sequences in shared memory; larger batches are cut into launches
 
 // x / d for 0 <= x < 2^31 and a d that the host knows: with 2^s the power of two from d on and m = floor(2^32 (2^s - d) / d) + 1, (mulhi(x, m) + x) >> s
 // (the round-up method for invariant divisors). A division costs some 40 instructions, and the walk over items is made of them.
@@ -34,6 +34,7 @@ struct PagedGeom {
   int window, sinks;                       // window 0: none
   int tile_rows;                           // query rows of a tile
   DivBy by_rep, by_tile;                   // / rep, / tile_rows
+  int ends;                                // 1: this launch has the call's first sequence, which begins at row 0; 2: its last, which ends at row T
   unsigned int* status;
 };
 
@@ -49,9 +50,20 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedGeom& g, int b, bool* i
   s.q0 = min(max(a, 0), g.T);
   s.n = min(max(e, s.q0), g.T) - s.q0;
   s.kv = (int)min((long long)max(kv, 0), min(most, 0x7fffff00LL));
-  if (s.q0 != a || s.q0 + s.n != e || s.kv != kv || s.n > s.kv || s.n > g.max_new) atomicOr(g.status, (unsigned)ELFA_ST_BAD_PAGE);
+  if (s.q0 != a || s.q0 + s.n != e || s.kv != kv || s.n > s.kv || s.n > g.max_new || (b == 0 && (g.ends & 1) && a != 0) || (b == g.B - 1 && (g.ends & 2) && e != g.T))
+    atomicOr(g.status, (unsigned)ELFA_ST_BAD_PAGE);
   if (in_order) *in_order = s.q0 == a && s.q0 + s.n == e;
   return s;
+}
+// Rows that no sequence has give zeros: those in front of the launch's first sequence and behind its last one, by all threads of one block.
+__device__ __forceinline__ void paged_zero_rows(const PagedGeom& g, __nv_bfloat16* out, int from, int to) {
+  uint4* p = reinterpret_cast<uint4*>(out);
+  const long long row = (long long)g.H * g.hd / 8;
+  for (long long i = from * row + threadIdx.x; i < to * row; i += blockDim.x) p[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+__device__ __forceinline__ void paged_rest(const PagedGeom& g, __nv_bfloat16* out, const PagedSeq& first, const PagedSeq& last) {
+  if (g.ends & 1) paged_zero_rows(g, out, 0, first.q0);
+  if (g.ends & 2) paged_zero_rows(g, out, last.q0 + last.n, g.T);
 }
 __device__ __forceinline__ int paged_tiles(const PagedGeom& g, const PagedSeq& s) {
   return g.by_tile(s.n * g.rep + g.tile_rows - 1);

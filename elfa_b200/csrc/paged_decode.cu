@@ -138,10 +138,15 @@ __global__ void __launch_bounds__(DWARPS * 32) paged_decode_kernel(const __grid_
     const unsigned n = first.tiles ? first.span.n - FRONT : 0;
     u_begin = n * rank / a.whole;
     u_end = n * (rank + 1) / a.whole;
+    if (first.h == 0 && rank == 0) {
+      if (first.b == 0 && (g.ends & 1)) paged_zero_rows(g, a.out, 0, first.s.q0);
+      if (first.b == g.B - 1 && (g.ends & 2)) paged_zero_rows(g, a.out, first.s.q0 + first.s.n, g.T);
+    }
     __syncthreads();
   } else {
     const PagedLine line = paged_line(smem + L::LINE, g.B, reinterpret_cast<unsigned*>(smem + L::TOT));
     const unsigned W = paged_prefix<DBLK, DWARPS * 32>(g, line, a.wide);
+    if (blockIdx.x == 0) paged_rest(g, a.out, line.seqs[0], line.seqs[g.B - 1]);
     const int G = decode_ctas(W, gridDim.x, a.min_units);
     const PagedShares shares(W, G);
     u_begin = (int)blockIdx.x < G ? shares.first(blockIdx.x) : 0;
@@ -585,6 +590,7 @@ int paged_geom(PagedGeom* g, const void* pages, const int* table, const int* q_s
   g->by_rep = div_by((unsigned)g->rep);
   g->window = window > (1 << 30) ? 0 : window;
   g->sinks = sinks > (1 << 30) ? 1 << 30 : sinks;
+  g->ends = 3;
   return ELFA_OK;
 }
 
@@ -612,26 +618,22 @@ using namespace elfa;
 ELFA_API int elfa_paged_attention_scratch(int B, int N, int page, int H, int Hkv, int hd, int max_new, int window, int sinks) {
   if (B <= 0 || N <= 0 || page <= 0 || Hkv <= 0 || H % Hkv || max_new <= 0) return 0;
   if (many_rows(max_new, H / Hkv, hd)) return (int)paged_prefill_scratch(hd);
-  if (decode_whole(B, Hkv, hd, max_new, H / Hkv, (long long)N * page, window, sinks)) return 0;
+  const int full = B < PAGED_MAX_SEQS ? B : PAGED_MAX_SEQS, rest = B % PAGED_MAX_SEQS;      // sequences of the launches
+  const long long cache = (long long)N * page;
+  if (decode_whole(full, Hkv, hd, max_new, H / Hkv, cache, window, sinks) && (!rest || decode_whole(rest, Hkv, hd, max_new, H / Hkv, cache, window, sinks))) return 0;
   return decode_grid(hd) * (2 * DROWS * ((hd <= 64 ? 64 : 128) + 2) + 8);
 }
 
-// q: rows [T] of H heads, `qs` elements apart, heads packed, 16-byte aligned; out: [T, H * hd] contiguous. max_new: at least the most new tokens of a sequence.
-ELFA_API int elfa_paged_attention(const void* q, long long qs, const void* pages, const int* table, const int* q_start, const int* kv_len, void* out,
-                                  float* scratch, int B, int N, int P, int page, int T, int H, int Hkv, int hd, int max_new, int window, int sinks,
-                                  float scale, void* stream) {
-  DecodeArgs a{};
-  const int rc = paged_geom(&a.g, pages, table, q_start, kv_len, B, N, P, page, T, H, Hkv, hd, max_new, window, sinks);
-  if (rc != ELFA_OK) return rc;
-  ELFA_REQUIRE(q && out, "paged_attention: null pointer");
-  ELFA_REQUIRE(B <= PAGED_MAX_SEQS, "paged_attention: too many sequences for one launch");
-  ELFA_REQUIRE(qs % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
-               "paged_attention: query rows must lie on 16-byte boundaries");
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (many_rows(max_new, a.g.rep, hd)) {
+namespace {
+
+// One launch (and its join), of at most PAGED_MAX_SEQS sequences.
+int paged_part(const PagedGeom& g, const void* q, long long qs, const void* pages, void* out, float* scratch, int page, float scale, cudaStream_t st) {
+  if (many_rows(g.max_new, g.rep, g.hd)) {
     ELFA_REQUIRE(scratch && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0, "paged_attention: no scratch, or not 16-byte aligned");
-    return paged_prefill(a.g, q, qs, pages, out, scratch, page, scale, st);
+    return paged_prefill(g, q, qs, pages, out, scratch, page, scale, st);
   }
+  DecodeArgs a{};
+  a.g = g;
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.pages = static_cast<const __nv_bfloat16*>(pages);
   a.out = static_cast<__nv_bfloat16*>(out);
@@ -639,13 +641,38 @@ ELFA_API int elfa_paged_attention(const void* q, long long qs, const void* pages
   a.scale = scale;
   a.g.tile_rows = DROWS;
   a.g.by_tile = div_by(DROWS);
-  a.whole = decode_whole(B, Hkv, hd, max_new, a.g.rep, (long long)N * page, a.g.window, a.g.sinks);
-  a.wide = ((long long)max_new * a.g.rep + DROWS - 1) / DROWS > 4;
+  a.whole = decode_whole(g.B, g.Hkv, g.hd, g.max_new, g.rep, (long long)g.N * page, g.window, g.sinks);
+  a.wide = ((long long)g.max_new * g.rep + DROWS - 1) / DROWS > 4;
   a.min_units = MIN_UNITS;
   ELFA_REQUIRE(paged_units_fit(a.g, DBLK), "paged_attention: too much work for one call (2^32 tiles of 16 rows by 32 keys)");
   ELFA_REQUIRE(a.whole || (scratch && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0), "paged_attention: no scratch, or not 16-byte aligned");
   a.part = scratch;
-  a.stat = scratch + 2LL * decode_grid(hd) * DROWS * (hd <= 64 ? 64 : 128);
-  a.notes = reinterpret_cast<PagedJoin*>(a.stat + 2LL * decode_grid(hd) * DROWS * 2);
-  return hd <= 64 ? launch_decode<64>(a, page, st) : launch_decode<128>(a, page, st);
+  a.stat = scratch + 2LL * decode_grid(g.hd) * DROWS * (g.hd <= 64 ? 64 : 128);
+  a.notes = reinterpret_cast<PagedJoin*>(a.stat + 2LL * decode_grid(g.hd) * DROWS * 2);
+  return g.hd <= 64 ? launch_decode<64>(a, page, st) : launch_decode<128>(a, page, st);
+}
+
+}  // namespace
+
+// q: rows [T] of H heads, `qs` elements apart, heads packed, 16-byte aligned; out: [T, H * hd] contiguous. max_new: at least the most new tokens of a sequence.
+ELFA_API int elfa_paged_attention(const void* q, long long qs, const void* pages, const int* table, const int* q_start, const int* kv_len, void* out,
+                                  float* scratch, int B, int N, int P, int page, int T, int H, int Hkv, int hd, int max_new, int window, int sinks,
+                                  float scale, void* stream) {
+  PagedGeom g{};
+  int rc = paged_geom(&g, pages, table, q_start, kv_len, B, N, P, page, T, H, Hkv, hd, max_new, window, sinks);
+  if (rc != ELFA_OK) return rc;
+  ELFA_REQUIRE(q && out, "paged_attention: null pointer");
+  ELFA_REQUIRE(qs % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
+               "paged_attention: query rows must lie on 16-byte boundaries");
+  for (int b = 0; b < B; b += PAGED_MAX_SEQS) {            // q_start counts from the first row of the whole call in every launch
+    PagedGeom part = g;
+    part.B = B - b < PAGED_MAX_SEQS ? B - b : PAGED_MAX_SEQS;
+    part.table = table + (long long)b * N;
+    part.q_start = q_start + b;
+    part.kv_len = kv_len + b;
+    part.ends = (b == 0 ? 1 : 0) | (part.B == B - b ? 2 : 0);
+    rc = paged_part(part, q, qs, pages, out, scratch, page, scale, static_cast<cudaStream_t>(stream));
+    if (rc != ELFA_OK) return rc;
+  }
+  return ELFA_OK;
 }

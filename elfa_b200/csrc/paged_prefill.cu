@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) paged_prefill_kernel(const __grid
   fence_proxy_async();
   const PagedLine line = paged_line(smem + L::OUT, g.B, tmem_holder + 4);
   const unsigned W = paged_prefix<PBLK, PTHREADS>(g, line, true);
+  if (blockIdx.x == 0) paged_rest(g, a.out, line.seqs[0], line.seqs[g.B - 1]);
   const int G = (int)min(W, gridDim.x);
   const PagedShares shares(W, G);
   const unsigned u_begin = (int)blockIdx.x < G ? shares.first(blockIdx.x) : 0, u_end = (int)blockIdx.x < G ? shares.first(blockIdx.x + 1) : 0;

@@ -23,7 +23,6 @@ import torch
 from ..native import lib, stream_ptr
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
-_MAX_SEQS = 1024        # sequences of one launch
 
 
 def paged_attention_ref(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
@@ -94,16 +93,16 @@ def _rows(t: torch.Tensor, hd: int) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=256)
-def _scratch_floats(B: int, *sizes: int) -> int:
-    parts = {B} if B <= _MAX_SEQS else {_MAX_SEQS, B % _MAX_SEQS or _MAX_SEQS}
-    return max(lib.raw("elfa_paged_attention_scratch")(b, *sizes) for b in parts)
+def _scratch_floats(*sizes: int) -> int:
+    return lib.raw("elfa_paged_attention_scratch")(*sizes)
 
 
 def paged_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
                     max_new: Optional[int] = None, window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None) -> torch.Tensor:
     """The new tokens' queries ``q [T, H, hd]`` (rows may be strided) against the pages, which hold the new tokens' keys and values already
     (:func:`paged_write`). A query at position ``p`` sees the keys up to ``p``; with a ``window`` the last ``window`` of them and the first ``sinks``; never those of
-    pages that are not there. A row that sees nothing (or only scores of -inf) is zero, and what a row does not see cannot reach it whatever it holds. ``H`` is a
+    pages that are not there. A row that sees nothing (or only scores of -inf) is zero, and what a row does not see cannot reach it whatever it holds; so is a row that
+    no sequence has, which the status word tells of. ``H`` is a
     multiple of ``Hkv``. ``max_new``: an upper bound of the new tokens of one sequence, known to the host; without it the number of rows. Returns ``[T, H * hd]``."""
     P, Hkv, page, hd, B, N = _check(pages, table, q_start, kv_len, "paged_attention")
     qs = q.shape
@@ -135,10 +134,8 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q
     window, sinks = min(window or 0, 1 << 30), min(sinks, 1 << 30)
     n = _scratch_floats(B, N, page, H, Hkv, hd, max_new, window, sinks)
     scratch = q.new_empty(n, dtype=torch.float32) if n else None
-    pt, pq, pk, ps = table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), scratch.data_ptr() if n else None
-    for b in range(0, B, _MAX_SEQS):           # q_start counts from the first row of the whole call in every part
-        lib.call_plain("elfa_paged_attention", q.data_ptr(), q.stride(0), pages.data_ptr(), pt + 4 * b * N, pq + 4 * b, pk + 4 * b, out.data_ptr(), ps,
-                       min(_MAX_SEQS, B - b), N, P, page, T, H, Hkv, hd, max_new, window, sinks, scale if scale is not None else hd ** -0.5, stream_ptr(q))
+    lib.call_plain("elfa_paged_attention", q.data_ptr(), q.stride(0), pages.data_ptr(), table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), out.data_ptr(),
+                   scratch.data_ptr() if n else None, B, N, P, page, T, H, Hkv, hd, max_new, window, sinks, scale if scale is not None else hd ** -0.5, stream_ptr(q))
     return out
 
 

@@ -92,3 +92,29 @@ def test_a_step_of_many_sequences(cuda_device):
     def mix(vals):
         return torch.einsum("nhk,kd->nhd", p[..., :20], vals[:20, 0]) + p[..., 20:] * vals[20:, 0][:, None]
     assert native.status() == 0 and close(o, mix(v.double()), mix(v.double().abs()))
+
+
+@pytest.mark.parametrize("lens,H,Hkv,hd", [([(1, 60), (1, 33)], 4, 2, 64), ([(1, 2000)], 2, 2, 64), ([(1, 5000), (3, 900), (1, 1)], 8, 2, 128), ([(70, 300), (50, 90)], 8, 2, 64),
+                                           ([(1 + i % 3, 3 + i % 50) for i in range(1100)], 2, 1, 32)])
+@pytest.mark.parametrize("front,back", [(0, 3), (5, 0), (2, 40)])
+def test_rows_of_no_sequence(cuda_device, lens, H, Hkv, hd, front, back):
+    """Rows in front of the first sequence's and behind the last one's are zeros as on the host, and recorded; all forms of the attention."""
+    c = make(lens, H, Hkv, hd, 16)
+    ref, mag = attend64(c)
+    new = max(n for n, _ in lens)
+    n = c["q"].shape[0]
+    d = {**c, "q": torch.cat([torch.ones(front, H, hd, device=cuda_device).bfloat16(), c["q"], torch.ones(back, H, hd, device=cuda_device).bfloat16()]),
+         "q_start": c["q_start"] + front}
+    torch.full((n + front + back, H * hd), float("nan"), dtype=torch.bfloat16, device=cuda_device)       # what the result's memory held before
+    o = _run(d, max_new=new)
+    assert native.status() == native.ST_BAD_PAGE
+    assert close(o[front:front + n], ref, mag) and not o[:front].any() and not o[front + n:].any()
+    assert close(_run(c, max_new=new), ref, mag) and native.status() == 0
+
+
+def test_no_sequence_has_a_row(cuda_device):
+    for new, H in ((1, 4), (200, 4)):
+        c = make([(new, 300), (0, 20)], H, 2, 64, 16)
+        torch.full((new, H * 64), float("nan"), dtype=torch.bfloat16, device=cuda_device)
+        o = _run({**c, "q_start": torch.zeros_like(c["q_start"])})
+        assert native.status() == native.ST_BAD_PAGE and not o.any()
