@@ -56,7 +56,9 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedGeom& g, int b, bool* i
   return s;
 }
 // Rows that no sequence has give zeros: those in front of the launch's first sequence and behind its last one, by all threads of one block.
-__device__ __forceinline__ void paged_zero_rows(const PagedGeom& g, __nv_bfloat16* out, int from, int to) {
+// Out of line: the decoding kernel has no register to spare (inlined, it spills 36 bytes).
+template <int = 0>
+__device__ __noinline__ void paged_zero_rows(const PagedGeom& g, __nv_bfloat16* out, int from, int to) {
   uint4* p = reinterpret_cast<uint4*>(out);
   const long long row = (long long)g.H * g.hd / 8;
   for (long long i = from * row + threadIdx.x; i < to * row; i += blockDim.x) p[i] = make_uint4(0u, 0u, 0u, 0u);
