@@ -35,10 +35,12 @@ __global__ void __launch_bounds__(256) paged_write_kernel(const __grid_constant_
       if (g.q_start[mid] <= t) lo = mid;
       else hi = mid;
     }
-    const PagedSeq s = paged_seq(g, lo);
+    bool fits;                             // else the clamped lengths would lead to the places of other tokens
+    const PagedSeq s = paged_seq(g, lo, &fits);
+    fits = fits && s.kv == g.kv_len[lo] && s.n <= s.kv;
     const int pos = s.kv - s.n + t - s.q0;
     long long at = -1;
-    if (t >= s.q0 && t < s.q0 + s.n && pos >= 0) {
+    if (fits && t >= s.q0 && t < s.q0 + s.n) {
       const int id = paged_page(g, lo, pos);
       if (id >= 0) at = ((long long)id * 2 * g.Hkv * page + (pos & (page - 1))) * hv;
     }

@@ -140,7 +140,8 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q
 
 
 def paged_write(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor) -> None:
-    """Writes the new tokens' keys and values ``k, v [T, Hkv, hd]`` (rows may be strided) into their places, in place. Every new token needs a page."""
+    """Writes the new tokens' keys and values ``k, v [T, Hkv, hd]`` (rows may be strided) into their places, in place. Every new token needs a page;
+    of a sequence whose lengths do not fit nothing is written."""
     P, Hkv, page, hd, B, N = _check(pages, table, q_start, kv_len, "paged_write")
     ks, dev = k.shape, k.get_device()
     if len(ks) != 3 or ks != v.shape or ks[1] != Hkv or ks[2] != hd:

@@ -118,3 +118,24 @@ def test_no_sequence_has_a_row(cuda_device):
         torch.full((new, H * 64), float("nan"), dtype=torch.bfloat16, device=cuda_device)
         o = _run({**c, "q_start": torch.zeros_like(c["q_start"])})
         assert native.status() == native.ST_BAD_PAGE and not o.any()
+
+
+@pytest.mark.parametrize("change", [dict(kv_len=[5000, 50, 20]), dict(kv_len=[113, 50, 20]), dict(kv_len=[3, 50, 20]), dict(kv_len=[-9, 50, 20]), dict(q_start=[-2, 4, 5, 7]),
+                                    dict(q_start=[0, 4, 5, 9])])
+def test_lengths_that_do_not_fit_write_nothing(cuda_device, change):
+    """Tokens of such a sequence have no place: they must not land on those of others. The other sequences' are written."""
+    c = make([(4, 100), (1, 50), (2, 20)], 4, 2, 64, 16, unused=0.0)
+    for name, v in change.items():
+        c[name] = torch.tensor(v, dtype=torch.int32, device=cuda_device)
+    want = c["pages"].clone()
+    st, kv = c["q_start"].tolist(), c["kv_len"].tolist()
+    for b in range(3):
+        n = st[b + 1] - st[b]
+        if st[b] < 0 or st[b + 1] > 7 or not n <= kv[b] <= 112:
+            continue
+        for i in range(n):
+            p, r = divmod(kv[b] - n + i, 16)
+            want[c["table"][b, p].long(), 0, :, r], want[c["table"][b, p].long(), 1, :, r] = c["k"][st[b] + i], c["v"][st[b] + i]
+    ops.paged_write(c["k"], c["v"], c["pages"], c["table"], c["q_start"], c["kv_len"])
+    assert native.status() == native.ST_BAD_PAGE
+    assert torch.equal(c["pages"], want)
