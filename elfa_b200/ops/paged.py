@@ -156,15 +156,21 @@ def paged_write(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, table: to
     if B == 0 or N == 0:
         raise ValueError("paged_write: new tokens without a sequence or a page")
     if dev < 0:
-        starts = q_start.tolist()
-        for b, kv in enumerate(kv_len.tolist()):
+        starts, lens, places = q_start.tolist(), kv_len.tolist(), []
+        if starts[0] != 0 or starts[-1] != T or sorted(starts) != starts:
+            raise ValueError(f"paged_write: q_start must rise from 0 to the {T} rows, got {starts}")
+        for b, kv in enumerate(lens):
             n = starts[b + 1] - starts[b]
-            pos = torch.arange(kv - n, kv)
-            ids = table[b, pos // page].long()
-            if bool(((ids < 0) | (ids >= pages.shape[0])).any()):
+            if n and not n <= kv <= N * page:
+                raise ValueError(f"paged_write: sequence {b} of {kv} tokens, {n} of them new, does not fit its table of {N * page}")
+            pos = torch.arange(kv - n, kv) if n else torch.empty(0, dtype=torch.int64)
+            ids = table[b, pos // page].long()                 # none of a sequence without new tokens
+            if bool(((ids < 0) | (ids >= P)).any()):
                 raise ValueError("paged_write: a new token without a page")
-            pages[ids, 0, :, pos % page] = k[starts[b]:starts[b + 1]]
-            pages[ids, 1, :, pos % page] = v[starts[b]:starts[b + 1]]
+            places.append((ids, pos % page))
+        for b, (ids, at) in enumerate(places):                 # nothing is written where a test fails
+            pages[ids, 0, :, at] = k[starts[b]:starts[b + 1]]
+            pages[ids, 1, :, at] = v[starts[b]:starts[b + 1]]
         return
     k, v = _rows(k, hd), _rows(v, hd)
     if not (table.is_contiguous() and q_start.is_contiguous() and kv_len.is_contiguous()):

@@ -2,6 +2,13 @@
 import re
 from pathlib import Path
 
+import pytest
+import torch
+
+from elfa_b200 import ops
+
+from paged_cases import make
+
 CSRC = Path(__file__).resolve().parent.parent / "elfa_b200" / "csrc"
 
 
@@ -19,3 +26,22 @@ def test_tensor_memory_is_touched_behind_a_fence():
         else:
             assert not open_wait, f"{word} behind a wait without a fence"
     assert seen >= 4
+
+
+@pytest.mark.parametrize("change", [dict(kv_len=[5000, 50, 20]), dict(kv_len=[3, 50, 20]), dict(kv_len=[-9, 50, 20]), dict(q_start=[-2, 4, 5, 7]), dict(q_start=[0, 4, 5, 9]),
+                                    dict(q_start=[0, 4, 5, 6]), dict(q_start=[1, 4, 5, 7]), dict(q_start=[0, 4, 3, 7])])
+def test_lengths_that_do_not_fit_write_nothing(change):
+    c = make([(4, 100), (1, 50), (2, 20)], 4, 2, 8, 16, device="cpu", dtype=torch.float32, unused=0.0)
+    for name, v in change.items():
+        c[name] = torch.tensor(v, dtype=torch.int32)
+    before = c["pages"].clone()
+    with pytest.raises(ValueError, match="paged_write"):
+        ops.paged_write(c["k"], c["v"], c["pages"], c["table"], c["q_start"], c["kv_len"])
+    assert torch.equal(c["pages"], before)
+
+
+def test_a_sequence_without_new_tokens_is_not_looked_at():
+    c = make([(4, 100), (0, 50)], 4, 2, 8, 16, device="cpu", dtype=torch.float32, unused=0.0)
+    c["kv_len"][1] = 9000
+    ops.paged_write(c["k"], c["v"], c["pages"], c["table"], c["q_start"], c["kv_len"])
+    assert torch.equal(c["pages"][c["table"][0, 6].long(), 0, :, :4], c["k"].transpose(0, 1))
