@@ -2,8 +2,8 @@
 //
 // w_i = exp((x_i - max x) / T). In the order of falling x (equal ones by index) every filter keeps a prefix: the first k; of those the
 // shortest one with mass >= p of theirs; of those the ones with w_i >= min_p. What is kept races: the token with the largest w_i / e_i wins, which
-// for independent exponential variates e_i is token i with probability w_i / sum w (the lowest index where two are equal). T <= 0 takes the first largest logit.
-// A NaN counts as -inf; a row without any number above -inf gives -1.
+// for independent exponential variates e_i is token i with probability w_i / sum w (the lowest index where two are equal). T <= 0 takes the first largest logit, and so
+// does a row of which nothing races (min_p above 1; variates that are NaN). A NaN logit counts as -inf; a row without any number above -inf gives -1.
 //
 // Sums are of fp32 weights, joined in fp32 or fp64; what decides between two tokens is fp32. Counts and places are integers, so a result does not depend on the order in
 // which threads come. Bound by latency where rows are few (a dozen meetings of a row's CTAs: one row of 32000, all filters, 20 us) and by the passes' instructions
@@ -135,6 +135,16 @@ __device__ __noinline__ float part_max(Part<T> p) {
   float mx = -CUDART_INF_F;
   p.template each<6>([&](float v, int) { mx = fmaxf(mx, v); });
   return mx;
+}
+
+// -> the place of the first token with that value, of the thread's ones; 0 for none.
+template <typename T>
+__device__ __noinline__ unsigned long long part_first(Part<T> p, float mx) {
+  unsigned long long first = 0;
+  p.template each<EACH>([&](float v, int i) {
+    if (v == mx) first = max(first, place(v, i));
+  });
+  return first;
 }
 
 // Tokens per bin; -> the mass.
@@ -336,12 +346,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
   if (C > 1) cluster_sync_all();           // every CTA of the row has started
   const float mx = value_of(most(place(part_max<T>(part), 0)));
   if (mx == -CUDART_INF_F || !(asked > 0.f)) {
-    unsigned long long first = 0;          // of the largest, the one with the lowest index
-    if (mx != -CUDART_INF_F)
-      each([&](float v, int i) {
-        if (v == mx) first = max(first, place(v, i));
-      });
-    first = most(first);
+    const unsigned long long first = most(mx == -CUDART_INF_F ? 0 : part_first<T>(part, mx));
     if (rank == 0 && tid == 0) a.out[b] = index_of(first);             // -1 of 0
     return;
   }
@@ -725,12 +730,11 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
           race_list(n);
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) win = max(win, __shfl_xor_sync(0xffffffffu, win, o));
-          __syncthreads();
-          if (lane == 0) s.list[warp] = win;
+          if (lane == 0) s.swap[warp] = win;
           __syncthreads();
           if (tid == 0) {
-            for (int w = 0; w < SW; ++w) win = max(win, s.list[w]);
-            a.out[b] = index_of(win);
+            for (int w = 0; w < SW; ++w) win = max(win, s.swap[w]);
+            a.out[b] = index_of(win ? win : s.list[0]);    // the first largest where none of them raced
           }
           return;
         }
@@ -806,6 +810,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     settle(all);
   }
   win = most(win);
+  if (win == 0) win = most(part_first<T>(part, mx));       // nothing raced: the first largest (the same turn in every thread of the row)
   if (rank == 0 && tid == 0) a.out[b] = index_of(win);
 }
 

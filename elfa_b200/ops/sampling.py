@@ -61,7 +61,8 @@ def sample(logits: torch.Tensor, noise: Optional[torch.Tensor], temperature: _Se
 
     With ``w_i = exp((x_i - max x) / temperature)`` and the tokens by falling logit (equal ones by index): the first ``top_k`` (0: all), of those the shortest
     prefix with at least ``top_p`` of their mass (1: all), of those the ones with ``w_i >= min_p``. The token with the largest ``w_i / noise_i`` is returned, which is
-    token ``i`` with probability ``w_i / sum w``; the lowest index where two are equal. ``temperature <= 0``: the first largest logit. A NaN counts as -inf; a row
+    token ``i`` with probability ``w_i / sum w``; the lowest index where two are equal. ``temperature <= 0``: the first largest logit, and so where no token races (``min_p`` above 1, variates that are
+    NaN). A NaN counts as -inf; a row
     with nothing above -inf gives -1. Each setting is a number or a tensor with one per row. Runs on the current stream without a host synchronisation."""
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"sample: logits must be [B, V], got {tuple(logits.shape)}")

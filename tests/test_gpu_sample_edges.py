@@ -1,0 +1,47 @@
+"""Sampling at the edges of what it takes: the device against the host's form of the definition."""
+import pytest
+import torch
+
+from elfa_b200 import native, ops
+
+pytestmark = pytest.mark.gpu
+
+
+def _draws(B, V, seed, dtype=torch.float32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = (torch.randn(B, V, generator=g, device="cuda") * 2.5).to(dtype)
+    return x, torch.empty(B, V, device="cuda").exponential_(generator=g)
+
+
+def _both(x, noise, *settings):
+    host = [s.cpu() if isinstance(s, torch.Tensor) else s for s in settings]
+    return ops.sample(x, noise, *settings).tolist(), ops.sample(x.cpu(), noise.cpu(), *host).tolist()
+
+
+@pytest.mark.parametrize("B,V,dtype", [(1, 1, torch.float32), (4, 1000, torch.bfloat16), (3, 32000, torch.bfloat16), (2, 131072, torch.float32), (200, 9000, torch.float32)])
+@pytest.mark.parametrize("k,p", [(0, 1.0), (5, 1.0), (6000, 1.0), (0, 0.7), (40, 0.7), (6000, 0.7), (1, 1.0)])
+def test_rows_of_which_nothing_races(cuda_device, B, V, dtype, k, p):
+    """min_p above 1 keeps no token, and a variate that is NaN keeps its token out of the race: the first largest logit, of equal ones the first."""
+    x, noise = _draws(B, V, V + B, dtype)
+    x[:, V // 3] = x[:, V // 2] = x.amax(1)
+    first = x.float().cpu().numpy().argmax(1).tolist()                       # of equal ones the first
+    nan = torch.full_like(noise, float("nan"))
+    for e, m in ((noise, 1.5), (noise, float("inf")), (nan, 0.0), (nan, 0.1)):
+        got, want = _both(x, e, 0.8, k, p, m)
+        assert got == want == first
+    rows = torch.where(torch.arange(B, device=cuda_device) % 2 == 0, 1.5, 0.0)
+    got, want = _both(x, noise, 0.8, k, p, rows)
+    assert got[::2] == want[::2] == first[::2]
+    x[:] = float("-inf")
+    assert _both(x, nan, 0.8, k, p, 1.5) == ([-1] * B, [-1] * B)
+    assert native.status() == 0
+
+
+def test_only_what_is_kept_counts(cuda_device):
+    """The kept tokens' variates are NaN, those of the others are not."""
+    x, noise = _draws(4, 20000, 7)
+    order = x.argsort(1, descending=True, stable=True)
+    noise.scatter_(1, order[:, :10], float("nan"))
+    for k, p, m in ((10, 1.0, 0.0), (10, 0.9, 0.0), (0, 1e-4, 0.0)):
+        got, want = _both(x, noise, 1.0, k, p, m)
+        assert got == want == order[:, 0].tolist()
