@@ -341,8 +341,9 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
   auto race_top = [](double2 all) { return __int_as_float(__double2hiint(all.y)); };
 
   const int kr = a.top_k ? a.top_k[b] : a.top_k_all, k = kr > 0 && kr < V ? kr : V;
-  const float asked = a.temperature ? a.temperature[b] : a.temperature_all, temp = fminf(asked, 1e30f), p = a.top_p ? a.top_p[b] : a.top_p_all,
-              min_p = a.min_p ? a.min_p[b] : a.min_p_all;
+  const float asked = a.temperature ? a.temperature[b] : a.temperature_all, temp = fminf(asked, 1e30f), asked_p = a.top_p ? a.top_p[b] : a.top_p_all,
+              asked_min = a.min_p ? a.min_p[b] : a.min_p_all;
+  const float p = fmaxf(asked_p, 0.f), min_p = isnan(asked_min) ? CUDART_INF_F : asked_min;            // of a NaN: the first token, none in the race
   if (C > 1) cluster_sync_all();           // every CTA of the row has started
   const float mx = value_of(most(place(part_max<T>(part), 0)));
   if (mx == -CUDART_INF_F || !(asked > 0.f)) {

@@ -45,3 +45,21 @@ def test_only_what_is_kept_counts(cuda_device):
     for k, p, m in ((10, 1.0, 0.0), (10, 0.9, 0.0), (0, 1e-4, 0.0)):
         got, want = _both(x, noise, 1.0, k, p, m)
         assert got == want == order[:, 0].tolist()
+
+
+@pytest.mark.parametrize("V,dtype", [(1000, torch.float32), (32000, torch.bfloat16), (131072, torch.float32)])
+@pytest.mark.parametrize("name", ["temperature", "top_p", "min_p"])
+@pytest.mark.parametrize("k", [0, 50, 6000])
+def test_settings_that_are_nan(cuda_device, V, dtype, name, k):
+    """Every test on a NaN is false: such a row takes its first largest logit, whether the setting is one for all rows or the row's own."""
+    x, noise = _draws(6, V, V, dtype)
+    s = dict(temperature=0.9, top_k=k, top_p=0.8, min_p=0.01)
+    order = ("temperature", "top_k", "top_p", "min_p")
+    got, want = _both(x, noise, *({**s, name: float("nan")}[n] for n in order))
+    assert got == want == x.float().cpu().numpy().argmax(1).tolist()
+    rows = torch.full((6,), s[name], device=cuda_device)
+    rows[::2] = float("nan")
+    for others in (s, dict(temperature=0.9, top_k=k, top_p=1.0, min_p=0.0)):
+        mixed, want = _both(x, noise, *({**others, name: rows}[n] for n in order))
+        assert mixed[::2] == want[::2] == got[::2]
+    assert mixed[1::2] == ops.sample(x, noise, *({**others, name: s[name]}[n] for n in order)).tolist()[1::2]
