@@ -49,14 +49,15 @@ def paged_attention_ref(q: torch.Tensor, pages: torch.Tensor, table: torch.Tenso
         qb = q[starts[b]:starts[b + 1]].to(acc).view(n, Hkv, H // Hkv, hd)
         s = torch.einsum("nhrd,khd->hrnk", qb, rows[:, 0]) * sc
         s = s.masked_fill(~sees, float("-inf"))
-        p = torch.softmax(s, -1).masked_fill(~sees, 0.0)                                     # a row that sees nothing: zeros
+        nothing = (s == float("-inf")).all(-1, keepdim=True) | ~sees                         # a row that sees nothing, or only scores of -inf: zeros
+        p = torch.softmax(s, -1).masked_fill(nothing, 0.0)
         # what a row does not see must not reach it, not even as 0 times infinity
         v = rows[:, 1]
         if bool(torch.isfinite(v).all()):
             o = torch.einsum("hrnk,khd->nhrd", p, v)
         else:
             o = torch.stack([torch.einsum("hrk,khd->hrd", p[:, :, i][..., sees[i]], v[sees[i]]) for i in range(n)])
-        out[starts[b]:starts[b + 1]] = o.reshape(n, H, hd)
+        out[starts[b]:starts[b + 1]] = o.masked_fill(nothing.all(-1).permute(2, 0, 1)[..., None], 0.0).reshape(n, H, hd)
     return out.reshape(T, H * hd).to(q.dtype)
 
 

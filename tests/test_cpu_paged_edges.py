@@ -7,7 +7,7 @@ import torch
 
 from elfa_b200 import ops
 
-from paged_cases import make
+from paged_cases import attend64, make
 
 CSRC = Path(__file__).resolve().parent.parent / "elfa_b200" / "csrc"
 
@@ -45,3 +45,24 @@ def test_a_sequence_without_new_tokens_is_not_looked_at():
     c["kv_len"][1] = 9000
     ops.paged_write(c["k"], c["v"], c["pages"], c["table"], c["q_start"], c["kv_len"])
     assert torch.equal(c["pages"][c["table"][0, 6].long(), 0, :, :4], c["k"].transpose(0, 1))
+
+
+def test_rows_that_see_only_scores_of_minus_infinity():
+    """Zero, as the kernels give; a row that sees one finite score too is as without the others, and scores of plus infinity or NaN are no reason for a zero."""
+    c = make([(3, 40), (1, 17)], 4, 4, 8, 16, device="cpu", dtype=torch.float64)
+    c["q"] = c["q"].abs() + 0.1
+    ids = c["table"][0, :3].long()
+    c["pages"][ids[:2], 0] = float("-inf")
+    c["pages"][ids[2], 0, :, :6] = float("-inf")                   # tokens 0 to 37; 38 and 39 are finite
+    o = ops.paged_attention(c["q"], c["pages"], c["table"], c["q_start"], c["kv_len"]).view(4, 4, 8)
+    assert not o[0].any() and not o.isnan().any()
+    assert torch.allclose(o[1], c["pages"][ids[2], 1, :, 6], atol=1e-12)
+    ref, _ = attend64({**c, "q": c["q"][3:], "table": c["table"][1:], "q_start": torch.tensor([0, 1]), "kv_len": c["kv_len"][1:]})
+    assert torch.allclose(o[3].view(1, -1), ref, atol=1e-12)
+    c["pages"][ids[0], 1, 3, 5] = float("inf")                      # a value that a row with no weight at all sees
+    assert torch.equal(ops.paged_attention(c["q"], c["pages"], c["table"], c["q_start"], c["kv_len"])[0], o[0].reshape(-1))
+    c["pages"][ids[0], 1, 3, 5] = 0.0
+    for bad in (float("inf"), float("nan")):
+        c["pages"][ids[0], 0, 0, 3] = bad
+        o = ops.paged_attention(c["q"], c["pages"], c["table"], c["q_start"], c["kv_len"]).view(4, 4, 8)
+        assert o[:3, 0].isnan().all() and not o[0, 1:].any() and not o[3].isnan().any()

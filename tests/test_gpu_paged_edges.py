@@ -139,3 +139,21 @@ def test_lengths_that_do_not_fit_write_nothing(cuda_device, change):
     ops.paged_write(c["k"], c["v"], c["pages"], c["table"], c["q_start"], c["kv_len"])
     assert native.status() == native.ST_BAD_PAGE
     assert torch.equal(c["pages"], want)
+
+
+@pytest.mark.parametrize("lens,H,Hkv,hd", [([(1, 60), (2, 33)], 4, 2, 64), ([(1, 4000)], 2, 2, 64), ([(2, 5000), (3, 900)], 8, 2, 128), ([(70, 300), (50, 90)], 8, 2, 64),
+                                           ([(40, 3000)], 8, 1, 128)])
+@pytest.mark.parametrize("value", [0.0, float("inf")])
+def test_rows_that_see_only_scores_of_minus_infinity(cuda_device, lens, H, Hkv, hd, value):
+    """The first sequence's rows see keys of minus infinity but for the last one's; zero, whatever the values are, as on the host."""
+    c = make(lens, H, Hkv, hd, 16)
+    n, kv = lens[0]
+    c["q"] = c["q"].abs() + 0.1
+    pos = torch.arange(kv if n == 1 else kv - 1, device=cuda_device)
+    c["pages"][c["table"][0, pos // 16].long(), 0, :, pos % 16] = float("-inf")
+    c["pages"][c["table"][0, 0].long(), 1, 0, 5, 3] += value
+    o = _run(c, max_new=max(x for x, _ in lens)).view(-1, H, hd).float()
+    host = ops.paged_attention(*(c[x].cpu() for x in ("q", "pages", "table", "q_start", "kv_len"))).view(-1, H, hd).float()
+    assert native.status() == 0
+    assert not o[:max(n - 1, 1)].any()
+    assert torch.equal(o.isnan().cpu(), host.isnan()) and torch.allclose(o.cpu().nan_to_num(), host.nan_to_num(), atol=0.03)
