@@ -16,7 +16,7 @@ from typing import Dict, List, Optional
 
 import torch
 
-from .. import ops
+from .. import native, ops
 from ..data import BinaryDataset, DataLoader
 
 
@@ -110,7 +110,8 @@ class Generator:
         """``samples`` continuations of each prompt, all at once, from a cache of pages (softmax-attention family): a prompt runs once, in pieces of at most ``chunk``
         tokens, its samples fork off and share its pages, every step brings one token of each unfinished sequence, and tokens are drawn on the device
         (:func:`elfa_b200.ops.sample`). With a ``window`` tokens see the last ``window`` ones and the first ``sinks``, and pages out of sight are used again. Ends a
-        sequence behind ``eos_id``, or before the model's positions run out. Returns prompt and continuation of ``[prompt][sample]``."""
+        sequence behind ``eos_id``, or before the model's positions run out. Raises what kernels have recorded in the device status word. Returns prompt and
+        continuation of ``[prompt][sample]``."""
         if not hasattr(self.model, "forward_paged"):
             raise ValueError("generate_batch wants a model with a paged cache (the softmax-attention family)")
         if samples < 1 or chunk < 1:
@@ -144,6 +145,7 @@ class Generator:
             for row, (i, n) in zip(logits, part):
                 done[i] += n
                 last[i] = row
+        self._check_device()
         out = [[list(p) for _ in range(samples)] for p in prompts]
         seqs = [(i, j, s) for i, r in enumerate(roots) for j, s in enumerate([r] + cache.fork(r, samples - 1))]
         logits = torch.stack([last[i] for i, _, _ in seqs]) if seqs else None
@@ -160,6 +162,7 @@ class Generator:
             keep = []
             for x, ((i, j, s), t) in enumerate(zip(seqs, ids.tolist())):
                 if t < 0:
+                    self._check_device()
                     raise FloatingPointError("logits without a finite number: nothing to draw from")
                 out[i][j].append(t)
                 if t == eos_id:
@@ -171,7 +174,13 @@ class Generator:
             if not seqs or step + 1 == max_new_tokens:
                 break
             logits = self.model.forward_paged(ids, [s for _, _, s in seqs], [1] * len(seqs), cache)
+        self._check_device()
         return out
+
+    def _check_device(self) -> None:
+        """What kernels could only record (a wait that ran out, lengths or ids that do not fit) is an error here, not tokens drawn from what they left."""
+        if torch.device(self.device).type == "cuda":
+            native.check_status()
 
     def generate_greedy(self, prompt_ids, max_new_tokens=256):
         return self.generate_ids(prompt_ids, max_new_tokens, temperature=0.0)

@@ -68,3 +68,25 @@ def test_window_keeps_the_cache_small(cuda_device):
         lo = m.forward_paged(torch.randint(0, 2048, (n,), generator=g).cuda(), [s], [n], cache)
     assert cache.length(s) == 1550 and torch.isfinite(lo).all()
     native.check_status()
+
+
+@pytest.mark.parametrize("step", [0, 1, 5])
+def test_what_kernels_record_is_raised(cuda_device, monkeypatch, step):
+    """A table that names pages outside the pool, in the prompt or in one of the steps: an error, not tokens drawn from what was left."""
+    from elfa_b200.runtime.paged_cache import PagedCache
+    batch, calls = PagedCache._batch, []
+
+    def broken(self, seqs, new):
+        b = batch(self, seqs, new)
+        if len(calls) == step:
+            b.table.add_(1000)
+        calls.append(new)
+        return b
+    gen = Generator(_model(2))
+    native.status()
+    monkeypatch.setattr(PagedCache, "_batch", broken)
+    with pytest.raises(native.NativeError, match="paged cache"):
+        gen.generate_batch([[5, 6, 7]], 7, temperature=0.0, samples=2)
+    assert len(calls) == 7 if step else len(calls) == 1            # the prompt's is known before anything is drawn from it
+    monkeypatch.undo()
+    assert len(gen.generate_batch([[5, 6, 7]], 7, temperature=0.0, samples=2)[0][1]) == 10
