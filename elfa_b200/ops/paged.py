@@ -7,7 +7,7 @@ pages of each sequence in order (negative: not there). A call takes new tokens o
 
 CUDA tensors run the kernels of ``csrc/paged_decode.cu`` and ``csrc/pages.cu``: bf16, on the current stream, nothing is read back; lengths or
 page numbers that do not fit are recorded in the device status word (``native.check_status``). CPU tensors run the formula. There is no backward
-pass: sequences are generated, not trained, from a cache. :class:`elfa_b200.runtime.paged_cache.PagedCache` keeps pools, tables and lengths.
+pass, nor forward mode on CUDA: sequences are generated, not trained, from a cache. :class:`elfa_b200.runtime.paged_cache.PagedCache` keeps pools, tables and lengths.
 
 reference: ``src/eval/evaluator.zig:419-470`` (generation runs the whole context of one sequence again for every token).
 """
@@ -19,6 +19,7 @@ import math
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from ..native import lib, stream_ptr
 
@@ -85,6 +86,12 @@ def _check(pages: torch.Tensor, table: torch.Tensor, q_start: torch.Tensor, kv_l
     return ps[0], ps[2], ps[3], ps[4], ts[0], ts[1]
 
 
+def _no_tangent(what: str, *tensors: torch.Tensor) -> None:
+    """Kernels read addresses: the tangent of a forward-mode dual would be lost without a word."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative on CUDA: call it without tangents")
+
+
 def _rows(t: torch.Tensor, hd: int) -> torch.Tensor:
     """``t [T, heads, hd]`` with packed heads on 16-byte boundaries: itself (a slice of a fused projection is), or a copy."""
     st = t.stride()
@@ -121,6 +128,7 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, q
     T, H = qs[0], qs[1]
     if dev < 0:
         return paged_attention_ref(q, pages, table, q_start, kv_len, window, sinks, scale)
+    _no_tangent("paged_attention", q, pages)
     out = q.new_empty((T, H * hd))
     if T == 0:
         return out
@@ -173,6 +181,7 @@ def paged_write(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, table: to
             pages[ids, 0, :, at] = k[starts[b]:starts[b + 1]]
             pages[ids, 1, :, at] = v[starts[b]:starts[b + 1]]
         return
+    _no_tangent("paged_write", k, v, pages)
     k, v = _rows(k, hd), _rows(v, hd)
     if not (table.is_contiguous() and q_start.is_contiguous() and kv_len.is_contiguous()):
         table, q_start, kv_len = table.contiguous(), q_start.contiguous(), kv_len.contiguous()
@@ -203,6 +212,7 @@ def copy_pages(pages: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> N
         at = (slice(None),) * (pages.dim() - 5)
         pages[at + (torch.tensor(list(dst)),)] = pages[at + (torch.tensor(list(src)),)]
         return
+    _no_tangent("copy_pages", pages)
     L = pages.shape[0] if pages.dim() == 6 else 1
     if L == 0:
         return

@@ -157,3 +157,26 @@ def test_rows_that_see_only_scores_of_minus_infinity(cuda_device, lens, H, Hkv, 
     assert native.status() == 0
     assert not o[:max(n - 1, 1)].any()
     assert torch.equal(o.isnan().cpu(), host.isnan()) and torch.allclose(o.cpu().nan_to_num(), host.nan_to_num(), atol=0.03)
+
+
+def test_tangents_are_refused(cuda_device):
+    """A forward-mode dual among the inputs, which the kernels would drop; inside a level, plain tensors are taken as ever."""
+    import torch.autograd.forward_ad as fwd
+    c = make([(2, 40)], 4, 2, 64, 16)
+    args = ("table", "q_start", "kv_len")
+    plain = _run(c)
+    with torch.no_grad(), fwd.dual_level():
+        def dual(name):
+            return {**c, name: fwd.make_dual(c[name], torch.ones_like(c[name]))}
+        for name in ("q", "pages"):
+            with pytest.raises(RuntimeError, match="paged_attention has no forward"):
+                _run(dual(name))
+        for name in ("k", "v", "pages"):
+            d = dual(name)
+            with pytest.raises(RuntimeError, match="paged_write has no forward"):
+                ops.paged_write(d["k"], d["v"], d["pages"], *(d[a] for a in args))
+        with pytest.raises(RuntimeError, match="copy_pages has no forward"):
+            ops.copy_pages(dual("pages")["pages"], [0], [1])
+        assert torch.equal(_run(c), plain)
+        ops.paged_write(c["k"], c["v"], c["pages"], *(c[a] for a in args))
+    assert native.status() == 0
