@@ -124,7 +124,7 @@ class Generator:
         if any(len(p) > limit for p in prompts):
             raise ValueError(f"a prompt is longer than the model's {limit} positions")
         live = -(-min(max(longest, default=0), (window or limit) + sinks + chunk) // page_size) + 2        # pages of one sequence that are in use
-        pages = sum(-(-len(p) // page_size) + samples * min(-(-n // page_size) - len(p) // page_size + 1, live) for p, n in zip(prompts, longest))
+        pages = sum(min(-(-len(p) // page_size), live) + samples * min(-(-n // page_size) - len(p) // page_size + 1, live) for p, n in zip(prompts, longest))
         cache = self.model.new_paged_cache(max(pages, 1), page_size, window, sinks)
         gen = torch.Generator(device=dev)
         if seed is not None:

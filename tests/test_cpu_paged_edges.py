@@ -6,6 +6,9 @@ import pytest
 import torch
 
 from elfa_b200 import ops
+from elfa_b200.config import Config
+from elfa_b200.eval import Generator
+from elfa_b200.models.gpt import GPTModel
 
 from paged_cases import attend64, make
 
@@ -66,3 +69,29 @@ def test_rows_that_see_only_scores_of_minus_infinity():
         c["pages"][ids[0], 0, 0, 3] = bad
         o = ops.paged_attention(c["q"], c["pages"], c["table"], c["q_start"], c["kv_len"]).view(4, 4, 8)
         assert o[:3, 0].isnan().all() and not o[0, 1:].any() and not o[3].isnan().any()
+
+
+def _model(positions):
+    cfg = Config.from_file("configs/bench/smoke_cpu.yaml")
+    cfg.model.num_kv_heads, cfg.bench.learned_positions = 2, positions
+    return GPTModel(cfg, device=torch.device("cpu")).eval()
+
+
+@pytest.mark.parametrize("window,sinks,chunk,samples", [(20, 0, 16, 1), (20, 3, 16, 3), (33, 40, 7, 2), (1, 0, 1, 2), (16, 16, 16, 1)])
+def test_a_window_bounds_the_pool_of_long_prompts(monkeypatch, window, sinks, chunk, samples):
+    """Prompts far longer than the window take the pages that a window, the sinks and a piece of a prompt can hold, and no more; what is generated is what one that reserves
+    for the whole prompts gives."""
+    m = _model(False)
+    asked, make_cache = [], GPTModel.new_paged_cache
+
+    def new_paged_cache(self, pages, *args, **kw):
+        asked.append(pages)
+        return make_cache(self, pages * room, *args, **kw)
+    monkeypatch.setattr(GPTModel, "new_paged_cache", new_paged_cache)
+    prompts = [[(7 * i) % 90 for i in range(n)] for n in (600, 5, 333)]
+    outs = []
+    for room in (1, 8):
+        outs.append(Generator(m).generate_batch(prompts, 30, temperature=0.0, samples=samples, window=window, sinks=sinks, page_size=16, chunk=chunk))
+    assert outs[0] == outs[1] and all(len(o) == len(p) + 30 for p, s in zip(prompts, outs[0]) for o in s)
+    live = -(-(window + sinks + chunk) // 16) + 2
+    assert asked[0] <= len(prompts) * (1 + samples) * live < 600 // 16 + 333 // 16 + len(prompts) * samples * live
