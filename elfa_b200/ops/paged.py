@@ -93,9 +93,10 @@ def _no_tangent(what: str, *tensors: torch.Tensor) -> None:
 
 
 def _rows(t: torch.Tensor, hd: int) -> torch.Tensor:
-    """``t [T, heads, hd]`` with packed heads on 16-byte boundaries: itself (a slice of a fused projection is), or a copy."""
+    """``t [T, heads, hd]`` with packed heads on 16-byte boundaries and rows that do not overlap (a tensor map's must not): itself (a slice of a fused projection
+    is), or a copy."""
     st = t.stride()
-    if st[2] == 1 and st[1] == hd and st[0] % 8 == 0 and t.data_ptr() % 16 == 0:
+    if st[2] == 1 and st[1] == hd and st[0] % 8 == 0 and st[0] >= t.shape[1] * hd and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

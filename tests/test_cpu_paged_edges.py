@@ -95,3 +95,14 @@ def test_a_window_bounds_the_pool_of_long_prompts(monkeypatch, window, sinks, ch
     assert outs[0] == outs[1] and all(len(o) == len(p) + 30 for p, s in zip(prompts, outs[0]) for o in s)
     live = -(-(window + sinks + chunk) // 16) + 2
     assert asked[0] <= len(prompts) * (1 + samples) * live < 600 // 16 + 333 // 16 + len(prompts) * samples * live
+
+
+def test_rows_that_overlap_are_copied():
+    """A tensor map wants rows apart: a broadcast query, or rows that begin inside the one before, are copied for the kernels; slices of a fused projection are not."""
+    from elfa_b200.ops.paged import _rows
+    base = torch.randn(6, 4, 8)
+    for t in (base[0].expand(5, 4, 8), base.view(-1).as_strided((5, 4, 8), (8, 8, 1)), base.view(-1).as_strided((3, 4, 8), (24, 8, 1))):
+        r = _rows(t, 8)
+        assert r.is_contiguous() and r.data_ptr() != t.data_ptr() and torch.equal(r, t)
+    for t in (base, base[:, :3], base[::2, 1:], base[:1], base[0].expand(1, 4, 8)):
+        assert _rows(t, 8) is t

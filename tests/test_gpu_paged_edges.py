@@ -180,3 +180,16 @@ def test_tangents_are_refused(cuda_device):
         assert torch.equal(_run(c), plain)
         ops.paged_write(c["k"], c["v"], c["pages"], *(c[a] for a in args))
     assert native.status() == 0
+
+
+@pytest.mark.parametrize("new,H,Hkv,hd", [(1, 4, 2, 64), (6, 4, 2, 64), (1, 64, 2, 128), (90, 4, 2, 64)])
+def test_broadcast_rows(cuda_device, new, H, Hkv, hd):
+    """One row of queries, keys and values for all new tokens."""
+    c = make([(new, 300)], H, Hkv, hd, 16)
+    b = {**c, **{n: c[n][:1].contiguous()[0].expand(new, -1, -1) for n in ("q", "k", "v")}}
+    own = {**c, **{n: b[n].contiguous() for n in ("q", "k", "v")}}
+    for d in (b, own):
+        d["pages"] = c["pages"].clone()
+        ops.paged_write(d["k"], d["v"], d["pages"], d["table"], d["q_start"], d["kv_len"])
+    assert torch.equal(b["pages"].view(torch.int16), own["pages"].view(torch.int16))
+    assert torch.equal(_run(b), _run(own)) and close(_run(b), *attend64(own)) and native.status() == 0
