@@ -43,12 +43,15 @@ def sample_ref(logits: torch.Tensor, noise: Optional[torch.Tensor], temperature:
     return torch.where(empty, torch.full_like(ids, -1), torch.where((top.squeeze(1) < 0) | greedy.squeeze(1), order[:, 0], ids))
 
 
-def _setting(value: _Setting, name: str, dtype: torch.dtype, rows: torch.Size, dev: int):
-    """(tensor or None, number) of a setting that is one number for all rows or a tensor with one per row."""
+def _setting(value: _Setting, name: str, dtype: torch.dtype, rows: torch.Size, dev: int, most: int = 0):
+    """(tensor or None, number) of a setting that is one number for all rows or a tensor with one per row. ``most``: a bound of whole numbers, whose bits a narrower
+    type would drop."""
     if not isinstance(value, torch.Tensor):
-        return None, value
+        return None, max(0, min(int(value), most)) if most else value
     if value.shape != rows or value.get_device() != dev:
         raise ValueError(f"sample: {name} must be a number or one per row, {list(rows)} on device {dev} (-1: host)")
+    if most and value.dtype in (torch.int64, torch.float32, torch.float64):
+        value = value.clamp(0, most)
     if value.dtype is not dtype or not value.is_contiguous():
         value = value.to(dtype).contiguous()
     return value, 0
@@ -74,7 +77,7 @@ def sample(logits: torch.Tensor, noise: Optional[torch.Tensor], temperature: _Se
     elif noise.shape != logits.shape or noise.dtype is not torch.float32 or noise.get_device() != dev:
         raise ValueError(f"sample: noise must be fp32 {tuple(logits.shape)} on {logits.device}")
     t, tn = _setting(temperature, "temperature", torch.float32, rows, dev)
-    k, kn = _setting(top_k, "top_k", torch.int32, rows, dev)
+    k, kn = _setting(top_k, "top_k", torch.int32, rows, dev, V)
     p, pn = _setting(top_p, "top_p", torch.float32, rows, dev)
     m, mn = _setting(min_p, "min_p", torch.float32, rows, dev)
     if B == 0:
@@ -91,6 +94,6 @@ def sample(logits: torch.Tensor, noise: Optional[torch.Tensor], temperature: _Se
         noise = noise.contiguous()
     out = logits.new_empty(B, dtype=torch.int64)
     pt, pk, pp, pm, pe = (s.data_ptr() if s is not None else None for s in (t, k, p, m, noise))
-    lib.call_plain("elfa_sample", logits.data_ptr(), int(logits.dtype is torch.float32), logits.stride(0), pe, noise.stride(0) if pe else 0, pt, pk, pp, pm, tn,
-                   max(0, min(int(kn), V)), pn, mn, out.data_ptr(), B, V, stream_ptr(logits))
+    lib.call_plain("elfa_sample", logits.data_ptr(), int(logits.dtype is torch.float32), logits.stride(0), pe, noise.stride(0) if pe else 0, pt, pk, pp, pm, tn, kn,
+                   pn, mn, out.data_ptr(), B, V, stream_ptr(logits))
     return out

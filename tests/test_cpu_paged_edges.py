@@ -106,3 +106,16 @@ def test_rows_that_overlap_are_copied():
         assert r.is_contiguous() and r.data_ptr() != t.data_ptr() and torch.equal(r, t)
     for t in (base, base[:, :3], base[::2, 1:], base[:1], base[0].expand(1, 4, 8)):
         assert _rows(t, 8) is t
+
+
+def test_top_k_beyond_32_bits():
+    """Any number of tokens that is more than there are keeps all of them, negative ones too; no bit of it is dropped."""
+    x = torch.arange(6.).repeat(4, 1)
+    noise = torch.ones(4, 6)
+    noise[:, 0] = 1e-9
+    for k in (2 ** 32 + 1, 2 ** 40 + 2, 2 ** 31, 6, 10 ** 18, -(2 ** 40) + 3, -1, 0):
+        assert ops.sample(x, noise, 1.0, k).tolist() == [0] * 4
+        assert ops.sample(x, noise, 1.0, torch.full((4,), k, dtype=torch.int64)).tolist() == [0] * 4
+    assert ops.sample(x, noise, 1.0, torch.tensor([1, 5, 6, 2 ** 33 + 1])).tolist() == [5, 5, 0, 0]
+    assert ops.sample(x, noise, 1.0, torch.tensor([1, 5, 6, 7], dtype=torch.uint8)).tolist() == [5, 5, 0, 0]
+    assert ops.sample(x, noise, 1.0, torch.tensor([1.0, 5.0, 6.0, 1e12])).tolist() == [5, 5, 0, 0]

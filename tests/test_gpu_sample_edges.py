@@ -63,3 +63,13 @@ def test_settings_that_are_nan(cuda_device, V, dtype, name, k):
         mixed, want = _both(x, noise, *({**others, name: rows}[n] for n in order))
         assert mixed[::2] == want[::2] == got[::2]
     assert mixed[1::2] == ops.sample(x, noise, *({**others, name: s[name]}[n] for n in order)).tolist()[1::2]
+
+
+def test_top_k_beyond_32_bits(cuda_device):
+    x, noise = _draws(4, 3000, 2)
+    for k in ([2 ** 32 + 1, 2 ** 40 + 2, 2 ** 31, -(2 ** 40) + 3], [1, 50, 2 ** 33 + 1, 0]):
+        rows = torch.tensor(k, device=cuda_device)
+        own = [x if 0 < x < 3000 else 0 for x in k]
+        want = ops.sample(x, noise, 1.0, torch.tensor(own, dtype=torch.int32, device=cuda_device)).tolist()
+        assert ops.sample(x, noise, 1.0, rows).tolist() == want
+        assert [ops.sample(x, noise, 1.0, n).tolist()[i] for i, n in enumerate(k)] == want
