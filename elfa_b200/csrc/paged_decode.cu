@@ -514,13 +514,15 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(const __grid_con
   }
 }
 
-constexpr int MIN_UNITS = 4 + paged_front<DBLK>;                       // no share lies within the empty ones
+// The number of CTAs is rounded up, so a share has at least half of these (15 units make shares of 8 and 7): it may lie within an item's empty units, and is a part
+// of nothing then.
+constexpr int MIN_UNITS = 4 + paged_front<DBLK>;
 
 int decode_grid(int hd) { return 148 * (hd <= 64 ? 2 : 1); }
-// CTAs per item (a cluster) where items are alike or cannot be long, 0 for the line of units. us, line against clusters (their size), 16 heads of 64: 1 sequence of 500 12.6, 10.6 (1);
-// of 2000 13.6, 10.8 (8); of 8000 15.7, 16.9 (8; the line's two launches and scratch cost the host 7 us more); of 32000 34, 42 (8); 4 of 1000 14.9, 10.8 (4); of 2000 15.3, 13.8 (4);
-// 8 of 2000 21, 18 (2); 16 of 500 17.1, 11.4 (1); of 1000 21.6, 17.1 (1); of 2000 35, 29 (1), but then, as among 4 of 8000, one long sequence among short ones would hold up
-// the others.
+// CTAs per item (a cluster) where items are alike or cannot be long, 0 for the line of units. us, line against clusters (their size), 16 heads of 64, in a graph (the GPU's part)
+// and as a call among others (the line has two launches and scratch for the host to see to): 1 sequence of 2000 11.2, 10.0 and 24, 13 (8); of 8000 12.8, 15.6 and 18, 18 (8); of
+// 10000 14.3, 17.9 and 18, 21 (8); 4 of 2000 12.8, 11.6 and 18, 14 (4); 16 of 1000 19.0, 14.2 and 22, 17 (1). So one sequence of 8000 to 10000 would be the line's by now, and from
+// 10240 on it is. 32000 keys: 34 and 42. 16 of 2000: 35 and 29, but then, as among 4 of 8000, one long sequence among short ones would hold up the others.
 int decode_whole(int B, int Hkv, int hd, int max_new, int rep, long long cache, int window, int sinks) {
   if ((long long)max_new * rep > DROWS) return 0;
   const long long items = (long long)B * Hkv, seen = (long long)window + max_new + sinks + 2 * DBLK, most = window && seen < cache ? seen : cache;
@@ -607,7 +609,8 @@ bool paged_units_fit(const PagedGeom& g, int block) {
 // Which calls go to the tiles of 2 x 128 rows, by the rows of a key head. 16-row tiles read the keys again for every 16 rows, 128-row tiles take as long for one row as for
 // all. us, 16-row tiles against 128-row tiles: 8 sequences of 3000, 16 heads of 128: 16 rows 49, 60; 24 rows 73, 60; 48 rows 97, 61. Heads of 64: 32 rows 45, 51; 48 rows 55, 51.
 // 32 of 2000, 32 heads on 8 of 128: 16 rows 59, 76; 24 rows 97, 78. One of 30000: 16 rows 42, 49; 24 rows 50, 50; 48 rows 67, 51. Where the bound is far above what most
-// sequences have (up to 32 rows, half of that on average) 16-row tiles would be the faster ones, 50 against 57 us; the host knows the bound only.
+// sequences have (up to 32 rows, half of that on average) 16-row tiles would be the faster ones, 50 against 57 us; the host knows the bound only. It is why
+// 64-wide heads change forms above 48 rows, where a call that has all of the bound's rows would at 48.
 static bool many_rows(int max_new, int rep, int hd) { return (long long)max_new * rep > (hd > 64 ? 16 : 48) && rep <= 128; }
 
 }  // namespace elfa

@@ -9,6 +9,7 @@
 //   warp 2      : clears the value rows behind a sequence's last token before they are multiplied (what lies there may be anything)
 //   warps 4-11  : softmax and sums of tile 0 and tile 1, a thread per row: the whole S row in registers, P as packed bf16 in tensor memory, where the product takes
 //                 it from (through shared memory P cost 160 of the 384 KB that a block moves there, 128 bytes a cycle), O in tensor memory
+// The softmax warps hold a whole S row, P's words and the sums at once: 416 bytes of spill stores, 588 of loads (600 with 64-wide heads).
 // Tensor memory: S 128 | P 2 x 64 | O 2 x HDP columns. Parts of items go to scratch in fp32 and are joined by a second launch. Every wait is bounded.
 //
 // 2048 tokens over 16384, 32 heads on 8 of 128: 443 to 520 us (box and power), 1000 to 1160 TFLOP/s; prompts of six users with a window of 1024, 40 heads on 8 of 128:

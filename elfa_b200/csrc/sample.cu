@@ -8,6 +8,8 @@
 // Sums are of fp32 weights, joined in fp32 or fp64; what decides between two tokens is fp32. Counts and places are integers, so a result does not depend on the order in
 // which threads come. Bound by latency where rows are few (a dozen meetings of a row's CTAs: one row of 32000, all filters, 20 us) and by the passes' instructions
 // where they are many: 96 rows of 131072, top-p, 75 us out of the L2 and 84 from memory, of a CTA's row maximum 12, counting 19, window 8, race 30, sort 5.
+// Where a nucleus ends is decided by sums of exponentials that are off by 2^-22 each: where its line passes within some 10^-6 of the mass of a token's edge either may be
+// the last.
 #include <math_constants.h>
 
 #include <type_traits>
@@ -40,7 +42,8 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 constexpr int ST = 512, SW = ST / 32;      // threads of a CTA
 constexpr int BINS = 8192, LIST = 4096;    // bins of width T / 256 below the maximum; tokens that are sorted
 constexpr float BINS_PER = 256.f;
-// Vectors of 16 bytes that a thread asks for at once, tokens of the race's batches: what 64 registers hold (twice as many of either cost 7 to 25 %).
+// Vectors of 16 bytes that a thread asks for at once, tokens of the race's batches: about what 64 registers hold (the kernel around the passes spills 162 bytes of fp32
+// rows, 34 of bf16 ones; twice as many of either cost 7 to 25 %).
 constexpr int EACH = 2, RACE = 8;
 
 // (key, index) as one number: larger is earlier in the order of falling logits, equal ones by index. Never 0.
@@ -818,7 +821,8 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
 template <typename T>
 int launch_sample(const SampleArgs& a, int B, cudaStream_t st) {
   // CTAs per row: while each has an SM of its own and 8192 logits, twice as many. Measured, us on 1, 2, 4, 8 (top-p, but for the 8192): 1 row of 131072: 65, 49, 38, 32;
-  // 40: 71, 53, 54, 72; 96: 74, 76, 89, 127; 120: 91, 80, 109, 163; 64 of 32000 bf16: 33, 32, 37, 66; 150 of 50000: 58, 73, 94, 153; 32 of 8192: 17, 19, 19, 23.
+  // 40: 71, 53, 54, 72; 96: 74, 76, 89, 127; 120: 91, 80, 109, 163; 64 of 32000 bf16: 33, 32, 37, 66; 150 of 50000: 58, 73, 94, 153; 32 of 8192: 17, 19, 19, 23. Where two CTAs
+  // would share SMs the sizes above differ in sign, and rows stay with one.
   int C = 1;
   while (C < 8 && a.V > 8192LL * C && (long long)B * C * 2 <= 148) C *= 2;
   ELFA_CUDA(allow_shared<sample_kernel<T>>((int)sizeof(SampleShared)));
