@@ -336,6 +336,13 @@ def embedding(ids: torch.Tensor, tok: torch.Tensor, pos: Optional[torch.Tensor] 
               vocab_lo: int = 0, seq_first: bool = False, vocab_total: int = 0) -> torch.Tensor:
     """``tok[ids - vocab_lo] (+ pos[pos0 + t])`` for ids inside this rank's vocabulary slice, zeros
     for the others (summing over vocabulary-parallel ranks gives the full embedding)."""
+    if tok.is_cuda:                      # the kernel reads 64-bit ids at an address of the device
+        if ids.get_device() != tok.get_device():
+            raise ValueError(f"embedding: ids on {ids.device}, the table on {tok.device}")
+        if ids.dtype is not torch.int64:
+            if ids.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
+                raise TypeError(f"embedding: ids must be whole numbers, got {ids.dtype}")
+            ids = ids.long()
     return _Embedding.apply(ids, tok, pos, pos0, vocab_lo, seq_first, vocab_total)
 
 

@@ -90,3 +90,24 @@ def test_what_kernels_record_is_raised(cuda_device, monkeypatch, step):
     assert len(calls) == 7 if step else len(calls) == 1            # the prompt's is known before anything is drawn from it
     monkeypatch.undo()
     assert len(gen.generate_batch([[5, 6, 7]], 7, temperature=0.0, samples=2)[0][1]) == 10
+
+
+@pytest.mark.parametrize("paged", [True, False])
+def test_ids_of_other_types_and_places(cuda_device, paged):
+    """Narrower whole numbers are taken for what they are; ids on the host and ids that are no whole numbers are refused before a kernel reads them."""
+    m = _model(2)
+    ids = torch.arange(40, 140)
+
+    def call(x):
+        if not paged:
+            return m(x[None])
+        cache = m.new_paged_cache(8, 32)
+        return m.forward_paged(x, [cache.add()], [100], cache)
+    with torch.no_grad():
+        want = call(ids.cuda())
+        for kind in (torch.int32, torch.int16, torch.uint8):
+            assert torch.equal(call(ids.to(kind).cuda()), want)
+        for bad in (ids, ids.int(), ids.cuda().float(), ids.cuda() > 50):
+            with pytest.raises((ValueError, TypeError)):
+                call(bad)
+    native.check_status()
