@@ -381,6 +381,13 @@ class GPTModel(nn.Module):
             raise ValueError(f"ids must hold the new tokens of all sequences, [{sum(new)}], got {tuple(ids.shape)}")
         if len(cache.pool) != len(self.blocks):
             raise ValueError(f"the cache has {len(cache.pool)} layers, the model {len(self.blocks)}")
+        # what the layers would refuse is refused here: behind `append` the cache counts tokens that nobody has written
+        at, pool, home = self.blocks[0].attn, cache.pool, self.embed_tokens
+        if (pool.shape[3], pool.shape[5], pool.dtype, pool.device) != (at.n_kv_heads, at.head_dim, home.dtype, home.device):
+            raise ValueError(f"the cache has {pool.shape[3]} heads of {pool.shape[5]}, {pool.dtype} on {pool.device}, "
+                             f"the model {at.n_kv_heads} of {at.head_dim}, {home.dtype} on {home.device}")
+        if ids.device != home.device or ids.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
+            raise ValueError(f"ids must be whole numbers on {home.device}, got {ids.dtype} on {ids.device}")
         if self.pos_embed is not None:
             end = max(cache.length(s) + n for s, n in zip(seqs, new))
             if end > self.pos_embed.shape[0]:

@@ -48,6 +48,8 @@ class PagedCache:
             raise ValueError(f"page_size must be one of {ops.PAGE_SIZES}, got {page_size}")
         if layers < 1 or pages < 1 or (window is not None and window < 1) or sinks < 0:
             raise ValueError("a cache has layers and pages, a window holds at least the token itself, and there are no negative sinks")
+        if torch.empty(0, device=device).is_cuda and (dtype is not torch.bfloat16 or head_dim % 8 or not 8 <= head_dim <= 128):
+            raise ValueError(f"a cache on the device holds bf16 and head dimensions that are multiples of 8 up to 128, got {dtype} and {head_dim}")
         self.pool = torch.zeros((layers, pages, 2, kv_heads, page_size, head_dim), dtype=dtype, device=device)
         self.page_size, self.window, self.sinks = page_size, window, sinks
         self._refs = [0] * pages

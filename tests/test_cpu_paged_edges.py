@@ -9,6 +9,7 @@ from elfa_b200 import ops
 from elfa_b200.config import Config
 from elfa_b200.eval import Generator
 from elfa_b200.models.gpt import GPTModel
+from elfa_b200.runtime.paged_cache import PagedCache
 
 from paged_cases import attend64, make
 
@@ -119,3 +120,22 @@ def test_top_k_beyond_32_bits():
     assert ops.sample(x, noise, 1.0, torch.tensor([1, 5, 6, 2 ** 33 + 1])).tolist() == [5, 5, 0, 0]
     assert ops.sample(x, noise, 1.0, torch.tensor([1, 5, 6, 7], dtype=torch.uint8)).tolist() == [5, 5, 0, 0]
     assert ops.sample(x, noise, 1.0, torch.tensor([1.0, 5.0, 6.0, 1e12])).tolist() == [5, 5, 0, 0]
+
+
+def test_a_call_that_is_refused_counts_no_token():
+    """Caches and ids that do not fit the model, and sequences that are not there: the cache is as it was."""
+    m = _model(True)
+    at, ids = m.blocks[0].attn, torch.zeros(3, dtype=torch.int64)
+    L, Hkv, hd = len(m.blocks), at.n_kv_heads, at.head_dim
+    for cache, bad in ((PagedCache(L + 1, 4, 16, Hkv, hd, torch.float32, "cpu"), ids), (PagedCache(L, 4, 16, Hkv * 2, hd, torch.float32, "cpu"), ids),
+                       (PagedCache(L, 4, 16, Hkv, hd + 8, torch.float32, "cpu"), ids), (PagedCache(L, 4, 16, Hkv, hd, torch.float64, "cpu"), ids),
+                       (m.new_paged_cache(4, 16), ids.float()), (m.new_paged_cache(4, 16), ids[:2]), (m.new_paged_cache(4, 16), ids.to("meta"))):
+        s = cache.add()
+        with pytest.raises(ValueError):
+            m.forward_paged(bad, [s], [3], cache)
+        assert cache.length(s) == 0 and cache.free_pages == 4
+    cache = m.new_paged_cache(4, 16)
+    s = cache.add()
+    with pytest.raises(KeyError):
+        m.forward_paged(ids, [s, 77], [2, 1], cache)
+    assert cache.length(s) == 0 and m.forward_paged(ids.int(), [s], [3], cache).shape[0] == 1

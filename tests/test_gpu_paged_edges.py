@@ -193,3 +193,11 @@ def test_broadcast_rows(cuda_device, new, H, Hkv, hd):
         ops.paged_write(d["k"], d["v"], d["pages"], d["table"], d["q_start"], d["kv_len"])
     assert torch.equal(b["pages"].view(torch.int16), own["pages"].view(torch.int16))
     assert torch.equal(_run(b), _run(own)) and close(_run(b), *attend64(own)) and native.status() == 0
+
+
+def test_a_cache_that_no_kernel_can_read_is_refused(cuda_device):
+    """When it is made, not by the first write, behind which it would count tokens that are not there."""
+    for bad in (dict(head_dim=136), dict(head_dim=60), dict(head_dim=0), dict(dtype=torch.float32), dict(dtype=torch.float16)):
+        with pytest.raises(ValueError, match="cache on the device"):
+            PagedCache(1, 4, 16, 1, **{"head_dim": 64, "device": cuda_device, **bad})
+    assert PagedCache(1, 4, 16, 1, 136, torch.float32, "cpu").free_pages == PagedCache(1, 4, 16, 1, 128, device=cuda_device).free_pages == 4
